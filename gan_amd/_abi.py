@@ -37,6 +37,24 @@ class GenWireSet(C.Structure):
                 [("proj_half", I64), ("cls", P), ("classes", I64), ("pair_logit", P), ("pair_bit", P)])
 
 
+class Sampling(C.Structure):
+    """Mirror of ``aig_sampling``."""
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", C.c_int32),
+                ("temperature_rows", P), ("top_p_rows", P), ("min_p_rows", P), ("top_k_rows", P)]
+
+
+class Distill(C.Structure):
+    """Mirror of ``aig_distill``."""
+    _fields_ = ([(n, I64) for n in ("rows", "width", "ld", "m")] + [("dtype", C.c_int32), ("temperature", C.c_float)] +
+                [(n, P) for n in ("logits", "counts", "values", "index", "lse", "weight")])
+
+
+class ScoreWindowsArg(C.Structure):
+    """Mirror of ``aig_score_windows``."""
+    _fields_ = ([(n, I64) for n in ("rows", "width", "nodes", "kinds", "classes")] +
+                [(n, P) for n in ("cand", "counts", "cls", "row_kind", "by_kind", "kind_start")])
+
+
 # name -> (restype, argtypes); every symbol of include/aig_abi.h appears here
 SIGNATURES = {
     "aig_abi_version": (INT, []),
@@ -131,6 +149,14 @@ SIGNATURES = {
     "aig_resync_typed_batch_ws_bytes": (SZ, [I64, I64, I64]),
     "aig_resync_typed_batch": (INT, [I64, I64, I64, P, P, P, P, P, P, P, SZ, P]),
     "aig_pad_batch": (INT, [I64, I64, I64, P, P, P, I64, P, P, P]),
+    "aig_sample_rows": (INT, [I64, I64, I64, INT, P, P, P, P, I64, P, P, P]),
+    "aig_top_rows": (INT, [I64, I64, I64, INT, P, P, I64, C.c_float, P, P, P, P]),
+    "aig_distill_rows": (INT, [P, P, P, I64, P, I64, P]),
+    "aig_sum_rows_ws_bytes": (SZ, [I64]),
+    "aig_sum_rows": (INT, [I64, P, C.c_float, P, P, SZ, P]),
+    "aig_class_scores": (INT, [P, P, P, P]),
+    "aig_class_scores_bwd_ws_bytes": (SZ, [I64, I64, I64]),
+    "aig_class_scores_bwd": (INT, [P, P, P, P, SZ, P]),
 }
 
 _lib = None

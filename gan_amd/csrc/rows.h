@@ -1,0 +1,167 @@
+// Rows of logits: what the kernels on them share (rows.hip, distill.hip).  A row is held by a GROUP of 16 or 64 lanes,
+// lane L of which owns the E consecutive places L*E .. L*E + E - 1 in registers, so that an order by place is an order by
+// lane: one scan over the group's lanes orders everything.  Sixteen lanes are one row of the vector unit's lane
+// permutations, so their sums and scans are vector instructions alone, for four rows of logits at once.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "common.h"
+
+namespace aig {
+int check_row_limits(const char* what, int64_t rows, int64_t width);      // rows.hip
+namespace rows {
+
+constexpr int MAX_WIDTH = AIG_ROWS_MAX_WIDTH;
+constexpr int NARROW = 1024;            // rows up to this width are held by a group's registers
+
+// ---------------------------------------------------------------- values
+// logits as f32, exactly, whatever they are stored in
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_float(__hip_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half(v); }
+template <> __device__ __forceinline__ __hip_bfloat16 from_float<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
+
+// Order of the logits as whole numbers: larger logit, larger key; 0 for a place that holds nothing (masked, NaN, past the
+// row's count).  The two zeros are one value (x + 0 turns the negative one over).
+__device__ __forceinline__ unsigned key_of(float v) {
+    const unsigned b = __float_as_uint(v + 0.0f);
+    return v > -__builtin_inff() ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 0u;
+}
+__device__ __forceinline__ float value_of(unsigned key) {
+    return key == 0u ? -__builtin_inff() : __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+}
+
+// ---------------------------------------------------------------- lane exchange
+// (DPP controls: row_shr:n = 0x110 + n moves a value n lanes up inside a row of 16, row_ror:n = 0x120 + n rotates it;
+//  lanes that nothing reaches get 0)
+template <int CTRL> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true); }
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)dpp<CTRL>((int)v); }
+template <int CTRL> __device__ __forceinline__ float dpp(float v) { return __int_as_float(dpp<CTRL>(__float_as_int(v))); }
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = dpp<CTRL>((int)(b & 0xFFFFFFFFll)), hi = dpp<CTRL>((int)(b >> 32));
+    return __longlong_as_double(((long long)hi << 32) | (unsigned)lo);
+}
+
+struct Add { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };
+struct Max { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
+struct Min { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a < b ? a : b; } };
+
+// v over the lanes of a group, in every lane of it
+template <int G, typename V, typename OP> __device__ __forceinline__ V all(V v, OP op) {
+    static_assert(G == 16 || G == 64, "groups of 16 or 64 lanes");
+    v = op(v, dpp<0x128>(v));
+    v = op(v, dpp<0x124>(v));
+    v = op(v, dpp<0x122>(v));
+    v = op(v, dpp<0x121>(v));
+    if (G == 64) {
+        v = op(v, __shfl_xor(v, 16));
+        v = op(v, __shfl_xor(v, 32));
+    }
+    return v;
+}
+// sum over the lanes of the group in front of this one
+template <int G, typename V> __device__ __forceinline__ V before(V v) {
+    V s = v;
+    s += dpp<0x111>(s);
+    s += dpp<0x112>(s);
+    s += dpp<0x114>(s);
+    s += dpp<0x118>(s);
+    if (G == 64) {
+        const V t0 = __shfl(s, 15), t1 = __shfl(s, 31), t2 = __shfl(s, 47);
+        const int row = lane_id() >> 4;
+        s += (row > 0 ? t0 : V(0)) + (row > 1 ? t1 : V(0)) + (row > 2 ? t2 : V(0));
+    }
+    return s - v;        // (whole numbers throughout: the subtraction is exact)
+}
+
+// ---------------------------------------------------------------- weights
+// A row's weights exp((l - max)/T) as whole multiples of 2^-36 of the largest: sums of up to 2^17 of them stay below 2^53
+// and are exact in f64 in whatever order they are taken - by lanes, by blocks, by atomics - so a draw is a function of its
+// row alone.  What is lost is a weight's 2^-37, far below the 2^-24 steps of the random numbers.
+constexpr double UNIT = 68719476736.0;          // 2^36
+// d = (l - max) log2(e) / T <= 0: rint(2^d UNIT).  2^f on |f| <= 1/2 by its series, the first term left out is below
+// 7e-15 (ln2^12 / (12! 2^12)), three decimal digits under the unit.
+__device__ __forceinline__ double weight_of(double d) {
+    d = fmax(d, -64.0);
+    const double n = __builtin_rint(d), f = d - n;
+    double p = 4.4455382718708110e-10;          // ln2^k / k!, k = 11 .. 0
+    p = fma(p, f, 7.0549116208011210e-09);
+    p = fma(p, f, 1.0178086009239696e-07);
+    p = fma(p, f, 1.3215486790144305e-06);
+    p = fma(p, f, 1.5252733804059838e-05);
+    p = fma(p, f, 1.5403530393381606e-04);
+    p = fma(p, f, 1.3333558146428441e-03);
+    p = fma(p, f, 9.6181291076284772e-03);
+    p = fma(p, f, 5.5504108664821576e-02);
+    p = fma(p, f, 2.4022650695910070e-01);
+    p = fma(p, f, 6.9314718055994531e-01);
+    p = fma(p, f, 1.0);
+    const long long scale = (long long)(1023 + 36 + (int)n) << 52;      // 2^(n + 36), n >= -64
+    return __builtin_rint(p * __longlong_as_double(scale));
+}
+constexpr double LOG2E = 1.4426950408889634;
+
+// ---------------------------------------------------------------- loading and selecting in registers
+// The E places of lane `lane` as keys; places from n on hold nothing and are not read (a vector may reach past n, never
+// past width).  vec: rows start on the alignment of a lane's E values (or of 16 bytes).
+template <int BYTES> struct Words;
+template <> struct Words<2> { typedef unsigned short type; };
+template <> struct Words<4> { typedef unsigned type; };
+template <> struct Words<8> { typedef uint2 type; };
+template <> struct Words<16> { typedef uint4 type; };
+template <typename T, int E> struct Places {
+    static constexpr int BYTES = E * (int)sizeof(T) < 16 ? E * (int)sizeof(T) : 16;
+    static constexpr int PER = BYTES / (int)sizeof(T);
+    typedef typename Words<BYTES>::type word;
+};
+template <typename T, int E>
+__device__ __forceinline__ void load_values(const T* __restrict__ row, int n, int width, bool vec, int lane, float (&v)[E]) {
+    typedef Places<T, E> P;
+    const int at = lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = -__builtin_inff();
+    if (at >= n) return;
+    if (vec && at + E <= width) {
+        union { typename P::word w[E / P::PER]; T t[E]; } u;
+#pragma unroll
+        for (int j = 0; j < E / P::PER; ++j) u.w[j] = reinterpret_cast<const typename P::word*>(row + at)[j];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = at + e < n ? as_float(u.t[e]) : -__builtin_inff();
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = at + e < n ? as_float(row[at + e]) : -__builtin_inff();
+    }
+}
+
+// The k largest of a group's keys, ties by place: those with key > thr, and of those with key == thr the first `quota`.
+// 0 < k < number of places that hold something.  The threshold is found a bit at a time.
+template <int G, int E>
+__device__ __forceinline__ void kth_largest(const unsigned (&key)[E], int k, unsigned& thr, int& quota) {
+    unsigned t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned c = t | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) n += key[e] >= c;
+        n = all<G>(n, Add());
+        if (n >= k) t = c;
+        if (n == k) {
+            thr = c - 1;
+            quota = 0;
+            return;
+        }
+    }
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) n += key[e] > t;
+    thr = t;
+    quota = k - all<G>(n, Add());
+}
+
+}  // namespace rows
+}  // namespace aig

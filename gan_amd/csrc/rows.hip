@@ -1,0 +1,657 @@
+// Operators on rows of logits: sampling from given random numbers, and the largest logits of a row.
+#include "rows.h"
+
+namespace aig {
+namespace {
+using namespace rows;
+
+struct Settings {       // of every row, or of each where a pointer is given
+    float temperature, top_p, min_p;
+    int top_k;
+    const float *temperature_rows, *top_p_rows, *min_p_rows;
+    const int* top_k_rows;
+};
+struct RowSettings {
+    float temperature, top_p, min_p;
+    int top_k;
+    __device__ __forceinline__ RowSettings(const Settings& s, long long r)
+        : temperature(s.temperature_rows ? s.temperature_rows[r] : s.temperature), top_p(s.top_p_rows ? s.top_p_rows[r] : s.top_p),
+          min_p(s.min_p_rows ? s.min_p_rows[r] : s.min_p), top_k(s.top_k_rows ? s.top_k_rows[r] : s.top_k) {}
+    // the smallest weight that min-p and the unit leave
+    __device__ __forceinline__ double floor() const { return min_p > 0.0f ? fmax((double)fminf(min_p, 1.0f) * UNIT, 1.0) : 1.0; }
+    // the mass that top-p keeps of `total`: a place stays while the mass in front of it is below this; the first always does
+    __device__ __forceinline__ double mass(double total) const { return fmax((double)top_p * total, 1.0); }
+};
+
+struct SampleRows {
+    long long rows, ld;
+    int width, draws, vec, fill;
+    long long period;           // counts and want are shared by rows a period apart (0: every row has its own)
+    const int *counts, *want;
+    const float* u;
+    int* out;
+    Settings how;
+    __device__ __forceinline__ long long plan_row(long long r) const { return period ? r % period : r; }
+    __device__ __forceinline__ int count(long long r) const { return counts ? min(max(counts[plan_row(r)], 0), width) : width; }
+    __device__ __forceinline__ int wanted(long long r) const { return want ? min(want[plan_row(r)], draws) : draws; }
+    __device__ __forceinline__ double uniform(long long r, int d) const {
+        return fmin(fmax((double)u[r * draws + d], 0.0), 1.0 - 1.0 / 16777216.0);
+    }
+    // the d-th pick of row r (-1: none).  For wiring every fan-in needs an answer: the first pick stands in for a missing
+    // second one, the row's last place for a missing first.
+    __device__ __forceinline__ void store(long long r, int d, int pick, int& first, int n) const {
+        if (fill) {
+            if (d == 0) first = pick < 0 ? n - 1 : pick;
+            if (pick < 0) pick = first;
+        }
+        out[r * draws + d] = pick;
+    }
+};
+
+// A group of G lanes per row, the row in registers.
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleRows a) {
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
+    if (r >= a.rows) return;
+    const int lane = threadIdx.x & (G - 1);
+    const RowSettings how(a.how, r);
+    const int n = a.count(r), want = a.wanted(r);
+    float v[E];
+    load_values<T, E>(x + r * a.ld, n, a.width, a.vec, lane, v);
+    unsigned key[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = key_of(v[e]);
+    int first = -1;
+
+    if (!(how.temperature > 0.0f)) {      // the largest, then the next
+        for (int d = 0; d < a.draws; ++d) {
+            unsigned best = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) best = max(best, key[e]);
+            best = all<G>(best, Max());
+            int at = 0x7FFFFFFF;
+#pragma unroll
+            for (int e = E - 1; e >= 0; --e) at = key[e] == best ? lane * E + e : at;
+            at = all<G>(at, Min());
+#pragma unroll
+            for (int e = 0; e < E; ++e) key[e] = lane * E + e == at ? 0u : key[e];
+            if (lane == 0) a.store(r, d, best != 0u && d < want ? at : -1, first, n);
+        }
+        return;
+    }
+
+    unsigned top = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = max(top, key[e]);
+    top = all<G>(top, Max());
+    const double m = (double)value_of(top), per = LOG2E / (double)how.temperature;
+    double q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        q[e] = key[e] == top ? UNIT : weight_of(((double)value_of(key[e]) - m) * per);
+        q[e] = key[e] == 0u ? 0.0 : q[e];
+    }
+
+    int held = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) held += key[e] != 0u;
+    held = all<G>(held, Add());
+    if (how.top_k > 0 && how.top_k < held) {
+        unsigned thr;
+        int quota;
+        kth_largest<G, E>(key, how.top_k, thr, quota);
+        int ties = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) ties += key[e] == thr;
+        int tie = before<G>(ties);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool stays = key[e] > thr || (key[e] == thr && tie < quota);
+            tie += key[e] == thr;
+            q[e] = stays ? q[e] : 0.0;
+        }
+    }
+    if (how.top_p < 1.0f) {
+        double total = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) total += q[e];
+        const double p = how.mass(all<G>(total, Add()));
+        // the largest key whose place and everything above it hold mass p: the border
+        unsigned t = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const unsigned c = t | (1u << bit);
+            double w = 0.0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) w += key[e] >= c ? q[e] : 0.0;
+            if (all<G>(w, Add()) >= p) t = c;
+        }
+        double above = 0.0;
+        int ties = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            above += key[e] > t ? q[e] : 0.0;
+            ties += key[e] == t;
+        }
+        above = all<G>(above, Add());
+        int tie = before<G>(ties);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool stays = key[e] > t || (key[e] == t && above + (double)tie * q[e] < p);
+            tie += key[e] == t;
+            q[e] = stays ? q[e] : 0.0;
+        }
+    }
+    const double least = how.floor();
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[e] = q[e] >= least ? q[e] : 0.0;
+
+    for (int d = 0; d < a.draws; ++d) {
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += q[e];
+        const double total = all<G>(sum, Add());
+        double upto = before<G>(sum);
+        const double t = a.uniform(r, d) * total;
+        int at = -1;                       // one lane's range holds t (none: nothing is left)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const double next = upto + q[e];
+            const bool here = upto <= t && t < next;
+            at = here ? lane * E + e : at;
+            q[e] = here ? 0.0 : q[e];
+            upto = next;
+        }
+        at = all<G>(at, Max());
+        if (lane == 0) a.store(r, d, d < want ? at : -1, first, n);
+    }
+}
+
+// ---------------------------------------------------------------- wide rows: a workgroup per row
+constexpr int WIDE_T = 1024, WIDE_E = 8, TILE = WIDE_T * WIDE_E, TILES = MAX_WIDTH / TILE;
+
+struct Block {          // sums and scans over the sixteen waves of a workgroup
+    double* d;          // [17]
+    template <typename V, typename OP> __device__ __forceinline__ V all(V v, OP op) const {
+        V* s = reinterpret_cast<V*>(d);
+        v = rows::all<64>(v, op);
+        __syncthreads();
+        if (lane_id() == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        V t = s[0];
+#pragma unroll
+        for (int w = 1; w < WIDE_T / 64; ++w) t = op(t, s[w]);
+        return t;
+    }
+    // sum over the threads in front of this one; total over all
+    template <typename V> __device__ __forceinline__ V before(V v, V& total) const {
+        V* s = reinterpret_cast<V*>(d);
+        const V mine = rows::before<64>(v);
+        __syncthreads();
+        if (lane_id() == 63) s[threadIdx.x >> 6] = mine + v;
+        __syncthreads();
+        V front = V(0);
+        total = V(0);
+#pragma unroll
+        for (int w = 0; w < WIDE_T / 64; ++w) {
+            front += w < (int)(threadIdx.x >> 6) ? s[w] : V(0);
+            total += s[w];
+        }
+        return front + mine;
+    }
+};
+
+// The largest key such that it and everything above it amount to `target` (AMOUNT of a place: 1, or its weight): eight bits
+// at a time, a histogram over the places that share the bits found so far.  above: what the keys over it amount to.
+// The sums are of whole numbers below 2^53: exact, in any order of the atomics.
+template <typename KEY, typename AMOUNT>
+__device__ __forceinline__ unsigned border_key(int n, double target, double* hist, double* found, KEY key, AMOUNT amount, double& above) {
+    unsigned prefix = 0, mask = 0;
+    above = 0.0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        if (threadIdx.x < 256) hist[threadIdx.x] = 0.0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += WIDE_T) {
+            const unsigned k = key(i);
+            if (k != 0u && (k & mask) == prefix) unsafeAtomicAdd(&hist[(k >> shift) & 255u], amount(k, i));
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int hi = 255 - 4 * threadIdx.x;
+            const double h[4] = {hist[hi], hist[hi - 1], hist[hi - 2], hist[hi - 3]};
+            double upto = above + rows::before<64>(h[0] + h[1] + h[2] + h[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double next = upto + h[j];
+                if (upto < target && target <= next) {
+                    found[0] = (double)(hi - j);
+                    found[1] = upto;
+                }
+                upto = next;
+            }
+        }
+        __syncthreads();
+        prefix |= (unsigned)found[0] << shift;
+        mask |= 255u << shift;
+        above = found[1];
+    }
+    return prefix;
+}
+
+template <typename T>
+__global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x, SampleRows a) {
+    __shared__ double hist[256], found[2], red[WIDE_T / 64 + 1], tile_mass[TILES];
+    __shared__ int tile_ties[TILES], picked[8];
+    const Block block{red};
+    const long long r = blockIdx.x;
+    const RowSettings how(a.how, r);
+    const int n = a.count(r), want = a.wanted(r);
+    x += r * a.ld;
+    auto key = [&](int i) { return key_of(as_float(x[i])); };
+    int first = -1;
+
+    if (!(how.temperature > 0.0f)) {
+        for (int d = 0; d < a.draws; ++d) {
+            unsigned best = 0;
+            int at = 0x7FFFFFFF;
+            for (int i = threadIdx.x; i < n; i += WIDE_T) {
+                unsigned k = key(i);
+                for (int j = 0; j < d; ++j) k = picked[j] == i ? 0u : k;
+                if (k > best) { best = k; at = i; }
+            }
+            const unsigned top = block.all(best, Max());
+            at = block.all(best == top ? at : 0x7FFFFFFF, Min());
+            const int pick = top != 0u && d < want ? at : -1;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                picked[d] = top != 0u ? at : -1;
+                a.store(r, d, pick, first, n);
+            }
+            __syncthreads();
+        }
+        return;
+    }
+
+    unsigned top = 0;
+    int held = 0;
+    for (int i = threadIdx.x; i < n; i += WIDE_T) {
+        const unsigned k = key(i);
+        top = max(top, k);
+        held += k != 0u;
+    }
+    top = block.all(top, Max());
+    held = block.all(held, Add());
+    const double m = (double)value_of(top), per = LOG2E / (double)how.temperature;
+    auto weight = [&](unsigned k) { return k == 0u ? 0.0 : k == top ? UNIT : weight_of(((double)value_of(k) - m) * per); };
+
+    // what top-k keeps: keys over kthr, and the first kquota at it
+    unsigned kthr = 0;
+    int kquota = 0;
+    if (how.top_k > 0 && how.top_k < held) {
+        double above;
+        kthr = border_key(n, (double)how.top_k, hist, found, key, [](unsigned, int) { return 1.0; }, above);
+        kquota = how.top_k - (int)above;
+    }
+    unsigned pthr = 0;
+    double pabove = 0.0, p = 0.0;
+    if (how.top_p < 1.0f) {
+        double over = 0.0;         // the mass of the keys over top-k's border; the border itself keeps its quota
+        for (int i = threadIdx.x; i < n; i += WIDE_T) {
+            const unsigned k = key(i);
+            over += k > kthr ? weight(k) : 0.0;
+        }
+        over = block.all(over, Add());
+        p = how.mass(over + (double)kquota * weight(kthr));
+        if (over >= p) {           // (else the border is top-k's)
+            const unsigned lowest = kthr;
+            pthr = border_key(n, p, hist, found, [&](int i) { const unsigned k = key(i); return k > lowest ? k : 0u; },
+                              [&](unsigned k, int) { return weight(k); }, pabove);
+        } else {
+            pthr = kthr;
+            pabove = over;
+        }
+    }
+    const double least = how.floor();
+    // the weight of a place that is the tie-th of its key's (place order) where its key is a border
+    auto kept = [&](unsigned k, int ktie, int ptie) {
+        double q = weight(k);
+        if (k < kthr || (k == kthr && ktie >= kquota)) q = 0.0;
+        if (p > 0.0 && (k < pthr || (k == pthr && !(pabove + (double)ptie * q < p)))) q = 0.0;
+        return q >= least ? q : 0.0;
+    };
+    // ties in front of a place are counted for the higher of the two borders only: at the lower one everything is gone
+    const unsigned border = max(kthr, pthr);
+
+    // the mass of each tile of places, and the ties in front of it
+    double total = 0.0;
+    int tiles = (n + TILE - 1) / TILE, ties_so_far = 0;
+    auto tile_places = [&](int t, int front, double (&q)[WIDE_E], int& ties_here) {
+        const int base = t * TILE + (int)threadIdx.x * WIDE_E;
+        unsigned k[WIDE_E];
+        int ties = 0;
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e) {
+            k[e] = base + e < n ? key(base + e) : 0u;
+            ties += k[e] == border && border != 0u;
+        }
+        int tie = front + block.before(ties, ties_here);
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e) {
+            q[e] = kept(k[e], tie, tie);
+            tie += k[e] == border && border != 0u;
+        }
+    };
+    for (int t = 0; t < tiles; ++t) {
+        double q[WIDE_E], sum = 0.0;
+        int ties_here;
+        tile_places(t, ties_so_far, q, ties_here);
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e) sum += q[e];
+        sum = block.all(sum, Add());
+        if (threadIdx.x == 0) {
+            tile_mass[t] = sum;
+            tile_ties[t] = ties_so_far;
+        }
+        total += sum;
+        ties_so_far += ties_here;
+    }
+    __syncthreads();
+
+    for (int d = 0; d < a.draws; ++d) {
+        if (!(total > 0.0)) {
+            if (threadIdx.x == 0) a.store(r, d, -1, first, n);
+            continue;
+        }
+        const double t = a.uniform(r, d) * total;
+        int tile = 0;
+        double front = 0.0;
+        while (tile + 1 < tiles && front + tile_mass[tile] <= t) front += tile_mass[tile++];
+        double q[WIDE_E], sum = 0.0, all_mass;
+        int ties_here;
+        tile_places(tile, tile_ties[tile], q, ties_here);
+        const int base = tile * TILE + (int)threadIdx.x * WIDE_E;
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e) {
+            for (int j = 0; j < d; ++j) q[e] = picked[j] == base + e ? 0.0 : q[e];
+            sum += q[e];
+        }
+        double upto = front + block.before(sum, all_mass);
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e) {
+            const double next = upto + q[e];
+            if (upto <= t && t < next) {
+                picked[d] = base + e;
+                tile_mass[tile] -= q[e];
+                found[0] = q[e];
+            }
+            upto = next;
+        }
+        __syncthreads();
+        total -= found[0];
+        if (threadIdx.x == 0) a.store(r, d, d < want ? picked[d] : -1, first, n);
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- the largest logits
+struct TopArgs {
+    long long rows, ld;
+    int width, m, vec;
+    const int* counts;
+    float temperature;
+    float* values;
+    int* index;
+    float* lse;
+    __device__ __forceinline__ int count(long long r) const { return counts ? min(max(counts[r], 0), width) : width; }
+};
+constexpr int TOP_MAX = AIG_ROWS_MAX_TOP;
+
+// Orders `have` kept places (key, place; place order) and writes them, the rest of the m entries as absent: a place's rank is
+// the number of places in front of it.
+template <int THREADS>
+__device__ __forceinline__ void write_ranked(const TopArgs& a, long long r, const unsigned* key, const int* place, int have, int t) {
+    for (int j = t; j < a.m; j += THREADS) {
+        if (j >= have) {
+            a.values[r * a.m + j] = -__builtin_inff();
+            a.index[r * a.m + j] = -1;
+            continue;
+        }
+        const unsigned k = key[j];
+        int rank = 0;
+        for (int i = 0; i < have; ++i) rank += key[i] > k || (key[i] == k && i < j);
+        a.values[r * a.m + rank] = value_of(k);
+        a.index[r * a.m + rank] = place[j];
+    }
+}
+
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a) {
+    extern __shared__ unsigned lds[];            // per group: m keys, m places
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
+    if (r >= a.rows) return;
+    const int lane = threadIdx.x & (G - 1);
+    unsigned* lkey = lds + (size_t)(threadIdx.x / G) * 2 * a.m;
+    int* lplace = reinterpret_cast<int*>(lkey + a.m);
+    const int n = a.count(r);
+    float v[E];
+    load_values<T, E>(x + r * a.ld, n, a.width, a.vec, lane, v);
+    unsigned key[E], top = 0;
+    int held = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        key[e] = key_of(v[e]);
+        top = max(top, key[e]);
+        held += key[e] != 0u;
+    }
+    top = all<G>(top, Max());
+    held = all<G>(held, Add());
+    unsigned thr = 0;
+    int quota = 0;
+    if (a.m < held) kth_largest<G, E>(key, a.m, thr, quota);
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ties += key[e] == thr;
+    int tie = before<G>(ties), mine = 0;
+    bool stays[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        stays[e] = key[e] > thr || (key[e] != 0u && key[e] == thr && tie < quota);
+        tie += key[e] == thr;
+        mine += stays[e];
+    }
+    int at = before<G>(mine);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (stays[e]) {
+            lkey[at] = key[e];
+            lplace[at++] = lane * E + e;
+        }
+    const float m = value_of(top), per = (float)(LOG2E / (double)a.temperature);
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += key[e] == 0u ? 0.0f : key[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(key[e]) - m) * per);
+    s = all<G>(s, Add());
+    if (lane == 0) a.lse[r] = top == 0u ? -__builtin_inff() : m / a.temperature + logf(s);
+    // (the group's own wave wrote the list: its lanes see it once their writes are through)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    write_ranked<G>(a, r, lkey, lplace, min(a.m, held), lane);
+}
+
+template <typename T>
+__global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, TopArgs a) {
+    __shared__ double hist[256], found[2], red[WIDE_T / 64 + 1];
+    __shared__ unsigned lkey[TOP_MAX];
+    __shared__ int lplace[TOP_MAX];
+    const Block block{red};
+    const long long r = blockIdx.x;
+    const int n = a.count(r);
+    x += r * a.ld;
+    auto key = [&](int i) { return key_of(as_float(x[i])); };
+    unsigned top = 0;
+    int held = 0;
+    for (int i = threadIdx.x; i < n; i += WIDE_T) {
+        const unsigned k = key(i);
+        top = max(top, k);
+        held += k != 0u;
+    }
+    top = block.all(top, Max());
+    held = block.all(held, Add());
+    unsigned thr = 0;
+    int quota = 0;
+    if (a.m < held) {
+        double above;
+        thr = border_key(n, (double)a.m, hist, found, key, [](unsigned, int) { return 1.0; }, above);
+        quota = a.m - (int)above;
+    }
+    const float m = value_of(top), per = (float)(LOG2E / (double)a.temperature);
+    float s = 0.0f;
+    int ties_so_far = 0, kept_so_far = 0;
+    for (int t = 0; t * TILE < n; ++t) {
+        const int base = t * TILE + (int)threadIdx.x * WIDE_E;
+        unsigned k[WIDE_E];
+        int ties = 0, mine = 0, ties_here, kept_here;
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e) {
+            k[e] = base + e < n ? key(base + e) : 0u;
+            ties += thr != 0u && k[e] == thr;
+            s += k[e] == 0u ? 0.0f : k[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(k[e]) - m) * per);
+        }
+        int tie = ties_so_far + block.before(ties, ties_here);
+        bool stays[WIDE_E];
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e) {
+            stays[e] = k[e] > thr || (k[e] != 0u && k[e] == thr && tie < quota);
+            tie += thr != 0u && k[e] == thr;
+            mine += stays[e];
+        }
+        int at = kept_so_far + block.before(mine, kept_here);
+#pragma unroll
+        for (int e = 0; e < WIDE_E; ++e)
+            if (stays[e] && at < TOP_MAX) {
+                lkey[at] = k[e];
+                lplace[at++] = base + e;
+            }
+        ties_so_far += ties_here;
+        kept_so_far += kept_here;
+    }
+    s = block.all(s, Add());
+    if (threadIdx.x == 0) a.lse[r] = top == 0u ? -__builtin_inff() : m / a.temperature + logf(s);
+    __syncthreads();
+    write_ranked<WIDE_T>(a, r, lkey, lplace, min(a.m, held), threadIdx.x);
+}
+
+// ---------------------------------------------------------------- launches
+template <typename T> int sample_rows(hipStream_t s, const T* x, SampleRows a) {
+    // (a lane reads its places as vectors where every row starts on their alignment)
+    auto vec = [&](int e) {
+        const size_t align = e * sizeof(T) < 16 ? e * sizeof(T) : 16;
+        return (int)(reinterpret_cast<uintptr_t>(x) % align == 0 && (a.ld * sizeof(T)) % align == 0);
+    };
+    auto blocks = [&](int g) { return dim3((unsigned)((a.rows * g + 255) / 256)); };
+    if (a.width <= 64) {
+        a.vec = vec(4);
+        hipLaunchKernelGGL((k_sample<T, 16, 4>), blocks(16), dim3(256), 0, s, x, a);
+    } else if (a.width <= 256) {
+        a.vec = vec(16);
+        hipLaunchKernelGGL((k_sample<T, 16, 16>), blocks(16), dim3(256), 0, s, x, a);
+    } else if (a.width <= 512) {
+        a.vec = vec(8);
+        hipLaunchKernelGGL((k_sample<T, 64, 8>), blocks(64), dim3(256), 0, s, x, a);
+    } else if (a.width <= NARROW) {
+        a.vec = vec(16);
+        hipLaunchKernelGGL((k_sample<T, 64, 16>), blocks(64), dim3(256), 0, s, x, a);
+    } else {
+        hipLaunchKernelGGL(k_sample_wide<T>, dim3((unsigned)a.rows), dim3(WIDE_T), 0, s, x, a);
+    }
+    AIG_LAUNCH_CHECK();
+    return AIG_OK;
+}
+
+template <typename T> int top_rows(hipStream_t s, const T* x, TopArgs a) {
+    auto vec = [&](int e) {
+        const size_t align = e * sizeof(T) < 16 ? e * sizeof(T) : 16;
+        return (int)(reinterpret_cast<uintptr_t>(x) % align == 0 && (a.ld * sizeof(T)) % align == 0);
+    };
+    auto blocks = [&](int g) { return dim3((unsigned)((a.rows * g + 255) / 256)); };
+    auto lds = [&](int g) { return (size_t)(256 / g) * 2 * a.m * 4; };      // at most 32 KB
+    if (a.width <= 64) {
+        a.vec = vec(4);
+        hipLaunchKernelGGL((k_top<T, 16, 4>), blocks(16), dim3(256), lds(16), s, x, a);
+    } else if (a.width <= 256) {
+        a.vec = vec(16);
+        hipLaunchKernelGGL((k_top<T, 16, 16>), blocks(16), dim3(256), lds(16), s, x, a);
+    } else if (a.width <= 512) {
+        a.vec = vec(8);
+        hipLaunchKernelGGL((k_top<T, 64, 8>), blocks(64), dim3(256), lds(64), s, x, a);
+    } else if (a.width <= NARROW) {
+        a.vec = vec(16);
+        hipLaunchKernelGGL((k_top<T, 64, 16>), blocks(64), dim3(256), lds(64), s, x, a);
+    } else {
+        hipLaunchKernelGGL(k_top_wide<T>, dim3((unsigned)a.rows), dim3(WIDE_T), 0, s, x, a);
+    }
+    AIG_LAUNCH_CHECK();
+    return AIG_OK;
+}
+}  // namespace
+
+// (also the wiring's: every slot of a set of graphs gets an answer)
+int launch_sample_rows(hipStream_t s, int64_t rows, int64_t width, int64_t ld, int dtype, const void* logits, const int32_t* counts,
+                       const int32_t* want, int64_t period, const aig_sampling* how, int64_t draws, const float* u, bool fill,
+                       int32_t* out) {
+    SampleRows a{};
+    a.rows = rows; a.ld = ld; a.width = (int)width; a.draws = (int)draws; a.fill = fill; a.period = period;
+    a.counts = counts; a.want = want; a.u = u; a.out = out;
+    a.how = Settings{how->temperature, how->top_p, how->min_p, how->top_k, how->temperature_rows, how->top_p_rows,
+                     how->min_p_rows, how->top_k_rows};
+    if (dtype == AIG_F32) return sample_rows(s, static_cast<const float*>(logits), a);
+    if (dtype == AIG_F16) return sample_rows(s, static_cast<const __half*>(logits), a);
+    return sample_rows(s, static_cast<const __hip_bfloat16*>(logits), a);
+}
+}  // namespace aig
+
+using namespace aig;
+
+int aig::check_row_limits(const char* what, int64_t rows, int64_t width) {
+    if (width > AIG_ROWS_MAX_WIDTH) return fail(AIG_ELIMIT, "%s: rows of %lld: at most %d", what, (long long)width, AIG_ROWS_MAX_WIDTH);
+    // (a launch has fewer than 2^32 threads: a wave a row, a workgroup of 1024 for rows beyond a wave's registers)
+    const int64_t most = width <= rows::NARROW ? (1ll << 26) - 1 : (1ll << 22) - 1;
+    if (rows > most) return fail(AIG_ELIMIT, "%s: %lld rows of %lld: at most %lld", what, (long long)rows, (long long)width, (long long)most);
+    return AIG_OK;
+}
+
+static int check_rows(const char* what, int64_t rows, int64_t width, int64_t ld, int dtype) {
+    AIG_REQUIRE(rows >= 0 && width >= 1 && ld >= 0, "%s: bad sizes rows=%lld width=%lld ld=%lld", what, (long long)rows,
+                (long long)width, (long long)ld);
+    AIG_REQUIRE(dtype == AIG_F32 || dtype == AIG_F16 || dtype == AIG_BF16, "%s: unknown dtype %d", what, dtype);
+    return check_row_limits(what, rows, width);
+}
+
+extern "C" int aig_sample_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const void* logits, const int32_t* counts,
+                               const int32_t* want, const aig_sampling* how, int64_t draws, const float* u, int32_t* out,
+                               void* stream) {
+    if (const int rc = check_rows("aig_sample_rows", rows, width, ld, dtype)) return rc;
+    AIG_REQUIRE(draws >= 1 && draws <= AIG_ROWS_MAX_DRAWS, "aig_sample_rows: draws=%lld is not in 1..%d", (long long)draws,
+                AIG_ROWS_MAX_DRAWS);
+    AIG_REQUIRE(how, "aig_sample_rows: null settings");
+    if (rows == 0) return AIG_OK;
+    AIG_REQUIRE(logits && u && out, "aig_sample_rows: null pointer");
+    return launch_sample_rows(static_cast<hipStream_t>(stream), rows, width, ld, dtype, logits, counts, want, 0, how, draws, u,
+                              false, out);
+}
+
+extern "C" int aig_top_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const void* logits, const int32_t* counts,
+                            int64_t m, float temperature, float* values, int32_t* index, float* lse, void* stream) {
+    if (const int rc = check_rows("aig_top_rows", rows, width, ld, dtype)) return rc;
+    AIG_REQUIRE(m >= 1 && m <= AIG_ROWS_MAX_TOP, "aig_top_rows: m=%lld is not in 1..%d", (long long)m, AIG_ROWS_MAX_TOP);
+    AIG_REQUIRE(temperature > 0.0f, "aig_top_rows: the temperature must be positive");
+    if (rows == 0) return AIG_OK;
+    AIG_REQUIRE(logits && values && index && lse, "aig_top_rows: null pointer");
+    TopArgs a{};
+    a.rows = rows; a.ld = ld; a.width = (int)width; a.m = (int)m; a.counts = counts; a.temperature = temperature;
+    a.values = values; a.index = index; a.lse = lse;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == AIG_F32) return top_rows(s, static_cast<const float*>(logits), a);
+    if (dtype == AIG_F16) return top_rows(s, static_cast<const __half*>(logits), a);
+    return top_rows(s, static_cast<const __hip_bfloat16*>(logits), a);
+}

@@ -659,6 +659,101 @@ int aig_pad_batch(int64_t B, int64_t n, int64_t ecap, const int32_t* ecount, con
                   const int64_t* edge_attr, int64_t max_edges, int64_t* out_edge_index, int64_t* out_edge_attr,
                   void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Rows of logits: sampling, a teacher's top logits, distillation, scores by class
+ *
+ * A row is the logits of one slot's candidate window (the logits of aig_gen_score) or any other row of logits: `rows`
+ * rows of `width` places, row r at logits + r*ld elements (f32, IEEE halfs or bf16), of which the first counts[r] are
+ * valid (counts NULL: all; a count outside 0..width is taken as the nearer bound).  A valid place holds nothing when
+ * its logit is -inf; what lies past a row's count is never read as a value.  Widths to AIG_ROWS_MAX_WIDTH; rows of up
+ * to 1024 places are held in registers, wider ones are a workgroup's each.  The reference has none of these
+ * (its generator takes torch.topk, models/generator.py:162-168, and never receives a gradient, train.py:297-299).
+ * ------------------------------------------------------------------------------------------- */
+#define AIG_F32 0
+#define AIG_F16 1
+#define AIG_BF16 2
+#define AIG_ROWS_MAX_WIDTH 131072
+#define AIG_ROWS_MAX_DRAWS 8
+#define AIG_ROWS_MAX_TOP 256
+#define AIG_MAX_CLASSES 1024
+#define AIG_MAX_KINDS 1048576
+
+/* Settings of a draw: one value for all rows, or an array with one a row (not NULL: it counts). */
+typedef struct aig_sampling {
+    float temperature;    /* > 0; anything else: the largest logit, then the next (equal ones: lowest place) */
+    float top_p;          /* >= 1: off */
+    float min_p;          /* <= 0: off; above 1 counts as 1 */
+    int32_t top_k;        /* <= 0: off */
+    const float *temperature_rows, *top_p_rows, *min_p_rows;
+    const int32_t* top_k_rows;
+} aig_sampling;
+
+/* Draws positions of each row without replacement, from given random numbers.  With m the row's largest logit:
+ *   weights q_i = rint(2^36 exp((l_i - m) / temperature)), 0 for NaN and -inf; in order of (logit, then lowest place):
+ *   top_k keeps the first k; top_p keeps a place while the weights in front of it sum to less than top_p times the sum of
+ *   what top_k kept (the first place always); min_p keeps q_i >= min_p 2^36
+ *   draw d: t = u[r*draws + d] * (sum of the weights left), the lowest place with sum of weights up to and with it > t; it
+ *   is taken out.  u in [0, 1) (values outside are taken as the nearer end, NaN as 0).
+ *   out[r*draws + d] = place, -1 where nothing is left or d >= want[r] (want NULL: all draws)
+ * Weights are whole numbers whose sums are exact in f64, so a row's picks depend on nothing but the row. */
+int aig_sample_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const void* logits, const int32_t* counts,
+                    const int32_t* want, const aig_sampling* how, int64_t draws, const float* u, int32_t* out,
+                    void* stream);
+
+/* The m largest logits of each row (NaN and -inf never), largest first, equal ones by lowest place:
+ *   values [rows,m] f32, index [rows,m] (places; absent entries -inf and -1), lse[r] = log sum exp(l / temperature)
+ *   over the row's valid places (-inf for none) - what aig_distill_rows takes of a teacher. */
+int aig_top_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const void* logits, const int32_t* counts, int64_t m,
+                 float temperature, float* values, int32_t* index, float* lse, void* stream);
+
+/* Distillation.  y = l / T over a student row's valid places, p = softmax(y); the teacher's row gives m entries (logit t_j,
+ * place i_j; an entry whose place is not one of the row's, or whose logit is -inf, is absent), q_j = exp(t_j/T - lse[r]) -
+ * with lse NULL the log-sum-exp of the entries themselves.
+ *   loss[r] = weight[r] T^2 ( sum_j q_j (log q_j - log p[i_j]) + q_R (log q_R - log p_R) )
+ *   grad    = dloss[r]/dl, times upstream[r * upstream_stride] when given (stride 0: one factor for all rows)
+ * R: the valid places no entry names, taken as one outcome with the teacher's remaining q_R = 1 - sum_j q_j (with lse
+ * given and R not empty; else left out).  A row without valid places or entries: loss 0, gradient 0.  Places past a row's
+ * count get gradient 0.  Entries may name a place more than once.  lse must be the teacher's row's own at the same T
+ * (a smaller one makes sum q_j exceed 1; each q_j is held to 1).
+ * loss or grad may be NULL (not both); grad [rows, grad_ld >= width] in the logits' type, not overlapping them. */
+typedef struct aig_distill {
+    int64_t rows, width, ld, m;
+    int32_t dtype;
+    float temperature;            /* positive, finite */
+    const void* logits;
+    const int32_t* counts;        /* may be NULL */
+    const float* values;          /* [rows,m] */
+    const int32_t* index;         /* [rows,m] */
+    const float* lse;             /* [rows] or NULL */
+    const float* weight;          /* [rows] or NULL (ones) */
+} aig_distill;
+int aig_distill_rows(const aig_distill* d, float* loss, void* grad, int64_t grad_ld, const float* upstream,
+                     int64_t upstream_stride, void* stream);
+
+/* out[0] = factor * sum of v[0..rows), taken in f64 in an order that depends on rows alone */
+size_t aig_sum_rows_ws_bytes(int64_t rows);
+int aig_sum_rows(int64_t rows, const float* v, float factor, float* out, void* ws, size_t ws_bytes, void* stream);
+
+/* Candidate logits by class (nodes with equal feature rows score alike, see aig_gen_wire_set.cls) as a lookup that can be
+ * differentiated:  out[r*width + i] = table[row_kind[r]*classes + cls[cand[r*width + i]]]  for i < counts[r], -inf past it
+ * and for a candidate, class or kind outside its range;  d_table[k][c] = sum of grad over the rows of kind k and their
+ * places of class c, in f64 per block and in a fixed order (no atomics).
+ *   by_kind [rows]: the rows in the order of their kinds; kind_start [kinds+1]: where each kind begins in it (both for the
+ *   gradient only) */
+typedef struct aig_score_windows {
+    int64_t rows, width, nodes, kinds, classes;
+    const int32_t* cand;          /* [rows,width] */
+    const int32_t* counts;        /* [rows] or NULL */
+    const int32_t* cls;           /* [nodes] */
+    const int32_t* row_kind;      /* [rows] */
+    const int32_t* by_kind;
+    const int32_t* kind_start;
+} aig_score_windows;
+int aig_class_scores(const aig_score_windows* w, const float* table, float* out, void* stream);
+size_t aig_class_scores_bwd_ws_bytes(int64_t rows, int64_t kinds, int64_t classes);
+int aig_class_scores_bwd(const aig_score_windows* w, const float* grad, float* d_table, void* ws, size_t ws_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif
