@@ -45,8 +45,8 @@ class Sampling(C.Structure):
 
 class Distill(C.Structure):
     """Mirror of ``aig_distill``."""
-    _fields_ = ([(n, I64) for n in ("rows", "width", "ld", "m")] + [("dtype", C.c_int32), ("temperature", C.c_float)] +
-                [(n, P) for n in ("logits", "counts", "values", "index", "lse", "weight")])
+    _fields_ = ([(n, I64) for n in ("rows", "width", "ld", "m")] + [("dtype", C.c_int32), ("temperature", C.c_float), ("scale", C.c_float)] +
+                [(n, P) for n in ("logits", "counts", "values", "index", "lse", "weight", "stats")])
 
 
 class ScoreWindowsArg(C.Structure):
@@ -155,7 +155,7 @@ SIGNATURES = {
     "aig_sum_rows_ws_bytes": (SZ, [I64]),
     "aig_sum_rows": (INT, [I64, P, C.c_float, P, P, SZ, P]),
     "aig_class_scores": (INT, [P, P, P, P]),
-    "aig_class_scores_bwd_ws_bytes": (SZ, [I64, I64, I64]),
+    "aig_class_scores_bwd_ws_bytes": (SZ, [I64, I64, I64, I64]),
     "aig_class_scores_bwd": (INT, [P, P, P, P, SZ, P]),
 }
 

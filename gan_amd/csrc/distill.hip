@@ -13,55 +13,64 @@ using namespace rows;
 struct DistillArgs {
     long long rows, ld, grad_ld;
     int width, m, vec, grad_vec;
-    float temperature;
+    double per;                  // log2(e) / T
+    float temperature, factor;
     const int* counts;
     const float *values, *lse, *weight;
     const int* index;
     const float* upstream;       // factor of the gradient: one (stride 0) or one a row, or none
     long long upstream_stride;
     float* loss;                 // may be null
+    float* stats;                // [rows][STATS], wide rows: written with the loss, read for a gradient alone; may be null
     __device__ __forceinline__ int count(long long r) const { return counts ? min(max(counts[r], 0), width) : width; }
-    // whether entry j of the teacher's row names a place of the student's (absent entries: -1, or a logit of -inf)
-    __device__ __forceinline__ bool names(long long r, int j, int n) const {
-        const int i = index[r * m + j];
-        return i >= 0 && i < n && !(values[r * m + j] == -__builtin_inff());
+    __device__ __forceinline__ float scale(long long r) const { return temperature * temperature * factor * (weight ? weight[r] : 1.0f); }
+    __device__ __forceinline__ float scale_of_gradient(long long r) const {
+        return temperature * factor * (weight ? weight[r] : 1.0f) * (upstream ? upstream[r * upstream_stride] : 1.0f);
     }
 };
+// An entry of the teacher's row names a place of the student's (absent entries: place -1, or a logit of -inf).
+__device__ __forceinline__ bool names(int i, float v, int n) { return i >= 0 && i < n && !(v == -__builtin_inff()); }
 
 // Exponentials in base 2.  An argument of -d carries an error of d 2^-23, its exponential one of d 2^-d 2^-23 relative to the
-// row's largest: nowhere more than 2^-23.
+// row's largest: nowhere more than 2^-23.  What is summed or subtracted (probabilities, logarithms) is held in f64: the loss is a
+// small difference of numbers of the size of the logits, and the rest of a row a small difference from 1.
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
-constexpr float LN2F = 0.69314718056f;
-__device__ __forceinline__ float probability(float log_q) { return log_q > 0.0f ? 1.0f : expf(log_q); }      // (NaN stays NaN)
+constexpr double LN2 = 0.69314718055994531;
+__device__ __forceinline__ float probability(double log2_q) { return log2_q > 0.0 ? 1.0f : exp2_fast((float)log2_q); }      // (NaN stays NaN)
+// a sum over the rest of a row that is below this beside the row's largest place is taken again beside its own largest
+constexpr double FAINT = 1e-30;
 
-// A listed entry's probability is added to its place in LDS as a whole number of 2^-30: entries that name one place twice
-// add up to the same bits in any order.
+// A listed entry's probability is added to its place in LDS as a whole number of 2^-30, at least one: entries that name one
+// place twice add up to the same bits in any order, and a place is listed where the sum is not 0.
 constexpr float Q_UNIT = 1073741824.0f;
 
 template <typename T, int G, int E, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __restrict__ grad, DistillArgs a) {
-    constexpr int ROWS = 256 / G, WORDS = (G * E + 31) / 32;
-    __shared__ unsigned listed_bits[ROWS][WORDS];
-    __shared__ unsigned listed_q[GRAD ? ROWS : 1][GRAD ? G * E : 1];
+    constexpr int ROWS = 256 / G;
+    __shared__ __attribute__((aligned(16))) float row_values[ROWS][G * E];
+    __shared__ __attribute__((aligned(16))) unsigned row_listed[ROWS][G * E];
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
     if (r >= a.rows) return;
     const int lane = threadIdx.x & (G - 1), slot = threadIdx.x / G;
-    unsigned* bits = listed_bits[slot];
-    unsigned* qsum = listed_q[GRAD ? slot : 0];
-    for (int w = lane; w < WORDS; w += G) bits[w] = 0;
-    if (GRAD)
-        for (int i = lane; i < G * E; i += G) qsum[i] = 0;
-
+    float* lv = row_values[slot];
+    unsigned* listed = row_listed[slot];
     const int n = a.count(r);
-    x += r * a.ld;
     float v[E];
-    load_values<T, E>(x, n, a.width, a.vec, lane, v);
+    load_values<T, E>(x + r * a.ld, n, a.width, a.vec, lane, v);
+    const int* index = a.index + r * a.m;
+    const float* values = a.values + r * a.m;
+    const int i0 = lane < a.m ? index[lane] : -1;
+    const float v0 = lane < a.m ? values[lane] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        lv[lane * E + e] = v[e];
+        listed[lane * E + e] = 0;
+    }
     float top = -__builtin_inff();
 #pragma unroll
     for (int e = 0; e < E; ++e) top = fmaxf(top, v[e]);
     top = all<G>(top, Max());
-    const float inv_t = 1.0f / a.temperature, per = (float)LOG2E * inv_t;
-    const float base = top > -__builtin_inff() ? top : 0.0f;
+    const float base = top > -__builtin_inff() ? top : 0.0f, per = (float)a.per;
     float ex[E];
     double z = 0.0;
 #pragma unroll
@@ -70,93 +79,83 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
         z += (double)ex[e];
     }
     z = all<G>(z, Add());
-    const float logz = logf((float)z);
 
-    // the teacher's entries: the log-sum-exp of those that name a place of this row, where none is given
-    float lse = 0.0f;
-    int named = 0;
+    // the teacher's log-sum-exp in base 2, or that of the entries
+    double lse;
     if (a.lse) {
-        lse = a.lse[r];
-        for (int j = lane; j < a.m; j += G) {
-            named += a.names(r, j, n);
-        }
+        lse = (double)a.lse[r] * LOG2E;
     } else {
-        float tm = -__builtin_inff();
-        for (int j = lane; j < a.m; j += G) {
-            const bool in = a.names(r, j, n);
-            named += in;
-            tm = in ? fmaxf(tm, a.values[r * a.m + j]) : tm;
-        }
+        float tm = names(i0, v0, n) ? v0 : -__builtin_inff();
+        for (int j = lane + G; j < a.m; j += G) tm = names(index[j], values[j], n) ? fmaxf(tm, values[j]) : tm;
         tm = all<G>(tm, Max());
-        float s = 0.0f;
-        for (int j = lane; j < a.m; j += G) {
-            if (a.names(r, j, n)) s += exp2_fast((a.values[r * a.m + j] - tm) * per);
-        }
-        lse = tm * inv_t + logf(all<G>(s, Add()));
+        double s = names(i0, v0, n) ? (double)exp2_fast((v0 - tm) * per) : 0.0;
+        for (int j = lane + G; j < a.m; j += G) s += names(index[j], values[j], n) ? (double)exp2_fast((values[j] - tm) * per) : 0.0;
+        lse = (double)tm * a.per + log2_of(all<G>(s, Add()));
     }
+    double sum_q = 0.0, l = 0.0;
+    int named = 0;
+    auto entry = [&](int i, float t) {
+        if (!names(i, t, n)) return;
+        ++named;
+        const double lq = (double)t * a.per - lse;
+        const float q = probability(lq);
+        sum_q += (double)q;
+        if (GRAD) atomicAdd(&listed[i], max((unsigned)__float2int_rn(q * Q_UNIT), 1u));
+        else listed[i] = 1u;
+        if (LOSS) l += q > 0.0f ? (double)q * (lq - ((double)lv[i] - (double)base) * a.per) : q == 0.0f ? 0.0 : (double)q;
+    };
+    entry(i0, v0);
+    for (int j = lane + G; j < a.m; j += G) entry(index[j], values[j]);
+    sum_q = all<G>(sum_q, Add());
     named = all<G>(named, Add());
     const bool live = z != 0.0 && named > 0;        // (a NaN among the logits is not nothing: it shows in the loss)
-
-    float sum_q = 0.0f, l = 0.0f;
-    for (int j = lane; j < a.m; j += G) {
-        if (!a.names(r, j, n)) continue;
-        const int i = a.index[r * a.m + j];
-        const float lq = a.values[r * a.m + j] * inv_t - lse, q = probability(lq);
-        sum_q += q;
-        atomicOr(&bits[i >> 5], 1u << (i & 31));
-        if (GRAD) atomicAdd(&qsum[i], (unsigned)__float2int_rn(q * Q_UNIT));
-        if (LOSS && q > 0.0f) l += q * (lq - ((as_float(x[i]) - base) * inv_t - logz));
-    }
-    sum_q = all<G>(sum_q, Add());
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
 
     // the places that are not listed
+    unsigned q_here[E];
     double rest = 0.0;
-    float rest_top = -__builtin_inff();
-    unsigned mine = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int i = lane * E + e;
-        const bool in = (bits[i >> 5] >> (i & 31)) & 1u;
-        mine |= (unsigned)in << e;
-        rest += in ? 0.0 : (double)ex[e];
-        rest_top = in ? rest_top : fmaxf(rest_top, v[e]);
+        q_here[e] = listed[lane * E + e];
+        rest += q_here[e] ? 0.0 : (double)ex[e];
     }
     rest = all<G>(rest, Add());
-    rest_top = all<G>(rest_top, Max());
-    const float rest_q = a.lse && rest_top > -__builtin_inff() ? fmaxf(1.0f - sum_q, 0.0f) : 0.0f;
-    // (their sum may be too small for f32 beside the largest place: then beside their own largest)
-    float shift = 0.0f;
-    if (rest_q > 0.0f && rest < 1e-30) {
-        shift = (base - rest_top) * per;
+    float rest_q = a.lse ? (float)fmax(1.0 - sum_q, 0.0) : 0.0f;
+    float rest_top = base;
+    if (a.lse && rest < FAINT) {
+        rest_top = -__builtin_inff();
+#pragma unroll
+        for (int e = 0; e < E; ++e) rest_top = q_here[e] ? rest_top : fmaxf(rest_top, v[e]);
+        rest_top = all<G>(rest_top, Max());
+        if (!(rest_top > -__builtin_inff())) rest_q = 0.0f;
         rest = 0.0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) rest += (mine >> e) & 1u ? 0.0 : (double)exp2_fast((v[e] - rest_top) * per);
+        for (int e = 0; e < E; ++e) rest += q_here[e] || rest_q == 0.0f ? 0.0 : (double)exp2_fast((v[e] - rest_top) * per);
         rest = all<G>(rest, Add());
     }
-    const float scale = a.temperature * a.temperature * (a.weight ? a.weight[r] : 1.0f);
+    const bool faint = rest_q > 0.0f && rest_top != base;
     if (LOSS) {
         l = all<G>(l, Add());
-        if (rest_q > 0.0f) l += rest_q * (logf(rest_q) - (logf((float)rest) - shift * LN2F - logz));
-        if (lane == 0) a.loss[r] = live ? scale * l : 0.0f;
+        // two logarithms at once: the even lanes take that of z, the odd ones that of the rest's two probabilities' ratio (by z)
+        const double part = rest_q > 0.0f ? (double)rest_q / rest : 1.0;
+        const double lg = log2_of(lane & 1 ? part : z), other = dpp<0xB1>(lg);      // (lanes 1 apart)
+        const double logz = lane & 1 ? other : lg, log_part = lane & 1 ? lg : other;
+        l += sum_q * logz;
+        if (rest_q > 0.0f) l += (double)rest_q * (log_part + logz - ((double)rest_top - (double)base) * a.per);
+        if (lane == 0) a.loss[r] = live ? (float)((double)a.scale(r) * LN2 * l) : 0.0f;
     }
     if (GRAD) {
-        const float up = a.upstream ? a.upstream[r * a.upstream_stride] : 1.0f;
-        const float c = live ? scale * inv_t * up : 0.0f, inv_z = 1.0f / (float)z, inv_rest = rest_q > 0.0f ? rest_q / (float)rest : 0.0f;
-        grad += r * a.grad_ld;
+        const float c = live ? a.scale_of_gradient(r) : 0.0f, full = (float)((sum_q + (double)rest_q) / z),
+                    outside = rest_q > 0.0f ? (float)((double)rest_q / rest) : 0.0f;
         T g[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int i = lane * E + e;
-            const float p = ex[e] * inv_z;
-            float d = p * (sum_q + rest_q);
-            if ((mine >> e) & 1u)
-                d -= (float)qsum[i] * (1.0f / Q_UNIT);
-            else
-                d -= (shift > 0.0f ? exp2_fast((v[e] - rest_top) * per) : ex[e]) * inv_rest;
-            g[e] = from_float<T>(i < n && live ? c * d : 0.0f);
+            float d = faint && !q_here[e] ? exp2_fast((v[e] - rest_top) * per) : ex[e];
+            d = q_here[e] ? (float)q_here[e] * (1.0f / Q_UNIT) : d * outside;
+            g[e] = from_float<T>(lane * E + e < n && live ? c * (ex[e] * full - d) : 0.0f);
         }
+        grad += r * a.grad_ld;
         typedef Places<T, E> P;
         if (a.grad_vec && lane * E + E <= a.width) {
             union { typename P::word w[E / P::PER]; T t[E]; } u;
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
 }
 
 // ---------------------------------------------------------------- wide rows: a workgroup per row
-constexpr int WIDE_T = 1024;
+constexpr int WIDE_T = 1024, STATS = 8;
 
 template <typename V, typename OP> __device__ __forceinline__ V block_all(V v, OP op, double* red) {
     V* s = reinterpret_cast<V*>(red);
@@ -187,89 +186,147 @@ template <typename V, typename OP> __device__ __forceinline__ V block_all(V v, O
     return t;
 }
 
+// One pass over the row for the largest place, the sum of exponentials and that of the places that are not listed (each
+// thread beside its own largest so far), a second one for the gradient.  Listed places are a bitmap in LDS, shifted so that a
+// vector's bits are one byte of it (f32: half a byte).
 template <typename T, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x, T* __restrict__ grad, DistillArgs a) {
+    constexpr int PER = Span<T>::PER;
     __shared__ double red[WIDE_T / 64];
-    __shared__ unsigned bits[MAX_WIDTH / 32];
+    __shared__ unsigned bits[MAX_WIDTH / 32 + 1];
     __shared__ int place[AIG_ROWS_MAX_TOP];
     __shared__ float prob[AIG_ROWS_MAX_TOP];
     const long long r = blockIdx.x;
     const int n = a.count(r), t = threadIdx.x;
     x += r * a.ld;
-    for (int w = t; w < (n + 31) / 32; w += WIDE_T) bits[w] = 0;
-    float top = -__builtin_inff();
-    for (int i = t; i < n; i += WIDE_T) top = fmaxf(top, as_float(x[i]));
-    top = block_all(top, Max(), red);
-    const float inv_t = 1.0f / a.temperature, per = (float)LOG2E * inv_t;
-    const float base = top > -__builtin_inff() ? top : 0.0f;
+    const Span<T> row(x, n);
+    const int pad = (PER - row.head) & (PER - 1);
+    auto listed = [&](int i) { return bits[(i + pad) >> 5] >> ((i + pad) & 31); };      // bit 0: place i, bits 1 .. PER-1: the next ones of its vector
+    for (int w = t; w < (n + pad + 31) / 32; w += WIDE_T) bits[w] = 0;
+    const float per = (float)a.per;
 
     // (at most AIG_ROWS_MAX_TOP entries: one a thread)
     int i_mine = -1;
     float v_mine = -__builtin_inff();
-    if (t < a.m && a.names(r, t, n)) {
-        i_mine = a.index[r * a.m + t];
-        v_mine = a.values[r * a.m + t];
+    if (t < a.m) {
+        const int i = a.index[r * a.m + t];
+        const float v = a.values[r * a.m + t];
+        if (names(i, v, n)) {
+            i_mine = i;
+            v_mine = v;
+        }
     }
     const int named = block_all((int)(i_mine >= 0), Add(), red);
-    float lse;
-    if (a.lse)
-        lse = a.lse[r];
-    else {
+    if (i_mine >= 0) atomicOr(&bits[(i_mine + pad) >> 5], 1u << ((i_mine + pad) & 31));
+    double lse;
+    if (a.lse) {
+        lse = (double)a.lse[r] * LOG2E;
+    } else {
         const float tm = block_all(v_mine, Max(), red);
-        lse = tm * inv_t + logf(block_all(i_mine >= 0 ? exp2_fast((v_mine - tm) * per) : 0.0f, Add(), red));
+        lse = (double)tm * a.per + log2_of(block_all(i_mine >= 0 ? (double)exp2_fast((v_mine - tm) * per) : 0.0, Add(), red));
     }
-    const float lq = v_mine * inv_t - lse, q = i_mine >= 0 ? probability(lq) : 0.0f;
-    const float sum_q = block_all(q, Add(), red);
-    if (t < AIG_ROWS_MAX_TOP) {
+    const double lq = (double)v_mine * a.per - lse;
+    const float q = i_mine >= 0 ? probability(lq) : 0.0f;
+    const double sum_q = block_all((double)q, Add(), red);
+    if (GRAD && t < AIG_ROWS_MAX_TOP) {
         place[t] = i_mine;
         prob[t] = q;
     }
-    if (i_mine >= 0) atomicOr(&bits[i_mine >> 5], 1u << (i_mine & 31));
     __syncthreads();
 
-    double z = 0.0, rest = 0.0;
-    float rest_top = -__builtin_inff();
-    for (int i = t; i < n; i += WIDE_T) {
-        const float v = as_float(x[i]), ex = exp2_fast((v - base) * per);
-        const bool in = (bits[i >> 5] >> (i & 31)) & 1u;
-        z += (double)ex;
-        rest += in ? 0.0 : (double)ex;
-        rest_top = in ? rest_top : fmaxf(rest_top, v);
+    float top, rest_top;
+    double z, rest;
+    const bool known = GRAD && !LOSS && a.stats;
+    if (known) {
+        const float* s = a.stats + r * STATS;
+        top = s[0];
+        rest_top = s[1];
+        z = *reinterpret_cast<const double*>(s + 2);
+        rest = *reinterpret_cast<const double*>(s + 4);
+    } else {
+        float mine = -__builtin_inff();
+        z = rest = 0.0;
+        row.each(t, WIDE_T, [&](int i, const float (&v)[PER], int count) {
+            float here = v[0];
+            for (int j = 1; j < PER; ++j) here = j < count ? fmaxf(here, v[j]) : here;
+            if (here > mine) {
+                const double shrink = mine > -__builtin_inff() ? (double)exp2_fast((mine - here) * per) : 0.0;
+                z *= shrink;
+                rest *= shrink;
+                mine = here;
+            }
+            const float base = mine > -__builtin_inff() ? mine : 0.0f;
+            const unsigned in = listed(i);
+            float s = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const float e = j < count ? exp2_fast((v[j] - base) * per) : 0.0f;
+                s += e;
+                u += (in >> j) & 1u ? 0.0f : e;
+            }
+            z += (double)s;
+            rest += (double)u;
+        });
+        top = block_all(mine, Max(), red);
+        const float shrink = mine > -__builtin_inff() ? exp2_fast((mine - top) * per) : 1.0f;      // (1: keeps a NaN)
+        z = block_all(z * (double)shrink, Add(), red);
+        rest = block_all(rest * (double)shrink, Add(), red);
+        rest_top = top;
+        if (a.lse && rest < FAINT) {
+            float u = -__builtin_inff();
+            for (int i = t; i < n; i += WIDE_T) u = listed(i) & 1u ? u : fmaxf(u, as_float(x[i]));
+            rest_top = block_all(u, Max(), red);
+            double s = 0.0;
+            if (rest_top > -__builtin_inff())
+                for (int i = t; i < n; i += WIDE_T) s += listed(i) & 1u ? 0.0 : (double)exp2_fast((as_float(x[i]) - rest_top) * per);
+            rest = block_all(s, Add(), red);
+        }
+        if (LOSS && a.stats && t == 0) {
+            float* s = a.stats + r * STATS;
+            s[0] = top;
+            s[1] = rest_top;
+            *reinterpret_cast<double*>(s + 2) = z;
+            *reinterpret_cast<double*>(s + 4) = rest;
+        }
     }
-    z = block_all(z, Add(), red);
-    rest = block_all(rest, Add(), red);
-    rest_top = block_all(rest_top, Max(), red);
+    const float base = top > -__builtin_inff() ? top : 0.0f;
     const bool live = z != 0.0 && named > 0;
-    const float logz = logf((float)z);
-    const float rest_q = a.lse && rest_top > -__builtin_inff() ? fmaxf(1.0f - sum_q, 0.0f) : 0.0f;
-    float shift = 0.0f;
-    if (rest_q > 0.0f && rest < 1e-30) {
-        shift = (base - rest_top) * per;
-        rest = 0.0;
-        for (int i = t; i < n; i += WIDE_T)
-            rest += (bits[i >> 5] >> (i & 31)) & 1u ? 0.0 : (double)exp2_fast((as_float(x[i]) - rest_top) * per);
-        rest = block_all(rest, Add(), red);
-    }
-    const float scale = a.temperature * a.temperature * (a.weight ? a.weight[r] : 1.0f);
+    const float rest_q = a.lse && rest_top > -__builtin_inff() ? (float)fmax(1.0 - sum_q, 0.0) : 0.0f;
+    const bool faint = rest_q > 0.0f && rest_top != top;
     if (LOSS) {
-        float l = i_mine >= 0 && q > 0.0f ? q * (lq - ((as_float(x[i_mine]) - base) * inv_t - logz)) : 0.0f;
+        double l = 0.0;
+        if (i_mine >= 0) l = q > 0.0f ? (double)q * (lq - ((double)as_float(x[i_mine]) - (double)base) * a.per) : q == 0.0f ? 0.0 : (double)q;
         l = block_all(l, Add(), red);
-        if (rest_q > 0.0f) l += rest_q * (logf(rest_q) - (logf((float)rest) - shift * LN2F - logz));
-        if (t == 0) a.loss[r] = live ? scale * l : 0.0f;
+        if (t == 0) {
+            const double logz = log2_of(z);
+            l += sum_q * logz;
+            if (rest_q > 0.0f) l += (double)rest_q * (log2_of((double)rest_q / rest) + logz - ((double)rest_top - (double)base) * a.per);
+            a.loss[r] = live ? (float)((double)a.scale(r) * LN2 * l) : 0.0f;
+        }
     }
     if (GRAD) {
-        const float up = a.upstream ? a.upstream[r * a.upstream_stride] : 1.0f;
-        const float c = live ? scale * inv_t * up : 0.0f, inv_z = 1.0f / (float)z, inv_rest = rest_q > 0.0f ? rest_q / (float)rest : 0.0f;
+        const float c = live ? a.scale_of_gradient(r) : 0.0f, full = (float)((sum_q + (double)rest_q) / z),
+                    outside = rest_q > 0.0f ? (float)((double)rest_q / rest) : 0.0f;
         grad += r * a.grad_ld;
-        for (int i = t; i < a.width; i += WIDE_T) {
-            float d = 0.0f;
-            if (i < n && live) {
-                if ((bits[i >> 5] >> (i & 31)) & 1u) continue;       // below
-                const float v = as_float(x[i]), ex = exp2_fast((v - base) * per);
-                d = c * (ex * inv_z * (sum_q + rest_q) - (shift > 0.0f ? exp2_fast((v - rest_top) * per) : ex) * inv_rest);
-            }
-            grad[i] = from_float<T>(d);
-        }
+        const bool vec = ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(x)) & 15) == 0;
+        auto slope = [&](float v) {
+            const float e = exp2_fast((v - base) * per);
+            return c * (e * full - (faint ? exp2_fast((v - rest_top) * per) : e) * outside);
+        };
+        if (live)
+            row.each(t, WIDE_T, [&](int i, const float (&v)[PER], int count) {
+                const unsigned in = listed(i) & ((1u << count) - 1u);
+                if (vec && count == PER && in == 0u) {
+                    union { uint4 w; T t[PER]; } u;
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) u.t[j] = from_float<T>(slope(v[j]));
+                    *reinterpret_cast<uint4*>(grad + i) = u.w;
+                } else {
+                    for (int j = 0; j < PER; ++j)
+                        if (j < count && !((in >> j) & 1u)) grad[i + j] = from_float<T>(slope(v[j]));       // (listed places: below)
+                }
+            });
+        for (int i = (live ? n : 0) + t; i < a.width; i += WIDE_T) grad[i] = from_float<T>(0.0f);
         if (live && i_mine >= 0) {        // a listed place is written by the first entry that names it, for all of them
             float s = 0.0f;
             bool is_first = true;
@@ -278,24 +335,23 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
                     is_first = is_first && j >= t;
                     s += prob[j];
                 }
-            if (is_first) {
-                const float p = exp2_fast((as_float(x[i_mine]) - base) * per) * inv_z;
-                grad[i_mine] = from_float<T>(c * (p * (sum_q + rest_q) - s));
-            }
+            if (is_first) grad[i_mine] = from_float<T>(c * (exp2_fast((as_float(x[i_mine]) - base) * per) * full - s));
         }
     }
 }
 
 // The sum of the rows' losses, in an order that the number of rows alone gives.
-constexpr int SUM_T = 1024, SUM_BLOCKS = 256;
+constexpr int SUM_T = 1024, SUM_BLOCKS = 256, SUM_ONE = 32 * SUM_T;      // (up to SUM_ONE rows: one block, one launch)
 __global__ __launch_bounds__(SUM_T) void k_sum_rows(long long n, const float* __restrict__ v, double* __restrict__ partial,
                                                     const double* __restrict__ partial_in, float factor, float* __restrict__ out) {
     __shared__ double red[SUM_T / 64];
     double s = 0.0;
-    if (partial_in)
+    if (partial_in) {
         for (long long i = threadIdx.x; i < n; i += SUM_T) s += partial_in[i];
-    else
+    } else {
+#pragma unroll 8
         for (long long i = (long long)blockIdx.x * SUM_T + threadIdx.x; i < n; i += (long long)gridDim.x * SUM_T) s += (double)v[i];
+    }
     s = block_all(s, Add(), red);
     if (threadIdx.x == 0) {
         if (out)
@@ -349,7 +405,8 @@ extern "C" int aig_distill_rows(const aig_distill* d, float* loss, void* grad, i
     AIG_REQUIRE(loss || grad, "aig_distill_rows: nothing to compute");
     AIG_REQUIRE(d->logits && d->values && d->index, "aig_distill_rows: null pointer");
     DistillArgs a{};
-    a.rows = d->rows; a.ld = d->ld; a.grad_ld = grad_ld; a.width = (int)d->width; a.m = (int)d->m; a.temperature = d->temperature;
+    a.rows = d->rows; a.ld = d->ld; a.grad_ld = grad_ld; a.width = (int)d->width; a.m = (int)d->m; a.temperature = d->temperature; a.factor = d->scale;
+    a.per = rows::LOG2E / (double)d->temperature; a.stats = d->width > rows::NARROW ? d->stats : nullptr;
     a.counts = d->counts; a.values = d->values; a.lse = d->lse; a.weight = d->weight; a.index = d->index;
     a.upstream = upstream; a.upstream_stride = upstream_stride; a.loss = loss;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -358,12 +415,12 @@ extern "C" int aig_distill_rows(const aig_distill* d, float* loss, void* grad, i
     return distill(s, static_cast<const __hip_bfloat16*>(d->logits), static_cast<__hip_bfloat16*>(grad), a);
 }
 
-extern "C" size_t aig_sum_rows_ws_bytes(int64_t rows) { return rows > SUM_T * 8 ? SUM_BLOCKS * sizeof(double) : 0; }
+extern "C" size_t aig_sum_rows_ws_bytes(int64_t rows) { return rows > SUM_ONE ? SUM_BLOCKS * sizeof(double) : 0; }
 
 extern "C" int aig_sum_rows(int64_t rows, const float* v, float factor, float* out, void* ws, size_t ws_bytes, void* stream) {
     AIG_REQUIRE(rows >= 0 && out && (v || rows == 0), "aig_sum_rows: bad argument");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (rows <= SUM_T * 8) {
+    if (rows <= SUM_ONE) {
         hipLaunchKernelGGL(k_sum_rows, dim3(1), dim3(SUM_T), 0, s, (long long)rows, v, nullptr, nullptr, factor, out);
     } else {
         if (ws_bytes < aig_sum_rows_ws_bytes(rows) || !ws) return fail(AIG_EWORKSPACE, "aig_sum_rows: workspace too small");

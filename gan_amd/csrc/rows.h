@@ -84,10 +84,9 @@ template <int G, typename V> __device__ __forceinline__ V before(V v) {
 // and are exact in f64 in whatever order they are taken - by lanes, by blocks, by atomics - so a draw is a function of its
 // row alone.  What is lost is a weight's 2^-37, far below the 2^-24 steps of the random numbers.
 constexpr double UNIT = 68719476736.0;          // 2^36
-// d = (l - max) log2(e) / T <= 0: rint(2^d UNIT).  2^f on |f| <= 1/2 by its series, the first term left out is below
-// 7e-15 (ln2^12 / (12! 2^12)), three decimal digits under the unit.
-__device__ __forceinline__ double weight_of(double d) {
-    d = fmax(d, -64.0);
+// 2^(d + SHIFT), d in [-900, 900].  2^f on |f| <= 1/2 by its series: the first term left out is below 7e-15
+// (ln2^12 / (12! 2^12)), a hundredth of a step of what it is used for (2^-36 here, 2^-24 elsewhere).
+template <int SHIFT> __device__ __forceinline__ double pow2(double d) {
     const double n = __builtin_rint(d), f = d - n;
     double p = 4.4455382718708110e-10;          // ln2^k / k!, k = 11 .. 0
     p = fma(p, f, 7.0549116208011210e-09);
@@ -101,8 +100,14 @@ __device__ __forceinline__ double weight_of(double d) {
     p = fma(p, f, 2.4022650695910070e-01);
     p = fma(p, f, 6.9314718055994531e-01);
     p = fma(p, f, 1.0);
-    const long long scale = (long long)(1023 + 36 + (int)n) << 52;      // 2^(n + 36), n >= -64
-    return __builtin_rint(p * __longlong_as_double(scale));
+    return p * __longlong_as_double((long long)(1023 + SHIFT + (int)n) << 52);
+}
+// d = (l - max) log2(e) / T <= 0: the weight rint(2^d UNIT)
+__device__ __forceinline__ double weight_of(double d) { return __builtin_rint(pow2<36>(fmax(d, -64.0))); }
+// log2(z) to about 2^-45, z in the range of f32: the hardware's logarithm and one Newton step
+__device__ __forceinline__ double log2_of(double z) {
+    const double l = (double)__builtin_amdgcn_logf((float)z);
+    return fma(fma(z, pow2<0>(-l), -1.0), 1.4426950408889634, l);
 }
 constexpr double LOG2E = 1.4426950408889634;
 
@@ -162,6 +167,40 @@ __device__ __forceinline__ void kth_largest(const unsigned (&key)[E], int k, uns
     thr = t;
     quota = k - all<G>(n, Add());
 }
+
+// ---------------------------------------------------------------- wide rows
+// A row of n values read by a workgroup: single places up to the first 16-byte boundary, vectors, single places behind the
+// last one - whatever the row's alignment.  f(i, v, count): the places i .. i + count - 1, count 1 or PER; `first` and `step`
+// are the caller's thread and the number of threads.
+template <typename T> struct Span {
+    static constexpr int PER = 16 / (int)sizeof(T);
+    const T* x;
+    int n, head, vecs;
+    __device__ __forceinline__ Span(const T* row, int count) : x(row), n(count) {
+        head = min((int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T), n);
+        vecs = (n - head) / PER;
+    }
+    template <typename F> __device__ __forceinline__ void each(int first, int step, F f) const {
+        if (first < head) {
+            const float v[PER] = {as_float(x[first])};
+            f(first, v, 1);
+        }
+#pragma unroll 2
+        for (int k = first; k < vecs; k += step) {
+            union { uint4 w; T t[PER]; } u;
+            u.w = reinterpret_cast<const uint4*>(x + head)[k];
+            float v[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] = as_float(u.t[j]);
+            f(head + k * PER, v, PER);
+        }
+        const int tail = head + vecs * PER + first;
+        if (tail < n) {
+            const float v[PER] = {as_float(x[tail])};
+            f(tail, v, 1);
+        }
+    }
+};
 
 }  // namespace rows
 }  // namespace aig

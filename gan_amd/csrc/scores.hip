@@ -25,28 +25,70 @@ struct Windows {
     }
 };
 
-__global__ __launch_bounds__(256) void k_class_scores(Windows w, const float* __restrict__ table, float* __restrict__ out) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= w.rows * w.width) return;
-    const long long r = i / w.width;
-    const int at = (int)(i - r * w.width), kind = w.row_kind[r];
-    float v = NOTHING;
-    if (at < w.count(r) && kind >= 0 && kind < w.kinds) {
-        const int c = w.cls_of(w.cand[i]);
-        if (c >= 0) v = table[(long long)kind * w.classes + c];
+// V places a lane (4 where rows start on 16 bytes and hold whole vectors), LPR lanes a row: a row's kind and count are read
+// once for its places, and there is no division by the width.
+template <int V, typename W> __device__ __forceinline__ void load_vec(const W* p, W (&v)[V]) {
+    if constexpr (V == 4) {
+        const int4 q = *reinterpret_cast<const int4*>(p);
+        __builtin_memcpy(v, &q, 16);
+    } else {
+        v[0] = p[0];
     }
-    out[i] = v;
+}
+
+constexpr int AHEAD = 2;       // rows a lane has in flight: the chain row -> candidate -> class -> score is four memory trips
+
+template <int V>
+__global__ __launch_bounds__(256) void k_class_scores(Windows w, int lpr_bits, const float* __restrict__ table, float* __restrict__ out) {
+    const int lpr = 1 << lpr_bits, slots = 256 >> lpr_bits;
+    const long long r0 = (long long)blockIdx.x * (slots * AHEAD) + (threadIdx.x >> lpr_bits);
+    long long r[AHEAD];
+    int n[AHEAD];
+    const float* row[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+        r[k] = min(r0 + k * slots, w.rows - 1);
+        const int kind = w.row_kind[r[k]];
+        n[k] = kind >= 0 && kind < w.kinds ? w.count(r[k]) : 0;
+        row[k] = table + (long long)(n[k] > 0 ? kind : 0) * w.classes;
+    }
+    for (int at = (threadIdx.x & (lpr - 1)) * V; at < w.width; at += lpr * V) {
+        int c[AHEAD][V];
+        float v[AHEAD][V];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) load_vec<V>(w.cand + r[k] * w.width + at, c[k]);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[k][j] = at + j < n[k] ? w.cls_of(c[k][j]) : -1;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[k][j] = c[k][j] >= 0 ? row[k][c[k][j]] : NOTHING;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (r0 + k * slots >= w.rows) break;
+            if constexpr (V == 4)
+                *reinterpret_cast<float4*>(out + r[k] * w.width + at) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+            else
+                out[r[k] * w.width + at] = v[k][0];
+        }
+    }
 }
 
 // Rows in the order of their kinds are dealt to blocks in runs of RUN; a run may hold rows of several kinds.  A block adds
-// the gradients of one kind's rows into private columns acc[class][thread] in LDS, sums the columns in a fixed order when
-// the kind ends, and writes the sum as partial number (block + kind): no two (block, kind) pairs that occur share it.
-constexpr int RUN = 64;
+// the gradients of one kind's rows into private columns acc[class][thread] in LDS - a thread's own additions, in order, no
+// atomics - sums the columns in a fixed order in f64 when the kind ends, and writes the sum as partial number (block +
+// kind): no two (block, kind) pairs that occur share it.
+// A run holds about 4096 places: enough that the columns' sums at its end weigh little, few enough that there are several
+// blocks for every CU.
+static int run_rows(int64_t width) { return width >= 512 ? 8 : width <= 64 ? 64 : (int)(4096 / width); }
 
-__global__ __launch_bounds__(256) void k_class_scores_bwd(Windows w, int threads, const float* __restrict__ grad, double* __restrict__ partial) {
+template <int V>
+__global__ __launch_bounds__(256) void k_class_scores_bwd(Windows w, int run, int lpr_bits, const float* __restrict__ grad, double* __restrict__ partial) {
     extern __shared__ float acc[];          // [classes][threads]
-    const int t = threadIdx.x;
-    const long long p0 = (long long)blockIdx.x * RUN, p1 = min(p0 + RUN, w.rows);
+    const int t = threadIdx.x, threads = blockDim.x, lpr = 1 << lpr_bits, slots = threads >> lpr_bits;
+    const long long p0 = (long long)blockIdx.x * run, p1 = min(p0 + run, w.rows);
     for (int i = t; i < w.classes * threads; i += threads) acc[i] = 0.0f;
     __syncthreads();
     long long p = p0;
@@ -56,35 +98,75 @@ __global__ __launch_bounds__(256) void k_class_scores_bwd(Windows w, int threads
             ++p;
             continue;
         }
-        for (; p < p1 && w.kind_at(p) == kind; ++p) {
-            const long long r = w.by_kind[p];
-            const int n = w.count(r);
-            for (int i = t; i < n; i += threads) {
-                const int c = w.cls_of(w.cand[r * w.width + i]);
-                if (c >= 0) acc[c * threads + t] += grad[r * w.width + i];
+        const long long end = min(max((long long)w.kind_start[kind + 1], p + 1), p1);      // (ends whatever the array holds)
+        for (long long at_row = p + (t >> lpr_bits); at_row < end; at_row += AHEAD * slots) {
+            long long r[AHEAD];
+            int n[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const bool here = at_row + k * slots < end;
+                const int id = w.by_kind[here ? at_row + k * slots : at_row];
+                r[k] = id >= 0 && id < w.rows ? id : 0;
+                n[k] = here && r[k] == id ? w.count(r[k]) : 0;
+            }
+            int most = 0;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) most = max(most, n[k]);
+            for (int at = (t & (lpr - 1)) * V; at < most; at += lpr * V) {
+                int c[AHEAD][V];
+                float g[AHEAD][V];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    load_vec<V>(w.cand + r[k] * w.width + at, c[k]);
+                    load_vec<V>(grad + r[k] * w.width + at, g[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) c[k][j] = at + j < n[k] ? w.cls_of(c[k][j]) : -1;
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (c[k][j] >= 0) acc[c[k][j] * threads + t] += g[k][j];
             }
         }
+        p = end;
         __syncthreads();
-        for (int c = t; c < w.classes; c += threads) {
+        const int lane = t & 63, waves = (threads + 63) >> 6;
+        for (int c = t >> 6; c < w.classes; c += waves) {
             double s = 0.0;
-            for (int j = 0; j < threads; ++j) {
+            for (int j = lane; j < threads; j += 64) {
                 s += (double)acc[c * threads + j];
                 acc[c * threads + j] = 0.0f;
             }
-            partial[((long long)blockIdx.x + kind) * w.classes + c] = s;
+            for (int o = 32; o; o >>= 1) {
+                const double other = __shfl_down(s, o);
+                s += lane + o < threads ? other : 0.0;
+            }
+            if (lane == 0) partial[((long long)blockIdx.x + kind) * w.classes + c] = s;
         }
         __syncthreads();
     }
 }
 
-__global__ __launch_bounds__(64) void k_class_scores_finish(Windows w, const double* __restrict__ partial, float* __restrict__ d_table) {
-    const int kind = blockIdx.x;
+// A block a kind: class c of every groups-th partial by a thread, the groups' sums in order.
+__global__ __launch_bounds__(256) void k_class_scores_finish(Windows w, int run, int cp_bits, const double* __restrict__ partial, float* __restrict__ d_table) {
+    __shared__ double red[256];
+    const int kind = blockIdx.x, cp = 1 << cp_bits, groups = 256 >> cp_bits, g = threadIdx.x >> cp_bits;
     const long long s = max(w.kind_start[kind], 0), e = min((long long)w.kind_start[kind + 1], w.rows);
-    for (int c = threadIdx.x; c < w.classes; c += 64) {
+    for (int c0 = 0; c0 < w.classes; c0 += cp) {
+        const int c = c0 + (threadIdx.x & (cp - 1));
         double sum = 0.0;
-        if (e > s)
-            for (long long b = s / RUN; b <= (e - 1) / RUN; ++b) sum += partial[(b + kind) * w.classes + c];
-        d_table[(long long)kind * w.classes + c] = (float)sum;
+        if (e > s && c < w.classes)
+            for (long long b = s / run + g; b <= (e - 1) / run; b += groups) sum += partial[(b + kind) * w.classes + c];
+        red[threadIdx.x] = sum;
+        __syncthreads();
+        if (g == 0 && c < w.classes) {
+            for (int j = 1; j < groups; ++j) sum += red[(j << cp_bits) + threadIdx.x];
+            d_table[(long long)kind * w.classes + c] = (float)sum;
+        }
+        __syncthreads();
     }
 }
 }  // namespace
@@ -110,35 +192,54 @@ static Windows windows_of(const aig_score_windows* w) {
                    w->by_kind, w->kind_start};
 }
 
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// lanes a row (a power of two, as its logarithm): enough for the row's vectors, at most 2^most
+static int lanes_a_row(int64_t width, int per_lane, int most) {
+    int bits = 0;
+    while (bits < most && ((int64_t)per_lane << bits) < width) ++bits;
+    return bits;
+}
+
 extern "C" int aig_class_scores(const aig_score_windows* w, const float* table, float* out, void* stream) {
     if (const int rc = check_windows("aig_class_scores", w)) return rc;
     if (w->rows == 0) return AIG_OK;
     AIG_REQUIRE(table && out, "aig_class_scores: null pointer");
-    hipLaunchKernelGGL(k_class_scores, dim3((unsigned)((w->rows * w->width + 255) / 256)), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), windows_of(w), table, out);
+    const bool vec = w->width % 4 == 0 && aligned16(w->cand) && aligned16(out);
+    const int bits = lanes_a_row(w->width, vec ? 4 : 1, 8);
+    const int64_t per_block = (int64_t)(256 >> bits) * AHEAD;
+    const dim3 grid((unsigned)((w->rows + per_block - 1) / per_block));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (vec) hipLaunchKernelGGL(k_class_scores<4>, grid, dim3(256), 0, s, windows_of(w), bits, table, out);
+    else hipLaunchKernelGGL(k_class_scores<1>, grid, dim3(256), 0, s, windows_of(w), bits, table, out);
     AIG_LAUNCH_CHECK();
     return AIG_OK;
 }
 
-extern "C" size_t aig_class_scores_bwd_ws_bytes(int64_t rows, int64_t kinds, int64_t classes) {
-    if (rows < 0 || kinds < 1 || classes < 1) return 0;
-    return align_up((size_t)((rows + RUN - 1) / RUN + kinds) * (size_t)classes * sizeof(double));
+extern "C" size_t aig_class_scores_bwd_ws_bytes(int64_t rows, int64_t width, int64_t kinds, int64_t classes) {
+    if (rows < 0 || width < 1 || kinds < 1 || classes < 1) return 0;
+    return align_up((size_t)((rows + run_rows(width) - 1) / run_rows(width) + kinds) * (size_t)classes * sizeof(double));
 }
 
 extern "C" int aig_class_scores_bwd(const aig_score_windows* w, const float* grad, float* d_table, void* ws, size_t ws_bytes, void* stream) {
     if (const int rc = check_windows("aig_class_scores_bwd", w)) return rc;
     AIG_REQUIRE(d_table && (w->rows == 0 || (grad && w->by_kind)) && w->kind_start, "aig_class_scores_bwd: null pointer");
-    if (!ws || ws_bytes < aig_class_scores_bwd_ws_bytes(w->rows, w->kinds, w->classes))
+    if (!ws || ws_bytes < aig_class_scores_bwd_ws_bytes(w->rows, w->width, w->kinds, w->classes))
         return fail(AIG_EWORKSPACE, "aig_class_scores_bwd: workspace of %zu bytes is too small", ws_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
     double* partial = static_cast<double*>(ws);
-    const int threads = w->classes <= 128 ? 256 : w->classes <= 512 ? 64 : 32;      // columns of at most 128 KB
+    const int run = run_rows(w->width), threads = w->classes <= 128 ? 256 : w->classes <= 512 ? 64 : 32;      // columns of at most 128 KB
     const size_t lds = (size_t)w->classes * threads * sizeof(float);
-    AIG_HIP_CHECK(ensure_dynamic_lds(reinterpret_cast<const void*>(k_class_scores_bwd), 128 * 1024));
-    if (w->rows)
-        hipLaunchKernelGGL(k_class_scores_bwd, dim3((unsigned)((w->rows + RUN - 1) / RUN)), dim3(threads), lds, s, windows_of(w), threads,
-                           grad, partial);
-    hipLaunchKernelGGL(k_class_scores_finish, dim3((unsigned)w->kinds), dim3(64), 0, s, windows_of(w), partial, d_table);
+    if (w->rows) {
+        const bool vec = w->width % 4 == 0 && aligned16(w->cand) && aligned16(grad);
+        const int bits = lanes_a_row(w->width, vec ? 4 : 1, threads == 256 ? 8 : threads == 64 ? 6 : 5);
+        const dim3 grid((unsigned)((w->rows + run - 1) / run));
+        AIG_HIP_CHECK(ensure_dynamic_lds(vec ? reinterpret_cast<const void*>(k_class_scores_bwd<4>) : reinterpret_cast<const void*>(k_class_scores_bwd<1>), lds));
+        if (vec) hipLaunchKernelGGL(k_class_scores_bwd<4>, grid, dim3(threads), lds, s, windows_of(w), run, bits, grad, partial);
+        else hipLaunchKernelGGL(k_class_scores_bwd<1>, grid, dim3(threads), lds, s, windows_of(w), run, bits, grad, partial);
+    }
+    int cp_bits = 0;
+    while (cp_bits < 8 && (1 << cp_bits) < w->classes) ++cp_bits;
+    hipLaunchKernelGGL(k_class_scores_finish, dim3((unsigned)w->kinds), dim3(256), 0, s, windows_of(w), run, cp_bits, partial, d_table);
     AIG_LAUNCH_CHECK();
     return AIG_OK;
 }

@@ -15,8 +15,8 @@ receives a gradient (train.py:297-299).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -27,6 +27,7 @@ from . import _abi
 MAX_WIDTH = 131072
 MAX_DRAWS = 8
 MAX_TOP = 256
+NARROW = 1024          # rows up to this width are held in registers, wider ones are a workgroup's each
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -66,56 +67,72 @@ class ScoreWindows(NamedTuple):
 
 # ------------------------------------------------------------------ checks
 def _rows_of(logits: torch.Tensor, what: str) -> Tuple[int, int, int, int]:
-    if not torch.is_tensor(logits) or not logits.is_cuda:
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise _abi.AigAbiError(f"{what} needs the logits on a HIP device (no CPU path exists)")
-    if logits.dim() != 2 or logits.dtype not in _DTYPES:
+    dtype = _DTYPES.get(logits.dtype)
+    if dtype is None or logits.dim() != 2:
         raise _abi.AigAbiError(f"{what} takes logits [rows, width] in float32, float16 or bfloat16, got {logits.dtype} {tuple(logits.shape)}")
-    rows, width = int(logits.size(0)), int(logits.size(1))
+    (rows, width), (ld, step) = logits.shape, logits.stride()
     if not 1 <= width <= MAX_WIDTH:
         raise _abi.AigAbiError(f"{what} takes rows of 1 to {MAX_WIDTH} logits, got {width}")
-    if width > 1 and rows > 0 and logits.stride(1) != 1:
+    if step != 1 and width > 1 and rows > 0:
         raise _abi.AigAbiError(f"{what} takes rows of adjacent logits, got strides {logits.stride()}")
-    return rows, width, int(logits.stride(0)) if rows > 1 else width, _DTYPES[logits.dtype]
+    return rows, width, ld if rows > 1 else width, dtype
 
 
-def _side(t: Optional[torch.Tensor], shape: tuple, dtype: torch.dtype, like: torch.Tensor, what: str):
-    """Pointer of an operand beside the logits (None stays NULL)."""
+def _side(t: Optional[torch.Tensor], shape: tuple, dtype: torch.dtype, device: torch.device, what: str) -> Optional[int]:
+    """Address of an operand beside the logits (None stays NULL)."""
     if t is None:
         return None
-    if not torch.is_tensor(t) or t.device != like.device or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if torch.is_tensor(t) else type(t).__name__
-        raise _abi.AigAbiError(f"{what} must be a contiguous {dtype} tensor of shape {shape} on {like.device}, got {got}")
-    return C.c_void_p(t.data_ptr())
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise _abi.AigAbiError(f"{what} must be a contiguous {dtype} tensor of shape {shape} on {device}, got {got}")
+    return t.data_ptr()
 
 
-def _on(t: torch.Tensor):
-    """The tensor's device as the current one, where it is not already."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _data(t: torch.Tensor):
-    return C.c_void_p(t.data_ptr())
+def _call(name: str, device: torch.device, *args, meta=None) -> None:
+    """An entry point of the library on the current stream of ``device`` (the last argument of all of them)."""
+    fn = getattr(_abi.lib(), name)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _abi.check(_abi.timed(name, fn, *args, _abi.stream(), meta=meta), name)
+    rc = _abi.timed(name, fn, *args, _abi.stream(), meta=meta)
+    if rc:
+        _abi.check(rc, name)
 
 
 # ------------------------------------------------------------------ sampling
-def sampling_arg(how: Sampling, rows: int, like: torch.Tensor) -> _abi.Sampling:
-    """The argument block of a draw's settings; tensors must outlive the call that takes it."""
+def _setting(name: str, v):
+    v = int(v) if name == "top_k" else float(v)
+    if v != v or v < 0:
+        raise ValueError(f"{name} must not be negative, got {v}")
+    if name in ("top_p", "min_p") and v > 1:
+        raise ValueError(f"{name} is a share of 1, got {v}")
+    return min(v, 2 ** 31 - 1) if name == "top_k" else v
+
+
+@functools.lru_cache(maxsize=64)
+def _settings_of_all(temperature, top_k, top_p, min_p) -> _abi.Sampling:
+    return _abi.Sampling(temperature=_setting("temperature", temperature), top_k=_setting("top_k", top_k),
+                         top_p=_setting("top_p", top_p), min_p=_setting("min_p", min_p))
+
+
+_SETTING_TYPES = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32))
+
+
+def sampling_arg(how: Sampling, rows: int, device: torch.device) -> _abi.Sampling:
+    """The argument block of a draw's settings; tensors among them must outlive the call that takes it."""
+    if not any(isinstance(v, torch.Tensor) for v in how):
+        return _settings_of_all(*how)
     a = _abi.Sampling()
-    for name, dtype in (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32)):
-        v = getattr(how, name)
-        if torch.is_tensor(v):
-            setattr(a, name + "_rows", _side(v, (rows,), dtype, like, name))
-            continue
-        v = int(v) if name == "top_k" else float(v)
-        if v != v or v < 0:
-            raise ValueError(f"{name} must not be negative, got {v}")
-        if name in ("top_p", "min_p") and v > 1:
-            raise ValueError(f"{name} is a share of 1, got {v}")
-        setattr(a, name, min(v, 2 ** 31 - 1) if name == "top_k" else v)
+    for (name, dtype), v in zip(_SETTING_TYPES, how):
+        if isinstance(v, torch.Tensor):
+            setattr(a, name + "_rows", _side(v, (rows,), dtype, device, name))
+        else:
+            setattr(a, name, _setting(name, v))
     return a
 
 
-@torch.no_grad()
 def sample_rows(logits: torch.Tensor, u: torch.Tensor, counts: Optional[torch.Tensor] = None, want: Optional[torch.Tensor] = None,
                 temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
     """Draws ``u.size(1)`` (1 to 8) places of each row without replacement: int32 ``[rows, draws]``, -1 where nothing is
@@ -129,23 +146,20 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, counts: Optional[torch.Te
     are numbers or tensors with one value a row (float32; ``top_k`` int32; values outside their range count as the
     nearest inside)."""
     rows, width, ld, dtype = _rows_of(logits, "sample_rows")
-    if not torch.is_tensor(u) or u.dim() != 2 or not 1 <= int(u.size(1)) <= MAX_DRAWS:
+    device = logits.device
+    if not isinstance(u, torch.Tensor) or u.dim() != 2 or not 1 <= u.size(1) <= MAX_DRAWS:
         raise _abi.AigAbiError(f"sample_rows takes u as [rows, 1 to {MAX_DRAWS} draws]")
-    draws = int(u.size(1))
-    u_ptr = _side(u, (rows, draws), torch.float32, logits, "u")
-    counts_ptr = _side(counts, (rows,), torch.int32, logits, "counts")
-    want_ptr = _side(want, (rows,), torch.int32, logits, "want")
-    how = sampling_arg(Sampling(temperature, top_k, top_p, min_p), rows, logits)
-    out = torch.empty((rows, draws), dtype=torch.int32, device=logits.device)
-    with _on(logits):
-        _abi.check(_abi.timed("aig_sample_rows", _abi.lib().aig_sample_rows, rows, width, ld, dtype, _data(logits), counts_ptr,
-                              want_ptr, C.byref(how), draws, u_ptr, _data(out), _abi.stream(), meta=(rows, width)),
-                   "aig_sample_rows")
+    draws = u.size(1)
+    how = sampling_arg(Sampling(temperature, top_k, top_p, min_p), rows, device)
+    u_ptr = _side(u, (rows, draws), torch.float32, device, "u")
+    counts_ptr, want_ptr = (_side(v, (rows,), torch.int32, device, what) for v, what in ((counts, "counts"), (want, "want")))
+    out = torch.empty((rows, draws), dtype=torch.int32, device=device)
+    _call("aig_sample_rows", device, rows, width, ld, dtype, logits.data_ptr(), counts_ptr, want_ptr, C.byref(how), draws, u_ptr,
+          out.data_ptr(), meta=(rows, width))
     return out
 
 
 # ------------------------------------------------------------------ a teacher's top logits
-@torch.no_grad()
 def top_rows(logits: torch.Tensor, m: int, counts: Optional[torch.Tensor] = None, temperature: float = 1.0) -> TopRows:
     """The ``m`` (1 to 256) largest logits of each row, largest first, equal ones by lowest place: ``values`` float32 and
     ``index`` int32 ``[rows, m]`` (absent entries ``-inf`` and -1), and ``lse``, float32 ``[rows]``, the log-sum-exp of the
@@ -156,28 +170,20 @@ def top_rows(logits: torch.Tensor, m: int, counts: Optional[torch.Tensor] = None
         raise ValueError(f"top_rows keeps 1 to {MAX_TOP} logits a row, got {m}")
     if not 0 < temperature < math.inf:
         raise ValueError(f"the temperature must be positive and finite, got {temperature}")
-    counts_ptr = _side(counts, (rows,), torch.int32, logits, "counts")
-    values = torch.empty((rows, m), dtype=torch.float32, device=logits.device)
-    index = torch.empty((rows, m), dtype=torch.int32, device=logits.device)
-    lse = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    with _on(logits):
-        _abi.check(_abi.timed("aig_top_rows", _abi.lib().aig_top_rows, rows, width, ld, dtype, _data(logits), counts_ptr, m, temperature,
-                              _data(values), _data(index), _data(lse), _abi.stream(), meta=(rows, width)), "aig_top_rows")
+    device = logits.device
+    counts_ptr = _side(counts, (rows,), torch.int32, device, "counts")
+    values = torch.empty((rows, m), dtype=torch.float32, device=device)
+    index = torch.empty((rows, m), dtype=torch.int32, device=device)
+    lse = torch.empty(rows, dtype=torch.float32, device=device)
+    _call("aig_top_rows", device, rows, width, ld, dtype, logits.data_ptr(), counts_ptr, m, temperature, values.data_ptr(),
+          index.data_ptr(), lse.data_ptr(), meta=(rows, width))
     return TopRows(values, index, lse, temperature)
 
 
 # ------------------------------------------------------------------ distillation
-class _Teacher(NamedTuple):
-    values: torch.Tensor
-    index: torch.Tensor
-    lse: Optional[torch.Tensor]
-    counts: Optional[torch.Tensor]
-    weight: Optional[torch.Tensor]
-    temperature: float
-
-
-def _teacher(logits, top, counts, weight, temperature, tail) -> _Teacher:
-    rows, width, _, _ = _rows_of(logits, "distill_loss")
+def _teacher(logits, top, counts, weight, temperature, tail, scale=1.0):
+    """The argument block of a distillation, and the tensors it points to (they must outlive the calls that take it)."""
+    rows, width, ld, dtype = _rows_of(logits, "distill_loss")
     temperature = float(temperature)
     if not 0 < temperature < math.inf:
         raise ValueError(f"the temperature must be positive and finite, got {temperature}")
@@ -195,64 +201,61 @@ def _teacher(logits, top, counts, weight, temperature, tail) -> _Teacher:
             raise ValueError(f"the teacher's log-sum-exp was taken at temperature {taken_at}, the loss is asked for at {temperature}")
     else:
         lse = None
-    for name, t, shape, dtype in (("values", values, (rows, m), torch.float32), ("index", index, (rows, m), torch.int32),
-                                  ("lse", lse, (rows,), torch.float32), ("counts", counts, (rows,), torch.int32),
-                                  ("weight", weight, (rows,), torch.float32)):
-        _side(t, shape, dtype, logits, name)
-    return _Teacher(values.detach(), index, None if lse is None else lse.detach(), counts,
-                    None if weight is None else weight.detach(), temperature)
+    device, one, i32, f32 = logits.device, (rows,), torch.int32, torch.float32
+    a = _abi.Distill(rows, width, ld, m, dtype, temperature, scale, logits.data_ptr(), _side(counts, one, i32, device, "counts"),
+                     _side(values, (rows, m), f32, device, "values"), _side(index, (rows, m), i32, device, "index"),
+                     _side(lse, one, f32, device, "lse"), _side(weight, one, f32, device, "weight"))
+    return a, (counts, values, index, lse, weight)
 
 
-def _distill(logits: torch.Tensor, t: _Teacher, loss: Optional[torch.Tensor], grad: Optional[torch.Tensor],
-             upstream: Optional[torch.Tensor] = None) -> None:
-    rows, width, ld, dtype = _rows_of(logits, "distill_loss")
-    a = _abi.Distill()
-    a.rows, a.width, a.ld, a.m = rows, width, ld, int(t.values.size(1))
-    a.dtype, a.temperature = dtype, t.temperature
-    a.logits = logits.data_ptr()
-    for name in ("counts", "values", "index", "lse", "weight"):
-        v = getattr(t, name)
-        setattr(a, name, None if v is None else v.data_ptr())
-    with _on(logits):
-        _abi.check(_abi.timed("aig_distill_rows", _abi.lib().aig_distill_rows, C.byref(a), None if loss is None else _data(loss),
-                              None if grad is None else _data(grad), width, None if upstream is None else _data(upstream),
-                              0 if upstream is None or upstream.numel() == 1 else 1, _abi.stream(), meta=(rows, width)),
-                   "aig_distill_rows")
+_HELD = ("counts", "values", "index", "lse", "weight")
 
 
-def _sum_rows(v: torch.Tensor, factor: float) -> torch.Tensor:
-    lib = _abi.lib()
+def _distill(device, a: _abi.Distill, loss, grad, upstream=None) -> None:
+    _call("aig_distill_rows", device, C.byref(a), None if loss is None else loss.data_ptr(), None if grad is None else grad.data_ptr(),
+          a.width, None if upstream is None else upstream.data_ptr(), 0 if upstream is None or upstream.numel() == 1 else 1,
+          meta=(a.rows, a.width))
+
+
+def _sum_rows(v: torch.Tensor) -> torch.Tensor:
     out = torch.empty((), dtype=torch.float32, device=v.device)
-    need = lib.aig_sum_rows_ws_bytes(v.numel())
+    need = _abi.lib().aig_sum_rows_ws_bytes(v.numel())
     ws = _abi.workspace(need, v.device) if need else None
-    with _on(v):
-        _abi.check(lib.aig_sum_rows(v.numel(), _data(v), factor, _data(out), None if ws is None else _data(ws), need, _abi.stream()),
-                   "aig_sum_rows")
+    _call("aig_sum_rows", v.device, v.numel(), v.data_ptr(), 1.0, out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out
+
+
+def _refuse_second_derivative(what: str) -> None:
+    if torch.is_grad_enabled():        # (a backward pass runs with it on only when its own graph is asked for)
+        raise RuntimeError(f"{what} can be differentiated once: call backward without create_graph")
 
 
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher, factor):
-        rows = int(logits.size(0))
-        loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
-        _distill(logits, teacher, loss, None)
-        ctx.save_for_backward(logits, *(v for v in teacher[:5] if v is not None))
-        ctx.present, ctx.temperature, ctx.factor = [v is not None for v in teacher[:5]], teacher.temperature, factor
-        return loss if factor is None else _sum_rows(loss, factor)
+    def forward(ctx, logits, arg, held, reduce):
+        loss = torch.empty(arg.rows, dtype=torch.float32, device=logits.device)
+        if ctx.needs_input_grad[0] and arg.width > NARROW:
+            ctx.stats = torch.empty((arg.rows, 8), dtype=torch.float32, device=logits.device)
+            arg.stats = ctx.stats.data_ptr()
+        _distill(logits.device, arg, loss, None)
+        ctx.save_for_backward(logits, *held)
+        ctx.arg = arg
+        return _sum_rows(loss) if reduce else loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, *rest = ctx.saved_tensors
-        rest = iter(rest)
-        teacher = _Teacher(*(next(rest) if here else None for here in ctx.present), ctx.temperature)
+        _refuse_second_derivative("distill_loss")
+        logits, *held = ctx.saved_tensors
+        a = ctx.arg
+        a.logits = logits.data_ptr()       # (hooks on saved tensors may hand out copies)
+        for name, v in zip(_HELD, held):
+            if v is not None:
+                setattr(a, name, v.data_ptr())
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        g = g.float().contiguous()
-        if ctx.factor is not None and ctx.factor != 1.0:
-            g = g * ctx.factor
-        _distill(logits, teacher, None, grad, g)
-        return grad, None, None
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.float().contiguous()
+        _distill(logits.device, a, None, grad, g)
+        return grad, None, None, None
 
 
 def distill_loss(logits: torch.Tensor, top: TopRows, counts: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
@@ -271,76 +274,75 @@ def distill_loss(logits: torch.Tensor, top: TopRows, counts: Optional[torch.Tens
     (float32 ``[rows]``), "sum" or "mean" (over the rows)."""
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"reduction is 'none', 'sum' or 'mean', got {reduction!r}")
-    t = _teacher(logits, top, counts, weight, temperature, tail)
-    rows = int(logits.size(0))
+    rows = int(logits.size(0)) if torch.is_tensor(logits) and logits.dim() else 0
     if reduction == "mean" and rows == 0:
         raise ValueError("the mean over no rows")
-    return _DistillLoss.apply(logits, t, None if reduction == "none" else 1.0 if reduction == "sum" else 1.0 / rows)
+    arg, held = _teacher(logits, top, counts, weight, temperature, tail, 1.0 / rows if reduction == "mean" else 1.0)
+    return _DistillLoss.apply(logits, arg, held, reduction != "none")
 
 
-@torch.no_grad()
 def distill_loss_and_grad(logits: torch.Tensor, top: TopRows, counts: Optional[torch.Tensor] = None,
                           weight: Optional[torch.Tensor] = None, temperature: float = 1.0,
                           tail: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """``distill_loss`` of every row (float32 ``[rows]``) and the gradient of their sum w.r.t. the logits (in the logits'
     type), in one pass over the logits and without an autograd graph: what a training step needs, and what a HIP graph
     can record.  A mean over rows, or any other weighting, goes into ``weight``."""
-    t = _teacher(logits, top, counts, weight, temperature, tail)
-    loss = torch.empty(int(logits.size(0)), dtype=torch.float32, device=logits.device)
+    arg, held = _teacher(logits, top, counts, weight, temperature, tail)
+    loss = torch.empty(arg.rows, dtype=torch.float32, device=logits.device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _distill(logits, t, loss, grad)
+    _distill(logits.device, arg, loss, grad)
     return loss, grad
 
 
 # ------------------------------------------------------------------ scores by class
-def _windows_arg(table: torch.Tensor, w: ScoreWindows) -> _abi.ScoreWindowsArg:
-    if not torch.is_tensor(table) or not table.is_cuda:
-        raise _abi.AigAbiError("class_scores needs the table on a HIP device (no CPU path exists)")
-    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
-        raise _abi.AigAbiError(f"class_scores takes a contiguous float32 table [kinds, classes], got {table.dtype} {tuple(table.shape)}")
-    if w.cand.dim() != 2 or w.cls.dim() != 1:
+def _windows_arg(like: torch.Tensor, kinds: int, classes: int, w: ScoreWindows) -> _abi.ScoreWindowsArg:
+    if not torch.is_tensor(like) or not like.is_cuda:
+        raise _abi.AigAbiError("class_scores needs its tensors on a HIP device (no CPU path exists)")
+    if not torch.is_tensor(w.cand) or not torch.is_tensor(w.cls) or w.cand.dim() != 2 or w.cls.dim() != 1:
         raise _abi.AigAbiError("class_scores takes cand [rows, width] and cls [nodes]")
-    a = _abi.ScoreWindowsArg()
-    a.rows, a.width, a.nodes = int(w.cand.size(0)), int(w.cand.size(1)), int(w.cls.size(0))
-    a.kinds, a.classes = int(table.size(0)), int(table.size(1))
-    i32 = torch.int32
-    for name, shape in (("cand", (a.rows, a.width)), ("counts", (a.rows,)), ("cls", (a.nodes,)), ("row_kind", (a.rows,)),
-                        ("by_kind", (a.rows,)), ("kind_start", (a.kinds + 1,))):
-        setattr(a, name, _side(getattr(w, name), shape, i32, table, name))
-    return a
+    (rows, width), (nodes,), device, i32 = w.cand.shape, w.cls.shape, like.device, torch.int32
+    return _abi.ScoreWindowsArg(rows, width, nodes, kinds, classes, _side(w.cand, (rows, width), i32, device, "cand"),
+                                _side(w.counts, (rows,), i32, device, "counts"), _side(w.cls, (nodes,), i32, device, "cls"),
+                                _side(w.row_kind, (rows,), i32, device, "row_kind"), _side(w.by_kind, (rows,), i32, device, "by_kind"),
+                                _side(w.kind_start, (kinds + 1,), i32, device, "kind_start"))
 
 
 class _ClassScores(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, windows):
-        a = _windows_arg(table, windows)
+    def forward(ctx, table, windows, a):
         out = torch.empty((a.rows, a.width), dtype=torch.float32, device=table.device)
-        with _on(table):
-            _abi.check(_abi.timed("aig_class_scores", _abi.lib().aig_class_scores, C.byref(a), _data(table), _data(out), _abi.stream(),
-                                  meta=(int(a.rows), int(a.width))), "aig_class_scores")
-        ctx.windows, ctx.shape = windows, tuple(table.shape)
+        _call("aig_class_scores", table.device, C.byref(a), table.data_ptr(), out.data_ptr(), meta=(a.rows, a.width))
+        ctx.save_for_backward(*windows)
+        ctx.arg = a
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        return class_scores_grad(g.float().contiguous(), ctx.windows, *ctx.shape), None
+        _refuse_second_derivative("class_scores")
+        a, held = ctx.arg, ctx.saved_tensors
+        for name, v in zip(ScoreWindows._fields, held):
+            if v is not None:
+                setattr(a, name, v.data_ptr())
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.float().contiguous()
+        return _table_grad(g, a), None, None
 
 
-@torch.no_grad()
+def _table_grad(g: torch.Tensor, a: _abi.ScoreWindowsArg) -> torch.Tensor:
+    out = torch.empty((a.kinds, a.classes), dtype=torch.float32, device=g.device)
+    need = _abi.lib().aig_class_scores_bwd_ws_bytes(a.rows, a.width, a.kinds, a.classes)
+    ws = _abi.workspace(need, g.device)
+    _call("aig_class_scores_bwd", g.device, C.byref(a), g.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), meta=(a.rows, a.width))
+    return out
+
+
 def class_scores_grad(grad: torch.Tensor, windows: ScoreWindows, kinds: int, classes: int) -> torch.Tensor:
     """The gradient of ``class_scores``' table for a gradient of its output (float32 ``[rows, width]``): float32
-    ``[kinds, classes]``, the sum over the rows of a kind and their places of a class - sums in a fixed order."""
-    lib = _abi.lib()
-    out = torch.empty((kinds, classes), dtype=torch.float32, device=grad.device)
-    a = _windows_arg(out, windows)
-    g_ptr = _side(grad, (int(a.rows), int(a.width)), torch.float32, out, "grad")
-    need = lib.aig_class_scores_bwd_ws_bytes(a.rows, kinds, classes)
-    ws = _abi.workspace(need, grad.device)
-    with _on(grad):
-        _abi.check(_abi.timed("aig_class_scores_bwd", lib.aig_class_scores_bwd, C.byref(a), g_ptr, _data(out), _data(ws), ws.numel(),
-                              _abi.stream(), meta=(int(a.rows), int(a.width))), "aig_class_scores_bwd")
-    return out
+    ``[kinds, classes]``, the sum over the rows of a kind and their places of a class - sums in a fixed order.  What of
+    ``grad`` lies past a row's count is not read as a value."""
+    a = _windows_arg(grad, kinds, classes, windows)
+    _side(grad, (a.rows, a.width), torch.float32, windows.cand.device, "grad")
+    return _table_grad(grad, a)
 
 
 def class_scores(table: torch.Tensor, windows: ScoreWindows) -> torch.Tensor:
@@ -348,4 +350,8 @@ def class_scores(table: torch.Tensor, windows: ScoreWindows) -> torch.Tensor:
     the candidate, differentiable in the table: nodes with equal feature rows score alike, so a template's candidate
     logits are a table of a few entries.  Places past a row's count, and candidates, classes or kinds outside their range,
     are ``-inf``."""
-    return _ClassScores.apply(table, windows)
+    if not torch.is_tensor(table) or not table.is_cuda:
+        raise _abi.AigAbiError("class_scores needs the table on a HIP device (no CPU path exists)")
+    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise _abi.AigAbiError(f"class_scores takes a contiguous float32 table [kinds, classes], got {table.dtype} {tuple(table.shape)}")
+    return _ClassScores.apply(table, windows, _windows_arg(table, int(table.size(0)), int(table.size(1)), windows))

@@ -709,7 +709,7 @@ int aig_top_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const void*
 /* Distillation.  y = l / T over a student row's valid places, p = softmax(y); the teacher's row gives m entries (logit t_j,
  * place i_j; an entry whose place is not one of the row's, or whose logit is -inf, is absent), q_j = exp(t_j/T - lse[r]) -
  * with lse NULL the log-sum-exp of the entries themselves.
- *   loss[r] = weight[r] T^2 ( sum_j q_j (log q_j - log p[i_j]) + q_R (log q_R - log p_R) )
+ *   loss[r] = scale weight[r] T^2 ( sum_j q_j (log q_j - log p[i_j]) + q_R (log q_R - log p_R) )
  *   grad    = dloss[r]/dl, times upstream[r * upstream_stride] when given (stride 0: one factor for all rows)
  * R: the valid places no entry names, taken as one outcome with the teacher's remaining q_R = 1 - sum_j q_j (with lse
  * given and R not empty; else left out).  A row without valid places or entries: loss 0, gradient 0.  Places past a row's
@@ -720,12 +720,16 @@ typedef struct aig_distill {
     int64_t rows, width, ld, m;
     int32_t dtype;
     float temperature;            /* positive, finite */
+    float scale;                  /* factor of every loss and gradient (1, or 1/rows for a mean) */
     const void* logits;
     const int32_t* counts;        /* may be NULL */
     const float* values;          /* [rows,m] */
     const int32_t* index;         /* [rows,m] */
     const float* lse;             /* [rows] or NULL */
     const float* weight;          /* [rows] or NULL (ones) */
+    float* stats;                 /* [8 rows], 8-byte aligned, or NULL: rows of more than 1024 places leave their sums here in a
+                                   * call for the loss alone, and a later call for the gradient alone of the same rows
+                                   * reads them instead of passing over the logits once more */
 } aig_distill;
 int aig_distill_rows(const aig_distill* d, float* loss, void* grad, int64_t grad_ld, const float* upstream,
                      int64_t upstream_stride, void* stream);
@@ -750,7 +754,7 @@ typedef struct aig_score_windows {
     const int32_t* kind_start;
 } aig_score_windows;
 int aig_class_scores(const aig_score_windows* w, const float* table, float* out, void* stream);
-size_t aig_class_scores_bwd_ws_bytes(int64_t rows, int64_t kinds, int64_t classes);
+size_t aig_class_scores_bwd_ws_bytes(int64_t rows, int64_t width, int64_t kinds, int64_t classes);
 int aig_class_scores_bwd(const aig_score_windows* w, const float* grad, float* d_table, void* ws, size_t ws_bytes,
                          void* stream);
 

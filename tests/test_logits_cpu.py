@@ -34,7 +34,7 @@ def test_top_arguments(m, temperature, rc):
 
 
 def distill(**kw):
-    a = _abi.Distill(rows=4, width=8, ld=8, m=2, dtype=0, temperature=1.0, logits=4096, values=4096, index=4096)
+    a = _abi.Distill(rows=4, width=8, ld=8, m=2, dtype=0, temperature=1.0, scale=1.0, logits=4096, values=4096, index=4096)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -69,5 +69,5 @@ def test_class_scores_arguments(kw, rc):
 
 def test_class_scores_workspace_is_checked():
     a = _abi.ScoreWindowsArg(rows=4000, width=8, nodes=5, kinds=2, classes=3, cand=4096, cls=4096, row_kind=4096, by_kind=4096, kind_start=4096)
-    need = _abi.lib().aig_class_scores_bwd_ws_bytes(4000, 2, 3)
+    need = _abi.lib().aig_class_scores_bwd_ws_bytes(4000, 8, 2, 3)
     assert need > 0 and _abi.lib().aig_class_scores_bwd(C.byref(a), P, P, P, need - 1, None) == -2

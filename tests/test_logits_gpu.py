@@ -40,7 +40,7 @@ def check_sample(x, u, counts=None, want=None, **how):
     dev = {k: (v.to(DEV) if torch.is_tensor(v) else v) for k, v in how.items()}
     got = L.sample_rows(x.to(DEV) if not x.is_cuda else x, u.to(DEV), counts=None if counts is None else counts.to(DEV),
                         want=None if want is None else want.to(DEV), **dev).cpu().numpy()
-    xs, us = x.cpu().float().numpy().astype(np.float64), u.numpy().astype(np.float64)
+    xs, us = x.detach().cpu().float().numpy().astype(np.float64), u.numpy().astype(np.float64)
     for r in range(x.size(0)):
         n = x.size(1) if counts is None else min(max(int(counts[r]), 0), x.size(1))
         one = {k: (v[r].item() if torch.is_tensor(v) else v) for k, v in how.items()}
@@ -144,8 +144,12 @@ def test_strides_and_offsets(dtype, width, off, ld):
     check_sample(dense, u, top_p=0.9)
     top, ref = L.top_rows(x, 5), L.top_rows(dense.to(DEV), 5)
     assert all(torch.equal(a, b) for a, b in zip(top[:3], ref[:3]))
-    (l0, g0), (l1, g1) = (L.distill_loss_and_grad(v, ref) for v in (x, dense.to(DEV)))
-    assert torch.equal(l0, l1) and torch.equal(g0, g1)
+    if width <= 1024:
+        (l0, g0), (l1, g1) = (L.distill_loss_and_grad(v, ref) for v in (x, dense.to(DEV)))
+        assert torch.equal(l0, l1) and torch.equal(g0, g1)
+    else:      # (a wide row's sums are taken in an order that its alignment shapes: against 64 bits, not bit for bit)
+        v, i, s = make_teacher(dense, 5, 1.0, 3, None, True)
+        check_distill(x, v, i, s, 1.0)
     same = dense[:1].to(DEV).expand(rows, width)      # one row seen many times
     assert torch.equal(L.top_rows(same, 5).index, L.top_rows(same.contiguous(), 5).index)
 
@@ -196,12 +200,12 @@ def check_distill(x, v, i, s, t, counts=None, weight=None):
     kw = dict(counts=d(counts), weight=d(weight), temperature=t, tail=s is not None)
     top = L.TopRows(d(v), d(i), d(s))
     loss, grad = L.distill_loss_and_grad(d(x), top, **kw)
-    leaf = d(x).requires_grad_(True)
+    leaf = d(x).detach().requires_grad_(True)
     up = torch.randn(x.size(0), generator=rng(9))
     alone = L.distill_loss(leaf, top, reduction="none", **kw)
     alone.backward(up.to(DEV))
     assert torch.equal(alone.detach(), loss) or torch.isnan(loss).any()
-    step, xs, t64 = HALF_STEP[x.dtype], x.float().numpy().astype(np.float64), float(np.float32(t))
+    step, xs, t64 = HALF_STEP[x.dtype], x.detach().cpu().float().numpy().astype(np.float64), float(np.float32(t))
     tiny = 2.0 ** -25 if x.dtype == F16 else 2.0 ** -134      # half of the smallest step near zero
     for r in range(x.size(0)):
         n = x.size(1) if counts is None else int(counts[r])
@@ -268,6 +272,20 @@ def test_distill_special_rows(width):
     far[:, width - 2:] = float("nan")
     v, i, s = make_teacher(x, m, t, 4, counts, True)
     check_distill(far, v, i, s, t, counts)
+
+
+@pytest.mark.parametrize("width", [40, 300, 1500])
+def test_distill_every_unmasked_place_listed(width):
+    """The valid places that are not listed hold nothing: no rest, and their gradient is 0."""
+    x = torch.full((4, width), -math.inf)
+    x[:, ::9] = torch.randn(4, (width + 8) // 9, generator=rng(2))
+    m = min((width + 8) // 9, 256)
+    x[:, 9 * m:] = -math.inf
+    index = (torch.arange(m, dtype=torch.int32) * 9).expand(4, m).contiguous()
+    values = torch.randn(4, m, generator=rng(3))
+    lse = torch.logsumexp(values.double(), 1).float() + 0.25         # the teacher has something left that the student cannot reach
+    loss, grad = check_distill(x, values, index, lse, 1.0)
+    assert torch.isfinite(loss).all() and torch.isfinite(grad).all() and not grad[:, 1::9].any()
 
 
 def test_distill_listed_everywhere_has_no_rest():
