@@ -25,14 +25,17 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half(v); }
 template <> __device__ __forceinline__ __hip_bfloat16 from_float<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
 
-// Order of the logits as whole numbers: larger logit, larger key; 0 for a place that holds nothing (masked, NaN, past the
-// row's count).  The two zeros are one value (x + 0 turns the negative one over).
+// Order of the logits as whole numbers: larger logit, larger key.  A place that holds nothing (masked, NaN, past the row's
+// count) is -inf, whose key is NO_KEY: whatever is above it holds something.  The two zeros are one value (x + 0 turns the
+// negative one over).
+constexpr unsigned NO_KEY = 0x007FFFFFu;
+__device__ __forceinline__ float or_nothing(float v) { return fmaxf(v, -__builtin_inff()); }       // (NaN: the other operand)
 __device__ __forceinline__ unsigned key_of(float v) {
-    const unsigned b = __float_as_uint(v + 0.0f);
-    return v > -__builtin_inff() ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 0u;
+    const int b = __float_as_int(v + 0.0f);
+    return (unsigned)b ^ ((unsigned)(b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(unsigned key) {
-    return key == 0u ? -__builtin_inff() : __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+    return __uint_as_float(key ^ (~(unsigned)((int)key >> 31) | 0x80000000u));
 }
 
 // ---------------------------------------------------------------- lane exchange
@@ -136,10 +139,14 @@ __device__ __forceinline__ void load_values(const T* __restrict__ row, int n, in
 #pragma unroll
         for (int j = 0; j < E / P::PER; ++j) u.w[j] = reinterpret_cast<const typename P::word*>(row + at)[j];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = at + e < n ? as_float(u.t[e]) : -__builtin_inff();
+        for (int e = 0; e < E; ++e) v[e] = as_float(u.t[e]);
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = at + e < n ? as_float(row[at + e]) : -__builtin_inff();
+    }
+    if (at + E > n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = at + e < n ? v[e] : -__builtin_inff();
     }
 }
 
@@ -166,6 +173,78 @@ __device__ __forceinline__ void kth_largest(const unsigned (&key)[E], int k, uns
     for (int e = 0; e < E; ++e) n += key[e] > t;
     thr = t;
     quota = k - all<G>(n, Add());
+}
+
+// The keys of a group in descending order by place (lane 0's first is the largest): a bitonic network.  Blocks that sort the
+// other way hold their keys complemented, so that every exchange puts the larger key first; an exchange between lanes is a
+// lane permutation and a median with 0 or the largest key (that is: the larger, or the smaller).
+template <int X> __device__ __forceinline__ unsigned exchanged(unsigned v, unsigned keep_larger) {
+    unsigned a = v, b;
+    if constexpr (X == 1) b = dpp<0xB1>(v);
+    if constexpr (X == 2) b = dpp<0x4E>(v);
+    if constexpr (X == 4) b = dpp<0x1B>(dpp<0x141>(v));       // 7 - i, then 3 - i inside each four: i ^ 4
+    if constexpr (X == 8) b = dpp<0x128>(v);
+    if constexpr (X == 16) {                                  // (v and the partner's, in either order)
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        a = r[0];
+        b = r[1];
+    }
+    if constexpr (X == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        a = r[0];
+        b = r[1];
+    }
+    return max(min(a, b), min(max(a, b), keep_larger));
+}
+template <int X, int E> __device__ __forceinline__ void exchange_lanes(unsigned (&k)[E], int lane) {
+    const unsigned keep_larger = lane & X ? 0u : 0xFFFFFFFFu;
+#pragma unroll
+    for (int e = 0; e < E; ++e) k[e] = exchanged<X>(k[e], keep_larger);
+    if constexpr (X > 1) exchange_lanes<X / 2, E>(k, lane);
+}
+__device__ __forceinline__ void exchange_places(unsigned& a, unsigned& b) {
+    const unsigned larger = max(a, b);
+    b = min(a, b);
+    a = larger;
+}
+// places D, D/2, .. 1 apart inside a lane; blocks of SIZE alternate in direction (SIZE = E: one block)
+template <int D, int SIZE, int E> __device__ __forceinline__ void exchange_inside(unsigned (&k)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if ((e & D) == 0) {
+            if (SIZE < E && (e & SIZE)) exchange_places(k[e | D], k[e]);
+            else exchange_places(k[e], k[e | D]);
+        }
+    if constexpr (D > 1) exchange_inside<D / 2, SIZE, E>(k);
+}
+template <int SIZE, int E> __device__ __forceinline__ void sort_inside(unsigned (&k)[E]) {
+    if constexpr (SIZE < E) {
+        exchange_inside<SIZE / 2, SIZE, E>(k);
+        sort_inside<SIZE * 2, E>(k);
+    }
+}
+template <int L, int G, int E> __device__ __forceinline__ void sort_lanes(unsigned (&k)[E], int lane) {
+    const unsigned m = (lane & (L / 2) ? 0xFFFFFFFFu : 0u) ^ (L < G && (lane & L) ? 0xFFFFFFFFu : 0u);
+#pragma unroll
+    for (int e = 0; e < E; ++e) k[e] ^= m;
+    exchange_lanes<L / 2, E>(k, lane);
+    exchange_inside<E / 2, E, E>(k);
+    if constexpr (L < G) sort_lanes<L * 2, G, E>(k, lane);
+}
+template <int G, int E> __device__ __forceinline__ void sort_keys(unsigned (&k)[E], int lane) {
+    sort_inside<2, E>(k);
+    const unsigned m = lane & 1 ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) k[e] ^= m;
+    exchange_inside<E / 2, E, E>(k);
+    sort_lanes<2, G, E>(k, lane);
+}
+// the key at a rank of a sorted group: every lane offers its key of that register, the lane that owns the rank is read
+template <int G, int E> __device__ __forceinline__ unsigned at_rank(const unsigned (&k)[E], int rank) {
+    unsigned v = k[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) v = (rank & (E - 1)) == e ? k[e] : v;
+    return __shfl(v, rank / E, G);
 }
 
 // ---------------------------------------------------------------- wide rows

@@ -6,17 +6,17 @@ namespace {
 using namespace rows;
 
 struct Settings {       // of every row, or of each where a pointer is given
-    float temperature, top_p, min_p;
+    float temperature, top_p, min_p, per;       // per: log2(e) / temperature
     int top_k;
     const float *temperature_rows, *top_p_rows, *min_p_rows;
     const int* top_k_rows;
 };
 struct RowSettings {
-    float temperature, top_p, min_p;
+    float temperature, top_p, min_p, per;
     int top_k;
     __device__ __forceinline__ RowSettings(const Settings& s, long long r)
         : temperature(s.temperature_rows ? s.temperature_rows[r] : s.temperature), top_p(s.top_p_rows ? s.top_p_rows[r] : s.top_p),
-          min_p(s.min_p_rows ? s.min_p_rows[r] : s.min_p), top_k(s.top_k_rows ? s.top_k_rows[r] : s.top_k) {}
+          min_p(s.min_p_rows ? s.min_p_rows[r] : s.min_p), per(s.temperature_rows ? (float)(LOG2E / (double)temperature) : s.per), top_k(s.top_k_rows ? s.top_k_rows[r] : s.top_k) {}
     // the smallest weight that min-p and the unit leave
     __device__ __forceinline__ double floor() const { return min_p > 0.0f ? fmax((double)fminf(min_p, 1.0f) * UNIT, 1.0) : 1.0; }
     // the mass that top-p keeps of `total`: a place stays while the mass in front of it is below this; the first always does
@@ -34,8 +34,8 @@ struct SampleRows {
     __device__ __forceinline__ long long plan_row(long long r) const { return period ? r % period : r; }
     __device__ __forceinline__ int count(long long r) const { return counts ? min(max(counts[plan_row(r)], 0), width) : width; }
     __device__ __forceinline__ int wanted(long long r) const { return want ? min(want[plan_row(r)], draws) : draws; }
-    __device__ __forceinline__ double uniform(long long r, int d) const {
-        return fmin(fmax((double)u[r * draws + d], 0.0), 1.0 - 1.0 / 16777216.0);
+    __device__ __forceinline__ float uniform(long long r, int d) const {
+        return fminf(fmaxf(u[r * draws + d], 0.0f), 1.0f - 1.0f / 16777216.0f);
     }
     // the d-th pick of row r (-1: none).  For wiring every fan-in needs an answer: the first pick stands in for a missing
     // second one, the row's last place for a missing first.
@@ -48,82 +48,69 @@ struct SampleRows {
     }
 };
 
-// A group of G lanes per row, the row in registers.
-template <typename T, int G, int E>
-__global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleRows a) {
-    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
-    if (r >= a.rows) return;
-    const int lane = threadIdx.x & (G - 1);
-    const RowSettings how(a.how, r);
-    const int n = a.count(r), want = a.wanted(r);
-    float v[E];
-    load_values<T, E>(x + r * a.ld, n, a.width, a.vec, lane, v);
-    unsigned key[E];
+// Places that a row keeps, of those whose key is the threshold the first `quota` by place: w = 0 for the others.
+template <int G, int E, typename W> __device__ __forceinline__ void keep_first(const unsigned (&key)[E], W (&w)[E], unsigned thr, int quota) {
+    int ties = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) key[e] = key_of(v[e]);
-    int first = -1;
-
-    if (!(how.temperature > 0.0f)) {      // the largest, then the next
-        for (int d = 0; d < a.draws; ++d) {
-            unsigned best = 0;
+    for (int e = 0; e < E; ++e) ties += key[e] == thr;
+    int tie = before<G>(ties);
 #pragma unroll
-            for (int e = 0; e < E; ++e) best = max(best, key[e]);
-            best = all<G>(best, Max());
-            int at = 0x7FFFFFFF;
-#pragma unroll
-            for (int e = E - 1; e >= 0; --e) at = key[e] == best ? lane * E + e : at;
-            at = all<G>(at, Min());
-#pragma unroll
-            for (int e = 0; e < E; ++e) key[e] = lane * E + e == at ? 0u : key[e];
-            if (lane == 0) a.store(r, d, best != 0u && d < want ? at : -1, first, n);
-        }
-        return;
+    for (int e = 0; e < E; ++e) {
+        const bool stays = key[e] > thr || (key[e] == thr && tie < quota);
+        tie += key[e] == thr;
+        w[e] = stays ? w[e] : W(0);
     }
+}
 
-    unsigned top = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) top = max(top, key[e]);
-    top = all<G>(top, Max());
+// The draws of a row as they are defined, in whole weights (f64).  guess: the key at top-p's border or one near it (0: none).
+template <int G, int E>
+__device__ __forceinline__ void exact_draws(const SampleRows& a, const RowSettings& how, long long r, int lane, int n, int want,
+                                            const unsigned (&key)[E], unsigned top, unsigned guess) {
     const double m = (double)value_of(top), per = LOG2E / (double)how.temperature;
     double q[E];
+    int held = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         q[e] = key[e] == top ? UNIT : weight_of(((double)value_of(key[e]) - m) * per);
-        q[e] = key[e] == 0u ? 0.0 : q[e];
+        q[e] = key[e] > NO_KEY ? q[e] : 0.0;
+        held += key[e] > NO_KEY;
     }
-
-    int held = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) held += key[e] != 0u;
     held = all<G>(held, Add());
     if (how.top_k > 0 && how.top_k < held) {
         unsigned thr;
         int quota;
         kth_largest<G, E>(key, how.top_k, thr, quota);
-        int ties = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) ties += key[e] == thr;
-        int tie = before<G>(ties);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const bool stays = key[e] > thr || (key[e] == thr && tie < quota);
-            tie += key[e] == thr;
-            q[e] = stays ? q[e] : 0.0;
-        }
+        keep_first<G, E>(key, q, thr, quota);
     }
-    if (how.top_p < 1.0f) {
+    if (how.top_p < 1.0f && held > 0) {
         double total = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) total += q[e];
         const double p = how.mass(all<G>(total, Add()));
-        // the largest key whose place and everything above it hold mass p: the border
-        unsigned t = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const unsigned c = t | (1u << bit);
+        // the border: the largest key that, with everything above it, holds mass p
+        auto from = [&](unsigned c) {
             double w = 0.0;
 #pragma unroll
             for (int e = 0; e < E; ++e) w += key[e] >= c ? q[e] : 0.0;
-            if (all<G>(w, Add()) >= p) t = c;
+            return all<G>(w, Add());
+        };
+        unsigned t = guess;
+        if (t != 0u) {
+            while (from(t) < p) {              // too high: the next key below
+                unsigned next = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) next = max(next, key[e] < t ? key[e] : 0u);
+                t = all<G>(next, Max());
+            }
+            while (from(t + 1) >= p) {         // too low: the next key above
+                unsigned next = 0xFFFFFFFFu;
+#pragma unroll
+                for (int e = 0; e < E; ++e) next = min(next, key[e] > t ? key[e] : 0xFFFFFFFFu);
+                t = all<G>(next, Min());
+            }
+        } else {
+            for (int bit = 31; bit >= 0; --bit)
+                if (from(t | (1u << bit)) >= p) t |= 1u << bit;
         }
         double above = 0.0;
         int ties = 0;
@@ -145,13 +132,14 @@ __global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleR
 #pragma unroll
     for (int e = 0; e < E; ++e) q[e] = q[e] >= least ? q[e] : 0.0;
 
+    int first = -1;
     for (int d = 0; d < a.draws; ++d) {
         double sum = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) sum += q[e];
         const double total = all<G>(sum, Add());
         double upto = before<G>(sum);
-        const double t = a.uniform(r, d) * total;
+        const double t = (double)a.uniform(r, d) * total;
         int at = -1;                       // one lane's range holds t (none: nothing is left)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -163,6 +151,199 @@ __global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleR
         }
         at = all<G>(at, Max());
         if (lane == 0) a.store(r, d, d < want ? at : -1, first, n);
+    }
+}
+
+// The same in f32, as long as that is certain.  A sum of weights in f32 is off by less than 2^-19 of the row's total: an
+// exponential of -d carries three roundings of d (2^-24 each, times ln 2) and its own last bit, the average of d over the
+// weights of 1024 places is at most 6.5; a sum of 16 in a lane rounds by half of 16 such steps of the lane's, the six steps
+// over the lanes by six of the total: 0.8e-6 + 0.1e-6 + 0.8e-6.  A decision between two numbers that lie further apart than
+// MARGIN of the total is therefore the exact one; a row with a closer one is drawn again in f64 (returns false): one in a
+// hundred, mostly for top-p's border among places of small weight.  What that buys: an f64 exponential alone is 26
+// instructions a place, and sums in f32 take their lane permutations along.
+constexpr float MARGIN = 1.0f / 262144.0f;
+
+template <int G, int E>
+__device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettings& how, long long r, int lane, int n, int want,
+                                            const float (&v)[E], float m, float* lds, unsigned& guess) {
+    const float per = how.per;
+    bool sure = per > 0.0f && per < 1e30f && m < __builtin_inff();
+    float w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = __builtin_amdgcn_exp2f((v[e] - m) * per);
+    const bool by_p = how.top_p < 1.0f;
+    if (by_p || (how.top_k > 0 && how.top_k < a.width)) {
+        // in the order of the keys the places that stay are the first `keep`
+        unsigned key[E], s[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[e] = key[e] = key_of(v[e]);
+        sort_keys<G, E>(s, lane);
+        int keep = how.top_k > 0 ? min(how.top_k, a.width) : a.width;
+        if (by_p) {
+            float ws[E], sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                ws[e] = __builtin_amdgcn_exp2f((value_of(s[e]) - m) * per);
+                ws[e] = lane * E + e < keep ? ws[e] : 0.0f;
+                sum += ws[e];
+            }
+            const float total = all<G>(sum, Add()), p = how.top_p * total, margin = MARGIN * total;
+            float upto = before<G>(sum), nearest = 1e30f;
+            int stay = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                // (the first place always stays; past the last one there is nothing to decide)
+                const float gap = lane * E + e > 0 && lane * E + e < keep ? upto - p : -1e30f;
+                nearest = fminf(nearest, fabsf(gap));
+                stay += gap < 0.0f;
+                upto += ws[e];
+            }
+            sure = sure && nearest > margin;
+            // (places past `keep` were counted as staying)
+            keep = min(keep, all<G>(stay, Add()) - (G * E - keep));
+        }
+        const unsigned thr = at_rank<G, E>(s, keep - 1);
+        if (thr > NO_KEY) {
+            guess = thr;
+            int over = 0, here = 0;       // places over the threshold, and at it
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                over += key[e] > thr;
+                here += key[e] == thr;
+            }
+            const int both = all<G>(over | here << 16, Add()), quota = keep - (both & 0xFFFF);
+            if ((both >> 16) > quota) {
+                int tie = before<G>(here);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const bool at = key[e] == thr;
+                    w[e] = key[e] > thr || (at && tie < quota) ? w[e] : 0.0f;
+                    tie += at;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) w[e] = key[e] >= thr ? w[e] : 0.0f;
+            }
+        }
+    }
+    if (how.min_p > 0.0f) {
+        const float least = fminf(how.min_p, 1.0f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            sure = sure && !(v[e] < m && fabsf(w[e] - least) <= 4.0f * MARGIN * least);
+            w[e] = w[e] >= least ? w[e] : 0.0f;
+        }
+    }
+    if (!all<G>((int)sure, Min())) return false;
+
+    // Draws.  The lane whose places hold t is found from the lanes' sums; its places are then looked through by the group, from
+    // LDS (one a lane).  A lane with few places looks through them by itself.
+    constexpr bool BY_GROUP = E > 4;
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e];
+    if (BY_GROUP) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) lds[lane * E + e] = w[e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    }
+    int first = -1;
+    float margin = 0.0f;
+    for (int d = 0; d < a.draws; ++d) {
+        const float total = all<G>(sum, Add());
+        margin = fmaxf(margin, MARGIN * total);
+        float upto = before<G>(sum);
+        const float t = a.uniform(r, d) * total;
+        int at = -1;
+        if (BY_GROUP) {
+            const int owner = all<G>(t >= upto && t < upto + sum ? lane : -1, Max());
+            const int place = max(owner, 0) * E + (lane & (E - 1));
+            float here = lds[place];
+            here = lane < E ? here : 0.0f;
+            upto = __shfl(upto, max(owner, 0), G);
+            upto += before<G>(here);
+            const bool mine = owner >= 0 && lane < E && t - upto > margin && upto + here - t > margin;
+            at = all<G>(mine ? place : -1, Max());
+            if (mine) lds[place] = 0.0f;
+            const float gone = all<G>(mine ? here : 0.0f, Add());
+            sum = lane == owner ? fmaxf(sum - gone, 0.0f) : sum;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            // the lane's places that end at or before t, and the nearest end to it
+            float end = upto, nearest = fabsf(t - upto);
+            int passed = 0;
+            const bool mine = t >= upto && t < upto + sum;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                end += w[e];
+                nearest = fminf(nearest, fabsf(t - end));
+                passed += t >= end;
+            }
+            const bool clear = mine && nearest > margin;
+            at = all<G>(clear ? lane * E + passed : -1, Max());
+            sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                w[e] = clear && e == passed ? 0.0f : w[e];
+                sum += w[e];
+            }
+        }
+        if (at < 0 && total > 0.0f) return false;       // (no weight left at all: there is no place to draw)
+        if (lane == 0) a.store(r, d, d < want ? at : -1, first, n);
+    }
+    return true;
+}
+
+// A group of G lanes per row, the row in registers.
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleRows a) {
+    __shared__ __attribute__((aligned(16))) float lds[E > 4 ? 256 / G : 1][E > 4 ? G * E : 1];
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
+    if (r >= a.rows) return;
+    const int lane = threadIdx.x & (G - 1);
+    const RowSettings how(a.how, r);
+    const int n = a.count(r), want = a.wanted(r);
+    float v[E];
+    load_values<T, E>(x + r * a.ld, n, a.width, a.vec, lane, v);
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        v[e] = or_nothing(v[e]);
+        m = fmaxf(m, v[e]);
+    }
+    m = all<G>(m, Max());
+    if (!(how.temperature > 0.0f)) {      // the largest, then the next
+        int first = -1;
+        for (int d = 0; d < a.draws; ++d) {
+            int at = 0x7FFFFFFF;
+#pragma unroll
+            for (int e = E - 1; e >= 0; --e) at = v[e] == m ? lane * E + e : at;
+            at = all<G>(at, Min());
+            if (lane == 0) a.store(r, d, m > -__builtin_inff() && d < want ? at : -1, first, n);
+            m = -__builtin_inff();
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                v[e] = lane * E + e == at ? -__builtin_inff() : v[e];
+                m = fmaxf(m, v[e]);
+            }
+            m = all<G>(m, Max());
+        }
+        return;
+    }
+    int first = -1;
+    if (!(m > -__builtin_inff())) {       // nothing in the row
+        for (int d = 0; d < a.draws; ++d)
+            if (lane == 0) a.store(r, d, -1, first, n);
+        return;
+    }
+    unsigned guess = 0;
+    if (!quick_draws<G, E>(a, how, r, lane, n, want, v, m, lds[E > 4 ? threadIdx.x / G : 0], guess)) {
+        unsigned key[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) key[e] = key_of(v[e]);
+        exact_draws<G, E>(a, how, r, lane, n, want, key, key_of(m), guess);
     }
 }
 
@@ -213,7 +394,7 @@ __device__ __forceinline__ unsigned border_key(int n, double target, double* his
         __syncthreads();
         for (int i = threadIdx.x; i < n; i += WIDE_T) {
             const unsigned k = key(i);
-            if (k != 0u && (k & mask) == prefix) unsafeAtomicAdd(&hist[(k >> shift) & 255u], amount(k, i));
+            if (k > NO_KEY && (k & mask) == prefix) unsafeAtomicAdd(&hist[(k >> shift) & 255u], amount(k, i));
         }
         __syncthreads();
         if (threadIdx.x < 64) {
@@ -247,7 +428,7 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     const RowSettings how(a.how, r);
     const int n = a.count(r), want = a.wanted(r);
     x += r * a.ld;
-    auto key = [&](int i) { return key_of(as_float(x[i])); };
+    auto key = [&](int i) { return key_of(or_nothing(as_float(x[i]))); };
     int first = -1;
 
     if (!(how.temperature > 0.0f)) {
@@ -261,10 +442,10 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
             }
             const unsigned top = block.all(best, Max());
             at = block.all(best == top ? at : 0x7FFFFFFF, Min());
-            const int pick = top != 0u && d < want ? at : -1;
+            const int pick = top > NO_KEY && d < want ? at : -1;
             __syncthreads();
             if (threadIdx.x == 0) {
-                picked[d] = top != 0u ? at : -1;
+                picked[d] = top > NO_KEY ? at : -1;
                 a.store(r, d, pick, first, n);
             }
             __syncthreads();
@@ -277,12 +458,12 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     for (int i = threadIdx.x; i < n; i += WIDE_T) {
         const unsigned k = key(i);
         top = max(top, k);
-        held += k != 0u;
+        held += k > NO_KEY;
     }
     top = block.all(top, Max());
     held = block.all(held, Add());
     const double m = (double)value_of(top), per = LOG2E / (double)how.temperature;
-    auto weight = [&](unsigned k) { return k == 0u ? 0.0 : k == top ? UNIT : weight_of(((double)value_of(k) - m) * per); };
+    auto weight = [&](unsigned k) { return k <= NO_KEY ? 0.0 : k == top ? UNIT : weight_of(((double)value_of(k) - m) * per); };
 
     // what top-k keeps: keys over kthr, and the first kquota at it
     unsigned kthr = 0;
@@ -362,7 +543,7 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
             if (threadIdx.x == 0) a.store(r, d, -1, first, n);
             continue;
         }
-        const double t = a.uniform(r, d) * total;
+        const double t = (double)a.uniform(r, d) * total;
         int tile = 0;
         double front = 0.0;
         while (tile + 1 < tiles && front + tile_mass[tile] <= t) front += tile_mass[tile++];
@@ -439,13 +620,13 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
     int held = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        key[e] = key_of(v[e]);
+        key[e] = key_of(or_nothing(v[e]));
         top = max(top, key[e]);
-        held += key[e] != 0u;
+        held += key[e] > NO_KEY;
     }
     top = all<G>(top, Max());
     held = all<G>(held, Add());
-    unsigned thr = 0;
+    unsigned thr = NO_KEY;
     int quota = 0;
     if (a.m < held) kth_largest<G, E>(key, a.m, thr, quota);
     int ties = 0;
@@ -455,7 +636,7 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
     bool stays[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        stays[e] = key[e] > thr || (key[e] != 0u && key[e] == thr && tie < quota);
+        stays[e] = key[e] > thr || (key[e] == thr && tie < quota);
         tie += key[e] == thr;
         mine += stays[e];
     }
@@ -469,9 +650,9 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
     const float m = value_of(top), per = (float)(LOG2E / (double)a.temperature);
     float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += key[e] == 0u ? 0.0f : key[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(key[e]) - m) * per);
+    for (int e = 0; e < E; ++e) s += key[e] <= NO_KEY ? 0.0f : key[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(key[e]) - m) * per);
     s = all<G>(s, Add());
-    if (lane == 0) a.lse[r] = top == 0u ? -__builtin_inff() : m / a.temperature + logf(s);
+    if (lane == 0) a.lse[r] = top <= NO_KEY ? -__builtin_inff() : m / a.temperature + logf(s);
     // (the group's own wave wrote the list: its lanes see it once their writes are through)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
@@ -487,17 +668,17 @@ __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, To
     const long long r = blockIdx.x;
     const int n = a.count(r);
     x += r * a.ld;
-    auto key = [&](int i) { return key_of(as_float(x[i])); };
+    auto key = [&](int i) { return key_of(or_nothing(as_float(x[i]))); };
     unsigned top = 0;
     int held = 0;
     for (int i = threadIdx.x; i < n; i += WIDE_T) {
         const unsigned k = key(i);
         top = max(top, k);
-        held += k != 0u;
+        held += k > NO_KEY;
     }
     top = block.all(top, Max());
     held = block.all(held, Add());
-    unsigned thr = 0;
+    unsigned thr = NO_KEY;
     int quota = 0;
     if (a.m < held) {
         double above;
@@ -514,15 +695,15 @@ __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, To
 #pragma unroll
         for (int e = 0; e < WIDE_E; ++e) {
             k[e] = base + e < n ? key(base + e) : 0u;
-            ties += thr != 0u && k[e] == thr;
-            s += k[e] == 0u ? 0.0f : k[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(k[e]) - m) * per);
+            ties += k[e] == thr;
+            s += k[e] <= NO_KEY ? 0.0f : k[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(k[e]) - m) * per);
         }
         int tie = ties_so_far + block.before(ties, ties_here);
         bool stays[WIDE_E];
 #pragma unroll
         for (int e = 0; e < WIDE_E; ++e) {
-            stays[e] = k[e] > thr || (k[e] != 0u && k[e] == thr && tie < quota);
-            tie += thr != 0u && k[e] == thr;
+            stays[e] = k[e] > thr || (k[e] == thr && tie < quota);
+            tie += k[e] == thr;
             mine += stays[e];
         }
         int at = kept_so_far + block.before(mine, kept_here);
@@ -536,7 +717,7 @@ __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, To
         kept_so_far += kept_here;
     }
     s = block.all(s, Add());
-    if (threadIdx.x == 0) a.lse[r] = top == 0u ? -__builtin_inff() : m / a.temperature + logf(s);
+    if (threadIdx.x == 0) a.lse[r] = top <= NO_KEY ? -__builtin_inff() : m / a.temperature + logf(s);
     __syncthreads();
     write_ranked<WIDE_T>(a, r, lkey, lplace, min(a.m, held), threadIdx.x);
 }
@@ -602,7 +783,7 @@ int launch_sample_rows(hipStream_t s, int64_t rows, int64_t width, int64_t ld, i
     SampleRows a{};
     a.rows = rows; a.ld = ld; a.width = (int)width; a.draws = (int)draws; a.fill = fill; a.period = period;
     a.counts = counts; a.want = want; a.u = u; a.out = out;
-    a.how = Settings{how->temperature, how->top_p, how->min_p, how->top_k, how->temperature_rows, how->top_p_rows,
+    a.how = Settings{how->temperature, how->top_p, how->min_p, (float)(rows::LOG2E / (double)how->temperature), how->top_k, how->temperature_rows, how->top_p_rows,
                      how->min_p_rows, how->top_k_rows};
     if (dtype == AIG_F32) return sample_rows(s, static_cast<const float*>(logits), a);
     if (dtype == AIG_F16) return sample_rows(s, static_cast<const __half*>(logits), a);
