@@ -54,6 +54,28 @@ struct Add { template <typename V> __device__ __forceinline__ V operator()(V a, 
 struct Max { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct Min { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a < b ? a : b; } };
 
+// op over v and the value of the lane 16 (32) apart: the half-swaps of gfx950 put the two side by side, in either order
+template <int X, typename OP> __device__ __forceinline__ unsigned across(unsigned v, OP op) {
+    const auto r = X == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return op((unsigned)r[0], (unsigned)r[1]);
+}
+template <int X, typename OP> __device__ __forceinline__ int across(int v, OP op) {
+    const auto r = X == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return op((int)r[0], (int)r[1]);
+}
+template <int X, typename OP> __device__ __forceinline__ float across(float v, OP op) {
+    const unsigned b = __float_as_uint(v);
+    const auto r = X == 16 ? __builtin_amdgcn_permlane16_swap(b, b, false, false) : __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int X, typename OP> __device__ __forceinline__ double across(double v, OP op) {
+    const long long b = __double_as_longlong(v);
+    const unsigned lo = (unsigned)b, hi = (unsigned)(b >> 32);
+    const auto l = X == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto h = X == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    return op(__longlong_as_double((long long)h[0] << 32 | (unsigned)l[0]), __longlong_as_double((long long)h[1] << 32 | (unsigned)l[1]));
+}
+
 // v over the lanes of a group, in every lane of it
 template <int G, typename V, typename OP> __device__ __forceinline__ V all(V v, OP op) {
     static_assert(G == 16 || G == 64, "groups of 16 or 64 lanes");
@@ -62,8 +84,8 @@ template <int G, typename V, typename OP> __device__ __forceinline__ V all(V v, 
     v = op(v, dpp<0x122>(v));
     v = op(v, dpp<0x121>(v));
     if (G == 64) {
-        v = op(v, __shfl_xor(v, 16));
-        v = op(v, __shfl_xor(v, 32));
+        v = across<16>(v, op);
+        v = across<32>(v, op);
     }
     return v;
 }
@@ -264,7 +286,7 @@ template <typename T> struct Span {
             const float v[PER] = {as_float(x[first])};
             f(first, v, 1);
         }
-#pragma unroll 2
+#pragma unroll 4
         for (int k = first; k < vecs; k += step) {
             union { uint4 w; T t[PER]; } u;
             u.w = reinterpret_cast<const uint4*>(x + head)[k];

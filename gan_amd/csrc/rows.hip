@@ -419,8 +419,10 @@ __device__ __forceinline__ unsigned border_key(int n, double target, double* his
     return prefix;
 }
 
+// Any row of weights that are drawn in parts (no temperature 0): borders bit by bit over the whole row, a handful of
+// passes of f64 weights.  Taken where a list below overflows (thousands of equal logits at a border, top-k of thousands).
 template <typename T>
-__global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x, SampleRows a) {
+__device__ __forceinline__ void general_draws(const T* __restrict__ x, const SampleRows& a) {
     __shared__ double hist[256], found[2], red[WIDE_T / 64 + 1], tile_mass[TILES];
     __shared__ int tile_ties[TILES], picked[8];
     const Block block{red};
@@ -430,28 +432,6 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     x += r * a.ld;
     auto key = [&](int i) { return key_of(or_nothing(as_float(x[i]))); };
     int first = -1;
-
-    if (!(how.temperature > 0.0f)) {
-        for (int d = 0; d < a.draws; ++d) {
-            unsigned best = 0;
-            int at = 0x7FFFFFFF;
-            for (int i = threadIdx.x; i < n; i += WIDE_T) {
-                unsigned k = key(i);
-                for (int j = 0; j < d; ++j) k = picked[j] == i ? 0u : k;
-                if (k > best) { best = k; at = i; }
-            }
-            const unsigned top = block.all(best, Max());
-            at = block.all(best == top ? at : 0x7FFFFFFF, Min());
-            const int pick = top > NO_KEY && d < want ? at : -1;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                picked[d] = top > NO_KEY ? at : -1;
-                a.store(r, d, pick, first, n);
-            }
-            __syncthreads();
-        }
-        return;
-    }
 
     unsigned top = 0;
     int held = 0;
@@ -574,6 +554,354 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     }
 }
 
+// Lists of places picked out of a row, in LDS.
+constexpr int LIST = 1024, LIST_K = 512;
+struct List {
+    unsigned key[LIST];
+    int place[LIST];
+    double q[LIST];
+    int count;
+    __device__ __forceinline__ void add(unsigned k, int i) {
+        const int at = atomicAdd(&count, 1);
+        if (at < LIST) {
+            key[at] = k;
+            place[at] = i;
+        }
+    }
+    // places in front of (k, i) in the order of the keys, then of the places
+    __device__ __forceinline__ int rank(unsigned k, int i, int n) const {
+        int before = 0;
+        for (int j = 0; j < n; ++j) before += key[j] > k || (key[j] == k && place[j] < i);
+        return before;
+    }
+};
+
+// A key that at least k of the row's places reach, few more do: the k-th largest of the threads' own largest (mine: this
+// thread's).  NO_KEY + 1 where fewer than k threads hold a place.
+__device__ __forceinline__ unsigned bound_of_top(unsigned mine, int k, unsigned* keys, unsigned* result) {
+    keys[threadIdx.x] = mine;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        if (k <= 128) {          // (the largest of each four: few more places reach their k-th, and 256 keys sort quickly)
+            unsigned v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[e] = max(v[e], keys[(e * 4 + j) * 64 + threadIdx.x]);
+            }
+            sort_keys<64, 4>(v, threadIdx.x);
+            const unsigned thr = max(at_rank<64, 4>(v, k - 1), NO_KEY + 1);
+            if (threadIdx.x == 0) *result = thr;
+        } else {
+            unsigned v[16];
+            int held = 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                v[e] = keys[e * 64 + threadIdx.x];
+                held += v[e] > NO_KEY;
+            }
+            unsigned thr = NO_KEY + 1;
+            if (k < all<64>(held, Add())) {
+                int quota;
+                kth_largest<64, 16>(v, k, thr, quota);
+                thr += quota == 0;
+            }
+            if (threadIdx.x == 0) *result = thr;
+        }
+    }
+    __syncthreads();
+    return *result;
+}
+
+// Rows up to this width are read place by place (every thread holds some), wider ones by vectors.
+constexpr int BY_PLACE = 8192;
+template <typename T, typename F> __device__ __forceinline__ void each_place(const Span<T>& row, F f) {
+    if (row.n <= BY_PLACE) {
+        for (int i = threadIdx.x; i < row.n; i += WIDE_T) f(i, as_float(row.x[i]));
+    } else {
+        row.each(threadIdx.x, WIDE_T, [&](int i, const float (&v)[Span<T>::PER], int count) {
+#pragma unroll
+            for (int j = 0; j < Span<T>::PER; ++j)
+                if (j < count) f(i + j, v[j]);
+        });
+    }
+}
+
+// A row in parts that follow each other by place: the places in front of its vectors, the 64 vectors of each wave of each
+// sweep of the workgroup over them, the places behind.
+constexpr int PARTS = 2 + 16 * (MAX_WIDTH / (4 * WIDE_T) + 1);
+template <typename T> struct Parts {
+    static constexpr int PER = Span<T>::PER;
+    const Span<T>& row;
+    int sweeps;
+    __device__ __forceinline__ explicit Parts(const Span<T>& r) : row(r), sweeps((r.vecs + WIDE_T - 1) / WIDE_T) {}
+    __device__ __forceinline__ int count() const { return 2 + 16 * sweeps; }
+    __device__ __forceinline__ int of(int place) const {
+        if (place < row.head) return 0;
+        const int k = (place - row.head) / PER;
+        return k < row.vecs ? 1 + 16 * (k / WIDE_T) + (k % WIDE_T) / 64 : 1 + 16 * sweeps;
+    }
+    // the places of a lane in a part: first place, and how many
+    __device__ __forceinline__ int places(int part, int lane, int& first) const {
+        if (part == 0) {
+            first = lane;
+            return lane < row.head ? 1 : 0;
+        }
+        if (part == 1 + 16 * sweeps) {
+            first = row.head + row.vecs * PER + lane;
+            return first < row.n ? 1 : 0;
+        }
+        const int k = ((part - 1) / 16) * WIDE_T + ((part - 1) % 16) * 64 + lane;
+        first = row.head + k * PER;
+        return k < row.vecs ? PER : 0;
+    }
+    __device__ __forceinline__ void load(int first, int n, float (&v)[PER]) const {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = -__builtin_inff();
+        if (n == PER) {
+            union { uint4 w; T t[PER]; } u;
+            u.w = *reinterpret_cast<const uint4*>(row.x + first);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] = or_nothing(as_float(u.t[j]));
+        } else if (n == 1) {
+            v[0] = or_nothing(as_float(row.x[first]));
+        }
+    }
+};
+
+// A workgroup per row.  Weights are whole numbers in f64 throughout, so their sums do not depend on how the row is split.
+//   top-k (to LIST_K): the places that can be among the k largest are picked out into a list, everything else happens there.
+//   otherwise: top-p's border from a histogram of the weights over BINS steps of the logit, the places of its bin in a list;
+//   then the sum of what stays in each part of the row, and for each draw a look through the one part that holds it.
+constexpr int BINS = 4096;
+constexpr float OCTAVES = 37.0f;          // a weight under 2^-37 is 0
+
+template <typename T>
+__global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x, SampleRows a) {
+    constexpr int PER = Span<T>::PER;
+    __shared__ double hist[BINS], part_mass[PARTS], red[WIDE_T / 64 + 1], found[2];
+    __shared__ List list;
+    __shared__ unsigned shared_key;
+    __shared__ int picked[AIG_ROWS_MAX_DRAWS], found_at;
+    const Block block{red};
+    const long long r = blockIdx.x;
+    const RowSettings how(a.how, r);
+    const int n = a.count(r), want = a.wanted(r), t = threadIdx.x;
+    const Span<T> row(x + r * a.ld, n);
+    int first = -1;
+
+    if (!(how.temperature > 0.0f)) {      // the largest, then the next
+        for (int d = 0; d < a.draws; ++d) {
+            unsigned best = 0;
+            int at = 0x7FFFFFFF;
+            each_place(row, [&](int i, float v) {
+                unsigned k = key_of(or_nothing(v));
+                for (int j = 0; j < d; ++j) k = picked[j] == i ? 0u : k;
+                if (k > best) {
+                    best = k;
+                    at = i;
+                }
+            });
+            const unsigned top = block.all(best, Max());
+            at = block.all(best == top ? at : 0x7FFFFFFF, Min());
+            __syncthreads();
+            if (t == 0) {
+                picked[d] = top > NO_KEY ? at : -1;
+                a.store(r, d, top > NO_KEY && d < want ? at : -1, first, n);
+            }
+            __syncthreads();
+        }
+        return;
+    }
+    auto none = [&](int from) {
+        if (t == 0)
+            for (int d = from; d < a.draws; ++d) a.store(r, d, -1, first, n);
+    };
+
+    float m = -__builtin_inff();
+    each_place(row, [&](int, float v) { m = fmaxf(m, or_nothing(v)); });
+    const unsigned my_top = key_of(m);
+    m = block.all(m, Max());
+    if (!(m > -__builtin_inff())) return none(0);
+    const double m64 = (double)m, per = LOG2E / (double)how.temperature;
+    auto weight = [&](float v) { return v == m ? UNIT : v > -__builtin_inff() ? weight_of(((double)v - m64) * per) : 0.0; };
+    const double least = how.floor();
+    const bool by_k = how.top_k > 0 && how.top_k < n, by_p = how.top_p < 1.0f;
+    const float bins_per = (float)per * ((float)BINS / OCTAVES);
+    if ((by_k && how.top_k > LIST_K) || !(bins_per > 0.0f && bins_per < 1e30f && m < __builtin_inff())) return general_draws<T>(x, a);
+    if (t == 0) list.count = 0;
+
+    if (by_k) {
+        const unsigned low = bound_of_top(my_top, how.top_k, list.key, &shared_key);
+        each_place(row, [&](int i, float v) {
+            const unsigned k = key_of(or_nothing(v));
+            if (k >= low) list.add(k, i);
+        });
+        __syncthreads();
+        const int have = list.count;
+        if (have > LIST) return general_draws<T>(x, a);
+        const bool mine = t < have;
+        const unsigned key = mine ? list.key[t] : 0u;
+        const int place = mine ? list.place[t] : -1, rank = mine ? list.rank(key, place, have) : LIST, keep = min(how.top_k, have);
+        double q = rank < keep ? weight(value_of(key)) : 0.0;
+        if (rank < keep) hist[rank] = q;          // in the order of the keys
+        __syncthreads();
+        if (by_p) {
+            double front = 0.0, total = 0.0;
+            for (int j = 0; j < keep; ++j) {
+                const double w = hist[j];
+                front += j < rank ? w : 0.0;
+                total += w;
+            }
+            if (rank > 0 && !(front < how.mass(total))) q = 0.0;
+        }
+        if (q < least) q = 0.0;
+        list.q[t] = q;
+        __syncthreads();
+        double upto = 0.0, total = 0.0;           // in the order of the places
+        for (int j = 0; j < have; ++j) {
+            const double w = list.q[j];
+            upto += list.place[j] < place ? w : 0.0;
+            total += w;
+        }
+        for (int d = 0; d < a.draws; ++d) {
+            if (!(total > 0.0)) return none(d);
+            const double u = (double)a.uniform(r, d) * total;
+            if (q > 0.0 && upto <= u && u < upto + q) {
+                found[0] = q;
+                found_at = place;
+            }
+            __syncthreads();
+            const double gone = found[0];
+            const int at = found_at;
+            total -= gone;
+            if (place > at) upto -= gone;
+            if (place == at) q = 0.0;
+            if (t == 0) a.store(r, d, d < want ? at : -1, first, n);
+            __syncthreads();
+        }
+        return;
+    }
+
+    const Parts<T> parts(row);
+    const int wave = t >> 6, lane = t & 63;
+    auto bin_of = [&](float v) { return (int)fminf((m - v) * bins_per, (float)(BINS - 1)); };
+    int border_bin = BINS;          // places in bins below it stay; of its own places those up to (thr, last) in the order of the keys
+    double above = 0.0, p = 0.0;
+    if (by_p) {
+        for (int i = t; i < BINS; i += WIDE_T) hist[i] = 0.0;
+        __syncthreads();
+        each_place(row, [&](int, float raw) {
+            const float v = or_nothing(raw);
+            const double q = weight(v);
+            if (q > 0.0) unsafeAtomicAdd(&hist[bin_of(v)], q);
+        });
+        __syncthreads();
+        double h[BINS / WIDE_T], sum = 0.0, total;
+#pragma unroll
+        for (int j = 0; j < BINS / WIDE_T; ++j) sum += h[j] = hist[t * (BINS / WIDE_T) + j];
+        double upto = block.before(sum, total);
+        p = how.mass(total);
+#pragma unroll
+        for (int j = 0; j < BINS / WIDE_T; ++j) {
+            if (upto < p && p <= upto + h[j]) {
+                found[0] = upto;
+                found_at = t * (BINS / WIDE_T) + j;
+            }
+            upto += h[j];
+        }
+        __syncthreads();
+        above = found[0];
+        border_bin = found_at;
+    }
+    auto part_sum = [&](int part) {
+        int at;
+        const int here = parts.places(part, lane, at);
+        float v[PER];
+        parts.load(at, here, v);
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (j >= here) break;
+            const int b = bin_of(v[j]);
+            const double q = weight(v[j]);
+            if (b < border_bin) sum += q >= least ? q : 0.0;
+            else if (b == border_bin && q > 0.0) list.add(key_of(v[j]), at + j);
+        }
+        sum = all<64>(sum, Add());
+        if (lane == 0) part_mass[part] = sum;
+    };
+    for (int s = 0; s < parts.sweeps; ++s) part_sum(1 + 16 * s + wave);
+    if (wave == 0) part_sum(0);
+    if (wave == 1) part_sum(1 + 16 * parts.sweeps);
+    __syncthreads();
+    unsigned thr = 0xFFFFFFFFu;
+    int last = -1;
+    if (by_p) {
+        const int have = list.count;
+        if (have > LIST) return general_draws<T>(x, a);
+        const bool mine = t < have;
+        const unsigned key = mine ? list.key[t] : 0u;
+        const int place = mine ? list.place[t] : -1;
+        const double q = mine ? weight(value_of(key)) : 0.0;
+        list.q[t] = q;
+        __syncthreads();
+        double front = above;
+        if (mine)
+            for (int j = 0; j < have; ++j) front += list.key[j] > key || (list.key[j] == key && list.place[j] < place) ? list.q[j] : 0.0;
+        const bool stays = mine && (front == 0.0 || front < p);
+        thr = block.all(stays ? key : 0xFFFFFFFFu, Min());
+        last = block.all(stays && key == thr ? place : -1, Max());
+        if (stays && q >= least) unsafeAtomicAdd(&part_mass[parts.of(place)], q);
+        __syncthreads();
+    }
+    for (int d = 0; d < a.draws; ++d) {
+        const double mass = t < parts.count() ? part_mass[t] : 0.0;
+        double total;
+        const double upto = block.before(mass, total);
+        if (!(total > 0.0)) return none(d);
+        const double u = (double)a.uniform(r, d) * total;
+        if (upto <= u && u < upto + mass) {
+            found[0] = upto;
+            found_at = t;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            const int part = found_at;
+            int at;
+            const int here = parts.places(part, lane, at);
+            float v[PER];
+            parts.load(at, here, v);
+            double q[PER], sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int b = bin_of(v[j]);
+                const unsigned k = key_of(v[j]);
+                // (without branches: as a chain of || this compiler left the assignment of 0 out)
+                const bool stays = (b < border_bin) | ((b == border_bin) & ((k > thr) | ((k == thr) & (at + j <= last))));
+                const double w = weight(v[j]);
+                bool taken = j >= here;
+                for (int i = 0; i < d; ++i) taken |= picked[i] == at + j;
+                q[j] = stays & !taken & (w >= least) ? w : 0.0;
+                sum += q[j];
+            }
+            double end = found[0] + before<64>(sum);
+            const double left = part_mass[part];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (end <= u && u < end + q[j]) {
+                    picked[d] = at + j;
+                    part_mass[part] = left - q[j];
+                }
+                end += q[j];
+            }
+        }
+        __syncthreads();
+        if (t == 0) a.store(r, d, d < want ? picked[d] : -1, first, n);
+    }
+}
+
 // ---------------------------------------------------------------- the largest logits
 struct TopArgs {
     long long rows, ld;
@@ -659,67 +987,86 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
     write_ranked<G>(a, r, lkey, lplace, min(a.m, held), lane);
 }
 
+// A workgroup per row: the places that can be among the m largest are picked out into a list and ranked there.
 template <typename T>
 __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, TopArgs a) {
     __shared__ double hist[256], found[2], red[WIDE_T / 64 + 1];
-    __shared__ unsigned lkey[TOP_MAX];
-    __shared__ int lplace[TOP_MAX];
+    __shared__ List list;
+    __shared__ unsigned shared_key;
     const Block block{red};
     const long long r = blockIdx.x;
-    const int n = a.count(r);
-    x += r * a.ld;
-    auto key = [&](int i) { return key_of(or_nothing(as_float(x[i]))); };
-    unsigned top = 0;
-    int held = 0;
-    for (int i = threadIdx.x; i < n; i += WIDE_T) {
-        const unsigned k = key(i);
-        top = max(top, k);
-        held += k > NO_KEY;
-    }
-    top = block.all(top, Max());
-    held = block.all(held, Add());
-    unsigned thr = NO_KEY;
-    int quota = 0;
-    if (a.m < held) {
-        double above;
-        thr = border_key(n, (double)a.m, hist, found, key, [](unsigned, int) { return 1.0; }, above);
-        quota = a.m - (int)above;
-    }
-    const float m = value_of(top), per = (float)(LOG2E / (double)a.temperature);
-    float s = 0.0f;
-    int ties_so_far = 0, kept_so_far = 0;
-    for (int t = 0; t * TILE < n; ++t) {
-        const int base = t * TILE + (int)threadIdx.x * WIDE_E;
-        unsigned k[WIDE_E];
-        int ties = 0, mine = 0, ties_here, kept_here;
-#pragma unroll
-        for (int e = 0; e < WIDE_E; ++e) {
-            k[e] = base + e < n ? key(base + e) : 0u;
-            ties += k[e] == thr;
-            s += k[e] <= NO_KEY ? 0.0f : k[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(k[e]) - m) * per);
-        }
-        int tie = ties_so_far + block.before(ties, ties_here);
-        bool stays[WIDE_E];
-#pragma unroll
-        for (int e = 0; e < WIDE_E; ++e) {
-            stays[e] = k[e] > thr || (k[e] == thr && tie < quota);
-            tie += k[e] == thr;
-            mine += stays[e];
-        }
-        int at = kept_so_far + block.before(mine, kept_here);
-#pragma unroll
-        for (int e = 0; e < WIDE_E; ++e)
-            if (stays[e] && at < TOP_MAX) {
-                lkey[at] = k[e];
-                lplace[at++] = base + e;
-            }
-        ties_so_far += ties_here;
-        kept_so_far += kept_here;
-    }
-    s = block.all(s, Add());
-    if (threadIdx.x == 0) a.lse[r] = top <= NO_KEY ? -__builtin_inff() : m / a.temperature + logf(s);
+    const int n = a.count(r), t = threadIdx.x;
+    const Span<T> row(x + r * a.ld, n);
+    float m = -__builtin_inff();
+    each_place(row, [&](int, float v) { m = fmaxf(m, or_nothing(v)); });
+    unsigned low = bound_of_top(key_of(m), a.m, list.key, &shared_key);
+    m = block.all(m, Max());
+    if (t == 0) list.count = 0;
     __syncthreads();
-    write_ranked<WIDE_T>(a, r, lkey, lplace, min(a.m, held), threadIdx.x);
+    const float per = (float)(LOG2E / (double)a.temperature);
+    double s = 0.0;
+    int held = 0;
+    each_place(row, [&](int i, float raw) {
+        const float v = or_nothing(raw);
+        const unsigned k = key_of(v);
+        s += v == m ? 1.0 : (double)__builtin_amdgcn_exp2f((v - m) * per);
+        held += k > NO_KEY;
+        if (k >= low && k > NO_KEY) list.add(k, i);
+    });
+    s = block.all(s, Add());
+    held = block.all(held, Add());
+    if (t == 0) a.lse[r] = m > -__builtin_inff() ? m / a.temperature + logf((float)s) : -__builtin_inff();
+    int have = list.count;
+    if (have > LIST) {
+        // thousands of equal logits at the border, or a row of few threads' places: the border bit by bit, then the list by place
+        double above;
+        const unsigned thr = held > a.m ? border_key(n, (double)a.m, hist, found, [&](int i) { return key_of(or_nothing(as_float(row.x[i]))); },
+                                                     [](unsigned, int) { return 1.0; }, above)
+                                        : NO_KEY;
+        const int quota = held > a.m ? a.m - (int)above : 0;
+        int ties_so_far = 0, kept_so_far = 0;
+        for (int tile = 0; tile * TILE < n; ++tile) {
+            const int base = tile * TILE + t * WIDE_E;
+            unsigned k[WIDE_E];
+            int ties = 0, mine = 0, ties_here, kept_here;
+#pragma unroll
+            for (int e = 0; e < WIDE_E; ++e) {
+                k[e] = base + e < n ? key_of(or_nothing(as_float(row.x[base + e]))) : 0u;
+                ties += k[e] == thr;
+            }
+            int tie = ties_so_far + block.before(ties, ties_here);
+            bool stays[WIDE_E];
+#pragma unroll
+            for (int e = 0; e < WIDE_E; ++e) {
+                stays[e] = k[e] > thr || (k[e] == thr && tie < quota);
+                tie += k[e] == thr;
+                mine += stays[e];
+            }
+            int at = kept_so_far + block.before(mine, kept_here);
+#pragma unroll
+            for (int e = 0; e < WIDE_E; ++e)
+                if (stays[e] && at < LIST) {
+                    list.key[at] = k[e];
+                    list.place[at++] = base + e;
+                }
+            ties_so_far += ties_here;
+            kept_so_far += kept_here;
+        }
+        have = min(held, a.m);
+        __syncthreads();
+    }
+    if (t < have) {
+        const unsigned k = list.key[t];
+        const int place = list.place[t], rank = list.rank(k, place, have);
+        if (rank < a.m) {
+            a.values[r * a.m + rank] = value_of(k);
+            a.index[r * a.m + rank] = place;
+        }
+    }
+    for (int j = have + t; j < a.m; j += WIDE_T) {
+        a.values[r * a.m + j] = -__builtin_inff();
+        a.index[r * a.m + j] = -1;
+    }
 }
 
 // ---------------------------------------------------------------- launches

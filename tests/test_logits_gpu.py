@@ -117,15 +117,56 @@ def test_sample_each_row_its_settings_and_want():
         check_sample(x, torch.rand(n, 4, generator=g), counts=make_counts(n, width, 1), want=want, **how)
 
 
-def test_sample_follows_the_probabilities():
-    """Evenly spread random numbers hit every place as often as its probability says, to within one."""
-    for width, N in ((9, 4096), (300, 8192)):
-        x = make_logits(1, width, F32, seed=width).expand(N, width)
-        u = ((torch.arange(N) + 0.5) / N).reshape(N, 1)
-        got = L.sample_rows(x.to(DEV), u.to(DEV), temperature=0.8)[:, 0].cpu().numpy()
-        p = np.exp(x[0].double().numpy() / np.float64(np.float32(0.8)))
+@pytest.mark.parametrize("width,dtype,off", [(9, F32, 0), (64, BF16, 0), (300, F32, 1), (1000, F16, 0), (1025, F16, 3), (5000, F32, 0), (9001, BF16, 1)])
+def test_sample_follows_the_probabilities(width, dtype, off):
+    """Evenly spread random numbers hit every place as often as its probability says, to within one - and never a place
+    that a filter took out."""
+    N, t = 4096, 0.8
+    row = make_logits(1, width + off, dtype, seed=width, ties=width == 1025)
+    x = row.to(DEV)[:, off:].expand(N, width)
+    v = row[0, off:].double().numpy()
+    w = np.exp((v - v.max()) / np.float64(np.float32(t)))
+    u = ((torch.arange(N) + 0.5) / N).reshape(N, 1)
+    order = np.lexsort((np.arange(width), -v))
+    for how in (dict(), dict(min_p=0.1), dict(top_k=5), dict(top_p=0.7), dict(top_p=0.7, min_p=0.2), dict(top_k=40, top_p=0.9)):
+        got = L.sample_rows(x, u.to(DEV), temperature=t, **how)[:, 0].cpu().numpy()
+        keep = order[:how.get("top_k", width)]
+        front = np.concatenate([[0.0], np.cumsum(w[keep])[:-1]])
+        keep = keep[(front < np.float64(np.float32(how["top_p"])) * w[keep].sum()) | (front == 0)] if "top_p" in how else keep
+        keep = keep[w[keep] >= how.get("min_p", 0.0)]
+        p = np.zeros(width)
+        p[keep] = w[keep] / w[keep].sum()
         hits = np.bincount(got, minlength=width)
-        assert np.all(np.abs(hits - N * p / p.sum()) <= 1.0 + 1e-6)
+        assert np.all(np.abs(hits - N * p) <= 1.0 + 1e-6), how
+        assert not hits[p == 0].any(), how
+
+
+@pytest.mark.parametrize("width", [4, 64, 256, 512, 1024, 2048, 16384])
+def test_sample_decisions_on_a_border(width):
+    """Equal logits: random numbers that fall on the borders between places exactly, and a share of the mass that does."""
+    x = torch.full((64, width), 0.25)
+    u = (torch.arange(64) / 64.0).reshape(64, 1)
+    got = check_sample(x, u)
+    assert np.array_equal(got[:, 0], np.arange(64) * width // 64)
+    for p in (0.25, 0.5, 0.75):
+        got = check_sample(x, u, top_p=p)
+        assert got.max() < p * width
+    check_sample(x, u, top_k=width // 2, top_p=0.5, min_p=1.0)
+
+
+@pytest.mark.parametrize("width", [1500, 8200, 40000])
+@pytest.mark.parametrize("ties", [False, True])
+def test_sample_wide_rows_every_way(width, ties):
+    """The list, the histogram, and the general form that takes what overflows them."""
+    x = make_logits(3, width, F32, seed=width, ties=ties)
+    u = torch.rand(3, 3, generator=rng(7))
+    for how in (dict(top_k=1), dict(top_k=200), dict(top_k=512, top_p=0.9), dict(top_k=513), dict(top_k=1400, min_p=0.01, top_p=0.8),
+                dict(top_p=0.3), dict(top_p=0.99, min_p=0.001), dict(top_p=0.9, temperature=0.05), dict(top_p=0.6, temperature=40.0),
+                dict(top_p=0.5, temperature=1e-30), dict(temperature=1e30, top_p=0.5), dict(min_p=0.5), dict(temperature=0.0)):
+        check_sample(x, u, **how)
+    counts = torch.tensor([width, 700, 1], dtype=torch.int32)
+    check_sample(x, u, counts=counts, top_p=0.9)
+    check_sample(x, u, counts=counts, top_k=100)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
