@@ -138,6 +138,7 @@ SIGNATURES = {
     "aig_gen_node_proj_batch_ws_bytes": (SZ, [I64, I64, INT]),
     "aig_gen_node_proj_batch": (INT, [I64, I64, P, INT, P, P, INT, P, P, SZ, P]),
     "aig_gen_wire_batch": (INT, [P, P]),
+    "aig_gen_wire_batch_sampled": (INT, [P, P, P, P]),
     "aig_enforce_batch_ws_bytes": (SZ, [I64, I64, I64]),
     "aig_enforce_batch": (INT, [I64, I64, I64, P, P, P, P, INT, P, I64, P, I64, P, P, P, P, P, SZ, P]),
     "aig_clean_depth_batch": (INT, [I64, I64, I64, P, P, P, P, P, SZ, P]),

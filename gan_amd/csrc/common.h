@@ -144,6 +144,13 @@ int launch_gp_tiles_param_grad(hipStream_t s, int n, const int* row_limit, int L
                                const float* g_h1, const float* g_z1, const float* g_x, float* dW1, float* db1, float* dW2,
                                float* db2, float* ubar_gr, float* partial, float out_scale);
 
+// Draws from rows of logits (rows.hip).  period: counts and want repeat every so many rows (0: one a row); fill: every row
+// gets an answer - the first pick stands in for a missing second one, the last valid place for a missing first.
+int check_row_limits(const char* what, int64_t rows, int64_t width);
+int launch_sample_rows(hipStream_t s, int64_t rows, int64_t width, int64_t ld, int dtype, const void* logits, const int32_t* counts,
+                       const int32_t* want, int64_t period, const aig_sampling* how, int64_t draws, const float* u, bool fill,
+                       int32_t* out);
+
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
 // Direct global -> LDS load of 16 bytes per lane that the compiler's wait-count bookkeeping does not

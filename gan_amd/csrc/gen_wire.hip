@@ -951,21 +951,26 @@ extern "C" int aig_gen_emit_half(int64_t n, int64_t K, int64_t E, const float* x
                     edge_index, edge_attr, x_out, stream);
 }
 
-extern "C" int aig_gen_wire_batch(const aig_gen_wire_set* a, void* stream) {
-    AIG_REQUIRE(a, "aig_gen_wire_batch: null argument block");
+// how / u: fan-ins drawn from the logits (NULL: the tie-exact top-k)
+static int wire_batch(const char* what, const aig_gen_wire_set* a, const aig_sampling* how, const float* u, void* stream) {
+    AIG_REQUIRE(a, "%s: null argument block", what);
     AIG_REQUIRE(a->B >= 1 && a->B <= 65535 && a->n >= 1 && a->K >= 1 && a->ecap >= 1 && (a->cls || a->proj_rows >= a->n),
-                "aig_gen_wire_batch: bad sizes B=%lld n=%lld K=%lld ecap=%lld rows=%lld", (long long)a->B, (long long)a->n,
+                "%s: bad sizes B=%lld n=%lld K=%lld ecap=%lld rows=%lld", what, (long long)a->B, (long long)a->n,
                 (long long)a->K, (long long)a->ecap, (long long)a->proj_rows);
     AIG_REQUIRE(a->B * a->proj_rows < INT_MAX && a->B * a->ecap < INT_MAX && a->n * a->K < INT_MAX,
-                "aig_gen_wire_batch: set too large for 32-bit indices");
+                "%s: set too large for 32-bit indices", what);
     AIG_REQUIRE(a->x && a->order && a->rank && a->want && a->cnt && a->fb && a->eoff && a->cand && a->proj && a->sc2_w &&
                     a->sc2_b && a->at2_w && a->at2_b && a->sel && a->edge_index && a->edge_attr &&
                     a->ecount && a->x_out,
-                "aig_gen_wire_batch: null pointer");
+                "%s: null pointer", what);
     // (the scores need not be stored when they come from the class table and every row is short enough for the
     //  selection kernel's LDS copy: it then forms them itself, and the pass that writes n K logits falls away)
     AIG_REQUIRE(a->logits || (a->cls && a->K <= SEL_CAP),
-                "aig_gen_wire_batch: logits may be NULL only with scores by class (cls) and K <= %d", SEL_CAP);
+                "%s: logits may be NULL only with scores by class (cls) and K <= %d", what, SEL_CAP);
+    if (how) {
+        AIG_REQUIRE(u && a->logits, "%s: drawing fan-ins needs the random numbers and a logits buffer", what);
+        if (const int rc = check_row_limits(what, a->B * a->n, a->K)) return rc;
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int B = (int)a->B, n = (int)a->n, K = (int)a->K;
     GenSet gs{};
@@ -981,8 +986,7 @@ extern "C" int aig_gen_wire_batch(const aig_gen_wire_set* a, void* stream) {
     if (a->cls) {
         AIG_REQUIRE(a->classes >= 1 && a->classes <= a->proj_rows && a->classes * a->classes * a->B < INT_MAX && a->pair_logit &&
                         a->pair_bit,
-                    "aig_gen_wire_batch: classes=%lld needs 1 <= classes <= proj_rows and the two pair tables",
-                    (long long)a->classes);
+                    "%s: classes=%lld needs 1 <= classes <= proj_rows and the two pair tables", what, (long long)a->classes);
         const dim3 tgrid((unsigned)((C * C + 255) / 256), B);
         if (half)
             hipLaunchKernelGGL(k_pair_table<true>, tgrid, dim3(256), 0, s, C, (long long)a->proj_rows, proj, proj + plane,
@@ -1006,7 +1010,11 @@ extern "C" int aig_gen_wire_batch(const aig_gen_wire_set* a, void* stream) {
                           a->sc2_b, a->logits, a->sel, &fused, gs);
         if (rc) return rc;
     }
-    if (a->logits && (rc = launch_select(s, B, n, K, a->logits, a->cnt, a->want, a->sel, fused, gs))) return rc;
+    if (how) {
+        if ((rc = launch_sample_rows(s, (int64_t)B * n, K, K, AIG_F32, a->logits, a->cnt, a->want, a->plan_shared ? n : 0, how, 2, u, true,
+                                     a->sel)))
+            return rc;
+    } else if (a->logits && (rc = launch_select(s, B, n, K, a->logits, a->cnt, a->want, a->sel, fused, gs))) return rc;
     const dim3 grid((unsigned)((n + 255) / 256), B);
     long long* ei = reinterpret_cast<long long*>(a->edge_index);
     long long* ea = reinterpret_cast<long long*>(a->edge_attr);
@@ -1020,4 +1028,13 @@ extern "C" int aig_gen_wire_batch(const aig_gen_wire_set* a, void* stream) {
                            a->x_out, gs, a->ecount, a->cls, C, a->pair_bit);
     AIG_LAUNCH_CHECK();
     return AIG_OK;
+}
+
+extern "C" int aig_gen_wire_batch(const aig_gen_wire_set* a, void* stream) {
+    return wire_batch("aig_gen_wire_batch", a, nullptr, nullptr, stream);
+}
+
+extern "C" int aig_gen_wire_batch_sampled(const aig_gen_wire_set* a, const aig_sampling* how, const float* u, void* stream) {
+    AIG_REQUIRE(how, "aig_gen_wire_batch_sampled: null settings");
+    return wire_batch("aig_gen_wire_batch_sampled", a, how, u, stream);
 }

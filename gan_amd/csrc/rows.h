@@ -9,7 +9,6 @@
 #include "common.h"
 
 namespace aig {
-int check_row_limits(const char* what, int64_t rows, int64_t width);      // rows.hip
 namespace rows {
 
 constexpr int MAX_WIDTH = AIG_ROWS_MAX_WIDTH;

@@ -28,6 +28,7 @@ import torch
 import torch.nn as nn
 
 from . import _abi
+from . import logits as L
 from .data import Data
 
 PI, PO, AND = 0, 1, 2
@@ -173,10 +174,79 @@ class AIGGenerator(nn.Module):
         key = _plan_key(x, nd, int(self.candidate_k))
         plan = template.__dict__.get("_gen_plan")
         if plan is None or plan.key != key:
-            plan = GeneratorPlan.build(x, nd, int(self.candidate_k))
-            plan.key = key
+            # (a template that two generators with windows of their own take turns on - a teacher and its student - keeps
+            #  a plan for each width)
+            others = template.__dict__.setdefault("_gen_plans", {})
+            plan = others.get(key[0])
+            if plan is None or plan.key != key:
+                plan = GeneratorPlan.build(x, nd, int(self.candidate_k))
+                plan.key = key
+                others[key[0]] = plan
             template.__dict__["_gen_plan"] = plan
         return plan
+
+    # ------------------------------------------------------------------ drawn fan-ins
+    def _draw_arg(self, sampling, u, rows: int, dev):
+        """The settings of a draw for ``rows`` slots as the C block, and its random numbers."""
+        if not isinstance(sampling, L.Sampling):
+            raise TypeError("sampling is a gan_amd.logits.Sampling")
+        if u is None:
+            u = torch.rand((rows, 2), device=dev)
+        if not (torch.is_tensor(u) and u.device == dev and u.dtype == torch.float32 and u.numel() == 2 * rows):
+            raise _abi.AigAbiError(f"the random numbers of a draw are float32 [{rows} slots, 2] on {dev}")
+        return L.sampling_arg(sampling, rows, dev), u.reshape(rows, 2).contiguous()
+
+    # ------------------------------------------------------------------ candidate logits with a gradient
+    TRAIN_CLASS_LIMIT = 256      # distinct feature rows up to which the logits can be differentiated (a table entry is 128 channels)
+
+    def score_windows(self, templates):
+        """The candidate windows of templates of one node count, back to back, as ``class_scores`` takes them, and the
+        weight that makes a sum over their slots the mean over the slots that need a fan-in.  Row ``g n + r`` is slot ``r`` of
+        template ``g``; its kind is ``g C + (class of its node)``.  The last few are kept, with the plans they are made of."""
+        st = self._stacked_plans(list(templates), templates[0].x.device)
+        cache = self.__dict__.setdefault("_window_stacks", {})
+        key = tuple(id(p) for p in st["plans"])
+        hit = cache.get(key)
+        if hit is not None and all(a is b for a, b in zip(hit[0], st["plans"])):
+            return hit[1], hit[2], st
+        B, n, C = len(templates), st["n"], st["C"]
+        if not 0 < C <= self.TRAIN_CLASS_LIMIT:
+            raise ValueError(f"candidate logits can be differentiated for templates of 1 to {self.TRAIN_CLASS_LIMIT} distinct "
+                             f"feature rows, got {C}")
+        cls, order = st["cls"].reshape(B, n), st["order"].reshape(B, n).long()
+        graph = torch.arange(B, device=cls.device, dtype=torch.int32)[:, None]
+        kind = (cls.gather(1, order) + graph * C).reshape(-1)
+        cand = (st["cand"].reshape(B, n, -1) + (graph * n)[:, :, None]).reshape(B * n, -1)
+        counts = st["cnt"].reshape(-1)
+        needs = (st["want"].reshape(-1) > 0) & (counts > 0)
+        windows = L.ScoreWindows.of(cand.contiguous(), counts, cls.reshape(-1), kind.contiguous(), B * C)
+        weight = needs.float() / needs.sum().clamp(min=1)
+        if len(cache) >= 4:
+            cache.pop(next(iter(cache)))
+        cache[key] = (list(st["plans"]), windows, weight)
+        return windows, weight, st
+
+    def score_table(self, st, zs: torch.Tensor) -> torch.Tensor:
+        """The scores of (target class, candidate class) pairs of every template, ``[B C, C]``, differentiable in the
+        generator's parameters: the arithmetic of ``forward``'s node pipeline and edge scorer on one row per class
+        (models/generator.py:84-99,115-117), through torch's own linear layers - a few dozen rows."""
+        B, C = zs.size(0), st["C"]
+        z = zs.float().repeat_interleave(C, dim=0)
+        h = self.node_proj(torch.cat([self.node_enc(st["x_cls"]), z], dim=1))
+        first, last = self.edge_scorer[0], self.edge_scorer[2]
+        w = first.weight
+        H = self.hidden_dim
+        source = (h @ w[:, :H].t()).reshape(B, 1, C, H)
+        target = (h @ w[:, H:2 * H].t() + z @ w[:, 2 * H:].t() + first.bias).reshape(B, C, 1, H)
+        return ((torch.relu(source + target) * last.weight.reshape(H)).sum(-1) + last.bias).reshape(B * C, C)
+
+    def candidate_logits(self, templates, zs: torch.Tensor) -> torch.Tensor:
+        """The logits ``forward`` takes its fan-ins from, for templates of one node count, ``[B n, candidate_k]`` (slot
+        after slot, template after template; ``-inf`` past a slot's candidates), differentiable in the generator's
+        parameters."""
+        windows, _, st = self.score_windows(templates)
+        zs = zs.to(windows.cand.device).reshape(len(templates), self.z_dim)
+        return L.class_scores(self.score_table(st, zs), windows)
 
     @torch.no_grad()
     def forward_many(self, template: Data, zs: torch.Tensor) -> list:
@@ -261,8 +331,8 @@ class AIGGenerator(nn.Module):
         return st
 
     @torch.no_grad()
-    def forward_set(self, templates, zs: torch.Tensor):
-        """``self(template, z)`` for a whole set of graphs in five launches: ``templates`` is ONE template (the
+    def forward_set(self, templates, zs: torch.Tensor, sampling=None, u: Optional[torch.Tensor] = None):
+        """``self(template, z)`` (``sampling``, ``u`` ``[B, n, 2]``: as for ``forward``) for a whole set of graphs in five launches: ``templates`` is ONE template (the
         graphs are samples of it that differ in z alone - bulk sampling) or a list of B templates of equal node
         count (the graphs of a padded minibatch), ``zs`` is ``[B, z_dim]``.  Returns a ``GraphSet`` whose graph
         ``g`` holds exactly the tensors ``self(template_g, zs[g])`` returns."""
@@ -301,17 +371,19 @@ class AIGGenerator(nn.Module):
         else:
             C, cls, x_cls = st["C"], st["cls"], st["x_cls"]
         ecap = max(max(Es), 1)
-        _, _, edge_index, edge_attr, ecount, x_out = self._wire_set(B, n, K, ecap, shared, x_all, arrays, zs, C, cls, x_cls)
+        draw = None if sampling is None else self._draw_arg(sampling, u, B * n, dev)
+        _, _, edge_index, edge_attr, ecount, x_out = self._wire_set(B, n, K, ecap, shared, x_all, arrays, zs, C, cls, x_cls, draw=draw)
         out = GraphSet(B, n, ecap, x_out, edge_index, edge_attr, ecount, nd_all, counts_host=Es, x_dtype=first.x.dtype)
         out.order_hint = arrays["rank"]      # every emitted edge runs from an earlier to a later node of this order
         return out
 
-    def _wire_set(self, B, n, K, ecap, shared, x_all, arrays, zs, C, cls, x_cls, h_cond=None, keep=None):
+    def _wire_set(self, B, n, K, ecap, shared, x_all, arrays, zs, C, cls, x_cls, h_cond=None, keep=None, draw=None):
         """Node projections, scores, selection and assembly of B graphs of n nodes (the launches behind ``forward_set``
         and, with B = 1, ``forward``).  When the templates' nodes take at most ``class_limit`` distinct feature rows
         the projections are made per class and pairs are scored through per-graph (source class, target class)
         tables - the same bits, since a projection depends on its own input row only.  ``keep``: a dict that receives
-        the projection planes (and the class-wise h_cond when ``h_cond`` is asked for) for debugging."""
+        the projection planes (and the class-wise h_cond when ``h_cond`` is asked for) for debugging.  ``draw``: settings
+        and random numbers of drawn fan-ins (``_draw_arg``); without, the tie-exact top of each row."""
         lib = _abi.lib()
         dev = x_all.device
         stream = _abi.stream()
@@ -358,7 +430,7 @@ class AIGGenerator(nn.Module):
         # (scores by class and windows short enough for the selection kernel's LDS copy: it forms the scores itself
         #  and the n K logits are never stored - unless the caller wants to look at them)
         logits = None
-        if keep is not None or not by_class or K > SELECT_FORMS_SCORES_MAX_K or B * n < SELECT_FORMS_SCORES_MIN_SLOTS:
+        if keep is not None or draw is not None or not by_class or K > SELECT_FORMS_SCORES_MAX_K or B * n < SELECT_FORMS_SCORES_MIN_SLOTS:
             logits = torch.empty((B, n, K), dtype=torch.float32, device=dev)
             if keep is not None:
                 logits.fill_(float("nan"))
@@ -369,8 +441,12 @@ class AIGGenerator(nn.Module):
         x_out = torch.empty((B * n, 2), dtype=torch.float32, device=dev)
         a.logits, a.sel = _abi.ptr(logits), _abi.ptr(sel)
         a.edge_index, a.edge_attr, a.ecount, a.x_out = _abi.ptr(edge_index), _abi.ptr(edge_attr), _abi.ptr(ecount), _abi.ptr(x_out)
-        _abi.check(_abi.timed("aig_gen_wire_batch", lib.aig_gen_wire_batch, C_.byref(a), stream, meta=(n, B, K)),
-                   "aig_gen_wire_batch")
+        if draw is not None:
+            _abi.check(_abi.timed("aig_gen_wire_batch_sampled", lib.aig_gen_wire_batch_sampled, C_.byref(a), C_.byref(draw[0]),
+                                  _abi.ptr(draw[1]), stream, meta=(n, B, K)), "aig_gen_wire_batch_sampled")
+        else:
+            _abi.check(_abi.timed("aig_gen_wire_batch", lib.aig_gen_wire_batch, C_.byref(a), stream, meta=(n, B, K)),
+                       "aig_gen_wire_batch")
         if keep is not None:
             idx = cls.long() if by_class else None
             keep["proj"] = proj[:, idx] if by_class else proj
@@ -413,7 +489,12 @@ class AIGGenerator(nn.Module):
 
     # ------------------------------------------------------------------ forward
     @torch.no_grad()
-    def forward(self, template: Data, z: torch.Tensor, return_debug: bool = False) -> Data:
+    def forward(self, template: Data, z: torch.Tensor, return_debug: bool = False, sampling=None,
+                u: Optional[torch.Tensor] = None) -> Data:
+        """models/generator.py:101-217.  Extension: with ``sampling`` (a ``gan_amd.logits.Sampling``; settings that are
+        tensors hold one value a slot) every slot's fan-ins are drawn without replacement from its candidate logits, from
+        the random numbers ``u`` (float32 ``[n, 2]`` in processing order; drawn here when None), instead of being its top
+        candidates."""
         lib = _abi.lib()
         dev = template.x.device if hasattr(template, "x") else self.device
         if dev.type != "cuda":
@@ -435,12 +516,13 @@ class AIGGenerator(nn.Module):
         st = _abi.stream()
         f32 = dict(dtype=torch.float32, device=dev)
 
-        if self.class_limit and 0 < plan.C <= self.class_limit and n > 0:
-            # per class: the launches of forward_set for a set of one graph
+        draw = None if sampling is None or n == 0 else self._draw_arg(sampling, u, n, dev)
+        if (draw is not None or self.class_limit and 0 < plan.C <= self.class_limit) and n > 0:
+            # per class (or, where fan-ins are drawn, per node): the launches of forward_set for a set of one graph
             arrays = {name: getattr(plan, name) for name in ("order", "rank", "want", "cnt", "fb", "eoff", "cand")}
             keep = {} if return_debug else None
             logits, sel, ei, ea, _, x_out = self._wire_set(1, n, K, max(E, 1), True, x_in, arrays, z.reshape(1, -1), plan.C,
-                                                           plan.cls, plan.x_cls, h_cond=True if return_debug else None, keep=keep)
+                                                           plan.cls, plan.x_cls, h_cond=True if return_debug else None, keep=keep, draw=draw)
             if x_src.dtype != torch.float32:
                 x_out = x_out.to(x_src.dtype)
             out = Data(x=x_out, edge_index=ei[0, :, :E], edge_attr=ea[0, :E].reshape(-1, 1),

@@ -8,7 +8,8 @@ reference's draw and the set of samples does not depend on how many ranks produc
 under torchrun the samples are dealt to the ranks with no collective at all.  Bulk sampling takes the
 draws in blocks of ``--batch``: a block goes through generator, repair and resync as one set of graphs
 (``sample_sets``); ``--batch 1`` keeps ``--in-flight`` single samples in the air on as many streams
-(``sample_many``).
+(``sample_many``).  ``--temperature`` (with ``--top-k``, ``--top-p``, ``--min-p``) draws every node's fan-ins from its candidate
+logits instead of taking its top candidates; sample i's random numbers come from its own generator, right after its z.
 """
 from __future__ import annotations
 
@@ -26,6 +27,7 @@ from .data import Data
 from .dataset import load_pt_dataset
 from .generator import AIGGenerator
 from .graphset import GraphSet
+from .logits import Sampling
 
 PI, PO, AND = 0, 1, 2
 
@@ -39,15 +41,15 @@ def summarize(d: Data) -> str:
     return f"N={n}, E={e}, PI={counts[0]}, PO={counts[1]}, AND={counts[2]}, inv_edges={inv}"
 
 
-def sample_one(G: AIGGenerator, tpl: Data, z: torch.Tensor) -> Data:
-    """AIGgan.py:104-111: forward, repair, resync."""
+def sample_one(G: AIGGenerator, tpl: Data, z: torch.Tensor, sampling: Optional[Sampling] = None, u=None) -> Data:
+    """AIGgan.py:104-111: forward, repair, resync (``sampling``, ``u``: drawn fan-ins, see ``AIGGenerator.forward``)."""
     with torch.no_grad():
-        raw = G(tpl, z)
+        raw = G(tpl, z, sampling=sampling, u=u)
     return repair_and_resync(raw)   # = resync_attrs(enforce_aig_constraints(raw)), one graph walk fewer
 
 
 def sample_many(G: AIGGenerator, jobs: Iterable[Tuple[Data, Callable[[], torch.Tensor]]], in_flight: int = 4,
-                streams: Optional[List[torch.cuda.Stream]] = None) -> Iterator[Data]:
+                streams: Optional[List[torch.cuda.Stream]] = None, sampling: Optional[Sampling] = None) -> Iterator[Data]:
     """``sample_one`` over many ``(template, draw_z)`` jobs with ``in_flight`` samples in the air.
 
     The repair and the resync of one sample each hold a level-by-level graph walk that keeps a single
@@ -55,8 +57,8 @@ def sample_many(G: AIGGenerator, jobs: Iterable[Tuple[Data, Callable[[], torch.T
     independent, so sample i is enqueued on stream ``i % in_flight`` and only finished (count read,
     resync enqueued) once ``in_flight - 1`` younger samples have been enqueued behind it: the walks of
     a few samples and the dense kernels of another run side by side.  ``draw_z`` is called under the
-    sample's stream.  Results come back in job order, the same tensors ``sample_one`` returns, and
-    the caller's current stream waits for each before it is handed out."""
+    sample's stream (with ``sampling`` it returns ``(z, u)``).  Results come back in job order, the same tensors
+    ``sample_one`` returns, and the caller's current stream waits for each before it is handed out."""
     if in_flight < 1:
         raise ValueError("in_flight must be at least 1")
     cur = torch.cuda.current_stream()
@@ -79,7 +81,8 @@ def sample_many(G: AIGGenerator, jobs: Iterable[Tuple[Data, Callable[[], torch.T
     for i, (tpl, draw_z) in enumerate(jobs):
         st = streams[i % len(streams)]
         with torch.cuda.stream(st), torch.no_grad():
-            pending.append((st, enforce_begin(G(tpl, draw_z()), want_depth=False)))   # the resync replaces it
+            z, u = (draw_z(), None) if sampling is None else draw_z()
+            pending.append((st, enforce_begin(G(tpl, z, sampling=sampling, u=u), want_depth=False)))   # the resync replaces it
         if len(pending) >= len(streams):
             yield finish()
     while pending:
@@ -108,9 +111,10 @@ def _set_streams(device: torch.device, count: int) -> List[torch.cuda.Stream]:
     return have[:count]
 
 
-def sample_sets(G: AIGGenerator, tpl: Data, z_batches: Iterable[torch.Tensor], in_flight: int = 3) -> Iterator[GraphSet]:
-    """Bulk sampling from ONE template: every element of ``z_batches`` is a ``[S, z_dim]`` block of draws that
-    goes through generator, repair and resync as one set of graphs (``AIGGenerator.forward_set``,
+def sample_sets(G: AIGGenerator, tpl: Data, z_batches: Iterable[torch.Tensor], in_flight: int = 3,
+                sampling: Optional[Sampling] = None) -> Iterator[GraphSet]:
+    """Bulk sampling from ONE template: every element of ``z_batches`` is a ``[S, z_dim]`` block of draws (with
+    ``sampling`` a pair of it and the fan-ins' random numbers ``[S, n, 2]``) that goes through generator, repair and resync as one set of graphs (``AIGGenerator.forward_set``,
     ``repair_and_resync_set``): about forty launches per block whatever its size, and one host read (the
     repaired edge counts) that is only awaited once ``in_flight - 1`` younger blocks have been enqueued.
     Block ``i`` runs on stream ``i % in_flight`` (``in_flight`` 1: the caller's stream): the narrow kernels of one
@@ -140,18 +144,21 @@ def sample_sets(G: AIGGenerator, tpl: Data, z_batches: Iterable[torch.Tensor], i
                     v.record_stream(cur)
         return gset
 
-    for i, zs in enumerate(z_batches):
+    for i, block in enumerate(z_batches):
+        zs, us = (block, None) if sampling is None else block
         st = streams[i % len(streams)]
         if st is not cur:
             st.wait_stream(cur)                # the draws (and the template) come from the caller's stream
         with torch.cuda.stream(st), torch.no_grad():
-            gset = repair_and_resync_set(G.forward_set(tpl, zs))
+            gset = repair_and_resync_set(G.forward_set(tpl, zs, sampling=sampling, u=us))
             counts_host = torch.empty(gset.B, dtype=torch.int32, pin_memory=True)
             counts_host.copy_(gset.count, non_blocking=True)
             ready = torch.cuda.Event()
             ready.record()
-        if st is not cur and torch.is_tensor(zs) and zs.is_cuda:
-            zs.record_stream(st)
+        if st is not cur:
+            for v in (zs, us):
+                if torch.is_tensor(v) and v.is_cuda:
+                    v.record_stream(st)
         pending.append((gset, counts_host, ready, st))
         if len(pending) >= in_flight:
             yield finish()
@@ -159,10 +166,11 @@ def sample_sets(G: AIGGenerator, tpl: Data, z_batches: Iterable[torch.Tensor], i
         yield finish()
 
 
-def sample_bulk(G: AIGGenerator, tpl: Data, z_batches: Iterable[torch.Tensor], in_flight: int = 3) -> Iterator[Data]:
+def sample_bulk(G: AIGGenerator, tpl: Data, z_batches: Iterable[torch.Tensor], in_flight: int = 3,
+                sampling: Optional[Sampling] = None) -> Iterator[Data]:
     """``sample_sets`` handed out graph by graph, in draw order: the same tensors ``sample_one(G, tpl, z)``
     returns for every z, as views of the block's tensors."""
-    for gset in sample_sets(G, tpl, z_batches, in_flight):
+    for gset in sample_sets(G, tpl, z_batches, in_flight, sampling):
         for g in range(gset.B):
             yield gset.graph(g, copy=False)
 
@@ -192,13 +200,31 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--score-dtype", choices=["fp32", "bf16"], default="fp32",
                     help="extension: arithmetic of the node projections behind the candidate scores (bf16 = bf16 matrix "
                          "cores with f32 accumulation, for bulk sampling; the default is the reference's f32)")
+    ap.add_argument("--temperature", type=float, default=None,
+                    help="extension: draw the fan-ins from the candidate logits at this temperature (0: the largest) instead of "
+                         "taking the top candidates")
+    ap.add_argument("--top-k", type=int, default=0, help="extension: draw among the k largest candidate logits (0: all)")
+    ap.add_argument("--top-p", type=float, default=1.0, help="extension: draw among the largest that hold this share of the probability")
+    ap.add_argument("--min-p", type=float, default=0.0, help="extension: draw among those with this share of the largest probability")
     ap.add_argument("--allow-pickle", action="store_true",
                     help="extension: also read dataset files that need a full unpickle (trusted files only)")
     return ap
 
 
+def sampling_of(args) -> Optional[Sampling]:
+    """The drawing of fan-ins that the flags ask for (None: the top candidates; a filter alone draws at temperature 1)."""
+    filters = (args.top_k, args.top_p, args.min_p)
+    if args.temperature is None and filters == (0, 1.0, 0.0):
+        return None
+    t = 1.0 if args.temperature is None else args.temperature
+    if not (0.0 <= t < float("inf")) or args.top_k < 0 or not (0.0 <= args.top_p <= 1.0) or not (0.0 <= args.min_p <= 1.0):
+        raise SystemExit("--temperature and --top-k must not be negative, --top-p and --min-p are shares of 1")
+    return Sampling(t, *filters)
+
+
 def main(argv=None) -> None:
     args = build_parser().parse_args(argv)
+    sampling = sampling_of(args)
     rank, local_rank, world = parallel.env_world()   # bulk sampling needs no process group
     if not torch.cuda.is_available():
         raise RuntimeError("gan_amd.sample needs a HIP device: the generator has no CPU path")
@@ -221,21 +247,26 @@ def main(argv=None) -> None:
     mine = parallel.shard_indices(args.num_samples, rank, world)
 
     def z_of(i):   # per-sample seed: the output set does not depend on the number of ranks
-        return lambda: torch.randn(args.z_dim, device=device, generator=torch.Generator(device=device).manual_seed(args.seed + i))
+        def draw():
+            gen = torch.Generator(device=device).manual_seed(args.seed + i)
+            z = torch.randn(args.z_dim, device=device, generator=gen)
+            return z if sampling is None else (z, torch.rand((tpl.x.size(0), 2), device=device, generator=gen))
+        return draw
 
     block = block_size(tpl.x.size(0), args.batch)
 
     def z_blocks():     # this rank's draws in blocks that go through the kernels as one set of graphs
         for b in range(0, len(mine), block):
-            yield torch.stack([z_of(i)() for i in mine[b:b + block]])
+            draws = [z_of(i)() for i in mine[b:b + block]]
+            yield torch.stack(draws) if sampling is None else tuple(torch.stack(v) for v in zip(*draws))
 
     def bulk():     # a block's tensors cross to the host in a few large copies; its graphs are cut out there
-        for gset in sample_sets(G, tpl, z_blocks()):
+        for gset in sample_sets(G, tpl, z_blocks(), sampling=sampling):
             host = gset.cpu()
             for g in range(host.B):
                 yield host.graph(g)
 
-    results = bulk() if block > 1 else sample_many(G, ((tpl, z_of(i)) for i in mine), in_flight=args.in_flight)
+    results = bulk() if block > 1 else sample_many(G, ((tpl, z_of(i)) for i in mine), in_flight=args.in_flight, sampling=sampling)
     for i, fixed in zip(mine, results):
         if args.num_samples == 1:
             print("[INFO] FIX:", summarize(fixed))

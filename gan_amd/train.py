@@ -42,6 +42,7 @@ from typing import Dict, List, Optional
 
 import torch
 
+from . import logits as logits_ops
 from . import parallel
 from .constraints import (aig_constraint_penalties, clean_depth_set, enforce_aig_constraints, enforce_begin,
                           enforce_finish, enforce_set, pad_set, penalties_set, validate_strict_aig)
@@ -633,6 +634,11 @@ class Trainer:
         self.fused_update = not bool(getattr(args, "no_fused_update", False))
         # the recorded penalty term over its distinct rows (same numbers up to the order of the sums)
         self.gp_rows = not bool(getattr(args, "gp_all_nodes", False))
+        # a teacher generator whose candidate logits the generator learns (the adversarial loss gives it no gradient)
+        self.teacher = None
+        if getattr(args, "teacher_ckpt", None):
+            self._load_teacher()
+        self._g_step_due = False
         self._d_updates = 0      # updates opt_D has made (its step counters hold the same number)
         self._fake_caps: Dict[tuple, int] = {}   # by minibatch shape: level cap the generated side was found to need
         self.marks: Optional[list] = None   # tuning aid: [(label, event on the main stream, host time)] of the last step
@@ -764,12 +770,67 @@ class Trainer:
         return Batch.from_uniform(gset.B, gset.n, self.max_edges, x=x, edge_index=ei, edge_attr=ea,
                                   node_depth=nd.to(torch.long))
 
+    # ------------------------------------------------------------------ a generator that learns from a teacher
+    def _load_teacher(self) -> None:
+        a = self.args
+        state = torch.load(a.teacher_ckpt, map_location=self.device, weights_only=True)
+        z_dim = int(state["node_proj.0.weight"].size(1)) - a.g_hidden
+        if z_dim != a.z_dim:
+            raise ValueError(f"the teacher takes a z of {z_dim} numbers, the generator one of {a.z_dim}: they are given the same z")
+        k = getattr(a, "teacher_candidate_k", None) or a.candidate_k
+        self.teacher = AIGGenerator(node_in_dim=2, hidden_dim=a.g_hidden, z_dim=a.z_dim, candidate_k=k).to(self.device)
+        self.teacher.load_state_dict(state)
+        self.teacher.requires_grad_(False)
+        self.g_reducer = parallel.FlatGradAllReduce(self.G.parameters()) if self.exchange else None
+
+    def distill_loss(self, templates: List[Data], zs: List[torch.Tensor]) -> torch.Tensor:
+        """Adds the gradient of ``distill_weight`` times the distillation loss of the teacher's top candidate logits - the
+        mean over the slots that need a fan-in, over the graphs - to the generator's parameters and returns the loss (a
+        device scalar, no host read).  Graphs of one node count go through together."""
+        a, by_size = self.args, OrderedDict()
+        for t, z in zip(templates, zs):
+            by_size.setdefault(int(t.x.size(0)), []).append((t, z))
+        total = None
+        for group in by_size.values():
+            graphs, z = [t for t, _ in group], torch.stack([z for _, z in group])
+            share = len(group) / len(templates)
+            windows, weight, st = self.G.score_windows(graphs)
+            with torch.no_grad():
+                same_windows = self.teacher.candidate_k == self.G.candidate_k
+                seen, _, st_seen = (windows, weight, st) if same_windows else self.teacher.score_windows(graphs)
+                theirs = logits_ops.class_scores(self.teacher.score_table(st_seen, z), seen)
+                top = logits_ops.top_rows(theirs, min(a.distill_top, theirs.size(1)), counts=seen.counts, temperature=a.distill_temperature)
+                if not same_windows:
+                    # both windows end at the same candidate: a place moves by the difference of their counts
+                    moved = top.index - (seen.counts - windows.counts)[:, None]
+                    top = top._replace(index=torch.where(top.index >= 0, moved, top.index))
+            table = self.G.score_table(st, z)
+            rows = logits_ops.class_scores(table.detach(), windows)
+            loss, grad = logits_ops.distill_loss_and_grad(rows, top, counts=windows.counts, weight=weight,
+                                                          temperature=a.distill_temperature, tail=same_windows)
+            d_table = logits_ops.class_scores_grad(grad, windows, table.size(0), table.size(1))
+            table.backward(d_table * (a.distill_weight * share))
+            loss = loss.sum() * share
+            total = loss if total is None else total + loss
+        return total
+
     def _as_set(self, templates: List[Data]) -> bool:
         """The graphs of the minibatch go through the generator and the constraint kernels as one set when
         they all have the padded node count (the reference's default: templates keep their padding)."""
         return self.use_sets and all(int(t.x.size(0)) == self.max_nodes for t in templates)
 
     def step(self, real_padded: Batch, epoch: int = 0, save_dir: Optional[str] = None) -> Dict[str, float]:
+        try:
+            return self._step(real_padded, epoch, save_dir)
+        finally:
+            # (a gradient that was exchanged is stepped on by every rank, whatever happened behind it, so their generators
+            #  stay equal; nothing in the step reads the weights any more)
+            if self._g_step_due:
+                self._g_step_due = False
+                torch.cuda.current_stream(self.device).wait_stream(self.raw_stream)
+                self.opt_G.step()
+
+    def _step(self, real_padded: Batch, epoch: int = 0, save_dir: Optional[str] = None) -> Dict[str, float]:
         a, dev, G, D = self.args, self.device, self.G, self.D
         real_padded = real_padded.to(dev)
         templates = self.templates_of(real_padded)
@@ -1100,18 +1161,35 @@ class Trainer:
                     raise
                 failed = e
         if failed is not None:
+            if self.teacher is not None and self.exchange:
+                self.g_reducer.reduce(False)
+                self._g_step_due = True
             raise failed
         self._edges_last = edges_fake + edges_real
 
         # ---- generator (train.py:275-299); its output carries no gradient, so backward only touches D
         self._mark("critic done")
         self.opt_G.zero_grad()
+        if zs is None:
+            zs = [self.draw_z() for _ in templates]
+        if self.teacher is not None:      # (extension) the one term that reaches the generator
+            learned = None
+            try:
+                learned = self.distill_loss(templates, zs)
+            except Exception:
+                if not self.exchange:
+                    raise
+                self.g_reducer.reduce(False)
+                self._g_step_due = True
+                raise
+            if self.exchange:
+                self.g_reducer.reduce(True)
+            self._g_step_due = True
         early_raw = early_raw and raw_set is not None
         pen_stream = self.raw_stream if early_raw else self.side_stream
         if early_raw:
             raw_gen = None
         else:
-            zs = [self.draw_z() for _ in templates]
             if as_set:
                 raw_set = G.forward_set(templates, torch.stack(zs))
                 raw_gen = None        # the separate graphs are only made when a save step asks for them
@@ -1180,9 +1258,12 @@ class Trainer:
             terms.add_raw_gradients(sign=-1.0)
         elif raw_recorded:
             terms.add_fake_gradients(sign=-1.0)
-        self.opt_G.step()
+        if self.teacher is None:
+            self.opt_G.step()
         self._probe("main: step end")
         self.last.update(loss_G=loss_G.detach(), pen=loss_pen.detach())
+        if self.teacher is not None:
+            self.last["distill"] = learned
         self._mark("generator done")
 
         if save_dir is not None and (self.global_step % a.save_every) == 0:
@@ -1252,6 +1333,8 @@ def train(args) -> None:
                 logger.log(step_no, epoch, d_real=m["D_real"].item(), d_fake=m["D_fake"].item(), gap=m["gap"].item(),
                            grad_norm=m["grad_norm"].item(), loss_d=m["loss_D"].item(), loss_g=m["loss_G"].item(),
                            gp=m["gp"].item(), pen=m["pen"].item())
+                if "distill" in m and step_no % args.log_every == 0 and rank == 0:
+                    print(f"[INFO] step {step_no}: distillation loss {m['distill'].item():.6f}")
                 if step_no % args.log_every == 0 and hasattr(it, "set_postfix"):
                     r = logger.rows[-1]
                     it.set_postfix({k: f"{r[k]:.4f}" for k in ("loss_D", "loss_G", "D_real", "D_fake", "gp", "pen")})
@@ -1300,6 +1383,13 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--seed", type=int, default=None, help="Seed torch's generators (the reference sets none).")
     p.add_argument("--unpad-templates", action="store_true",
                    help="Strip padding rows from templates (the reference keeps them padded).")
+    p.add_argument("--teacher-ckpt", type=str, default=None,
+                   help="generator state dict (.pt) of a teacher: the generator learns its candidate logits by distillation (without "
+                        "one it never moves: the adversarial loss gives it no gradient)")
+    p.add_argument("--teacher-candidate-k", type=int, default=None, help="the teacher's window (default: --candidate-k)")
+    p.add_argument("--distill-top", type=int, default=16, help="largest logits a slot that are taken of the teacher (1 to 256)")
+    p.add_argument("--distill-temperature", type=float, default=2.0)
+    p.add_argument("--distill-weight", type=float, default=1.0)
     p.add_argument("--no-progress", action="store_true")
     p.add_argument("--allow-pickle", action="store_true",
                    help="also read dataset files that need a full unpickle (pickled torch_geometric objects); trusted files only")

@@ -700,6 +700,12 @@ int aig_sample_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const vo
                     const int32_t* want, const aig_sampling* how, int64_t draws, const float* u, int32_t* out,
                     void* stream);
 
+/* aig_gen_wire_batch with the fan-ins drawn from the candidate logits instead of taken from their top: every slot's two
+ * draws without replacement as aig_sample_rows makes them, u [B][n][2], settings arrays (where given) [B][n]; a->logits
+ * must not be NULL.  A slot that needs a fan-in always gets one: a second one that is not there repeats the first, a first
+ * one that is not there (no finite logit) is the slot's last candidate. */
+int aig_gen_wire_batch_sampled(const aig_gen_wire_set* a, const aig_sampling* how, const float* u, void* stream);
+
 /* The m largest logits of each row (NaN and -inf never), largest first, equal ones by lowest place:
  *   values [rows,m] f32, index [rows,m] (places; absent entries -inf and -1), lse[r] = log sum exp(l / temperature)
  *   over the row's valid places (-inf for none) - what aig_distill_rows takes of a teacher. */

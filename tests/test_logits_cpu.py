@@ -71,3 +71,16 @@ def test_class_scores_workspace_is_checked():
     a = _abi.ScoreWindowsArg(rows=4000, width=8, nodes=5, kinds=2, classes=3, cand=4096, cls=4096, row_kind=4096, by_kind=4096, kind_start=4096)
     need = _abi.lib().aig_class_scores_bwd_ws_bytes(4000, 8, 2, 3)
     assert need > 0 and _abi.lib().aig_class_scores_bwd(C.byref(a), P, P, P, need - 1, None) == -2
+
+
+def test_sampling_flags():
+    from gan_amd.sample import build_parser, sampling_of
+    base = ["--dataset-dir", "d", "--gen-ckpt", "g", "--out", "o"]
+    parse = lambda *a: sampling_of(build_parser().parse_args(base + list(a)))
+    assert parse() is None
+    assert parse("--temperature", "0.5") == L.Sampling(0.5, 0, 1.0, 0.0)
+    assert parse("--top-k", "4") == L.Sampling(1.0, 4, 1.0, 0.0)
+    assert parse("--temperature", "0", "--top-p", "0.9", "--min-p", "0.1") == L.Sampling(0.0, 0, 0.9, 0.1)
+    for bad in (("--temperature", "-1"), ("--temperature", "nan"), ("--top-k", "-2"), ("--top-p", "1.5"), ("--min-p", "-0.1")):
+        with pytest.raises(SystemExit):
+            parse(*bad)
