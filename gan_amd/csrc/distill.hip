@@ -92,14 +92,14 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
         for (int j = lane + G; j < a.m; j += G) s += names(index[j], values[j], n) ? (double)exp2_fast((values[j] - tm) * per) : 0.0;
         lse = (double)tm * a.per + log2_of(all<G>(s, Add()));
     }
+    // (sum_q counts the entries along, NAMED each: at most 256 of at most 1 stay below it, and 2^-34 is left of its steps)
+    constexpr double NAMED = 1024.0;
     double sum_q = 0.0, l = 0.0;
-    int named = 0;
     auto entry = [&](int i, float t) {
         if (!names(i, t, n)) return;
-        ++named;
         const double lq = (double)t * a.per - lse;
         const float q = probability(lq);
-        sum_q += (double)q;
+        sum_q += NAMED + (double)q;
         if (GRAD) atomicAdd(&listed[i], max((unsigned)__float2int_rn(q * Q_UNIT), 1u));
         else listed[i] = 1u;
         if (LOSS) l += q > 0.0f ? (double)q * (lq - ((double)lv[i] - (double)base) * a.per) : q == 0.0f ? 0.0 : (double)q;
@@ -107,8 +107,8 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
     entry(i0, v0);
     for (int j = lane + G; j < a.m; j += G) entry(index[j], values[j]);
     sum_q = all<G>(sum_q, Add());
-    named = all<G>(named, Add());
-    const bool live = z != 0.0 && named > 0;        // (a NaN among the logits is not nothing: it shows in the loss)
+    const bool live = z != 0.0 && sum_q != 0.0;        // (a NaN among the logits is not nothing: it shows in the loss)
+    sum_q -= NAMED * __builtin_floor(sum_q * (1.0 / NAMED));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
 
@@ -137,17 +137,17 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
     const bool faint = rest_q > 0.0f && rest_top != base;
     if (LOSS) {
         l = all<G>(l, Add());
-        // two logarithms at once: the even lanes take that of z, the odd ones that of the rest's two probabilities' ratio (by z)
-        const double part = rest_q > 0.0f ? (double)rest_q / rest : 1.0;
-        const double lg = log2_of(lane & 1 ? part : z), other = dpp<0xB1>(lg);      // (lanes 1 apart)
-        const double logz = lane & 1 ? other : lg, log_part = lane & 1 ? lg : other;
+        // three logarithms at once, one in each of three lanes of every four
+        const bool some = rest_q > 0.0f;
+        const double of = (lane & 3) == 0 ? z : !some ? 1.0 : (lane & 3) == 1 ? rest : (double)rest_q;
+        const double lg = log2_of(of), logz = dpp<0x00>(lg), log_rest = dpp<0x55>(lg), log_rest_q = dpp<0xAA>(lg);
         l += sum_q * logz;
-        if (rest_q > 0.0f) l += (double)rest_q * (log_part + logz - ((double)rest_top - (double)base) * a.per);
+        if (some) l += (double)rest_q * (log_rest_q - log_rest + logz - ((double)rest_top - (double)base) * a.per);
         if (lane == 0) a.loss[r] = live ? (float)((double)a.scale(r) * LN2 * l) : 0.0f;
     }
     if (GRAD) {
-        const float c = live ? a.scale_of_gradient(r) : 0.0f, full = (float)((sum_q + (double)rest_q) / z),
-                    outside = rest_q > 0.0f ? (float)((double)rest_q / rest) : 0.0f;
+        const float c = live ? a.scale_of_gradient(r) : 0.0f, full = ((float)sum_q + rest_q) * __builtin_amdgcn_rcpf((float)z),
+                    outside = rest_q > 0.0f ? rest_q * __builtin_amdgcn_rcpf((float)rest) : 0.0f;
         T g[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {

@@ -50,7 +50,20 @@ template <int CTRL> __device__ __forceinline__ double dpp(double v) {
 }
 
 struct Add { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };
-struct Max { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
+struct Max {
+    template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; }
+};
+// The larger of v and the value N lanes round in the row of 16, as one vector instruction: from fmaxf the compiler makes a
+// move and two maxima, the first to make the moved value canonical.  (Two wait states between a vector write and a lane
+// permutation that reads it: the s_nop.)
+template <int N> __device__ __forceinline__ float max_rotated(float v) {
+    float r;
+    if constexpr (N == 8) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:8 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
+    if constexpr (N == 4) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:4 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
+    if constexpr (N == 2) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:2 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
+    if constexpr (N == 1) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:1 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
+    return r;
+}
 struct Min { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a < b ? a : b; } };
 
 // op over v and the value of the lane 16 (32) apart: the half-swaps of gfx950 put the two side by side, in either order
@@ -88,6 +101,14 @@ template <int G, typename V, typename OP> __device__ __forceinline__ V all(V v, 
     }
     return v;
 }
+template <int G> __device__ __forceinline__ float all(float v, Max op) {
+    v = max_rotated<1>(max_rotated<2>(max_rotated<4>(max_rotated<8>(v))));
+    if (G == 64) {
+        v = across<16>(v, op);
+        v = across<32>(v, op);
+    }
+    return v;
+}
 // sum over the lanes of the group in front of this one
 template <int G, typename V> __device__ __forceinline__ V before(V v) {
     V s = v;
@@ -108,21 +129,26 @@ template <int G, typename V> __device__ __forceinline__ V before(V v) {
 // and are exact in f64 in whatever order they are taken - by lanes, by blocks, by atomics - so a draw is a function of its
 // row alone.  What is lost is a weight's 2^-37, far below the 2^-24 steps of the random numbers.
 constexpr double UNIT = 68719476736.0;          // 2^36
-// 2^(d + SHIFT), d in [-900, 900].  2^f on |f| <= 1/2 by its series: the first term left out is below 7e-15
-// (ln2^12 / (12! 2^12)), a hundredth of a step of what it is used for (2^-36 here, 2^-24 elsewhere).
+// 2^(d + SHIFT), d in [-900, 900].  2^f on |f| <= 1/2 by its series ln2^k / k!, k = 11 .. 0: the first term left out is below
+// 7e-15 (ln2^12 / (12! 2^12)), a hundredth of a step of what it is used for (2^-36 here, 2^-24 elsewhere).  The coefficients are
+// held in scalar registers: as literals each costs two vector moves beside its product.
+__device__ __forceinline__ double scalar(double c) {
+    asm("" : "+s"(c));
+    return c;
+}
 template <int SHIFT> __device__ __forceinline__ double pow2(double d) {
     const double n = __builtin_rint(d), f = d - n;
-    double p = 4.4455382718708110e-10;          // ln2^k / k!, k = 11 .. 0
-    p = fma(p, f, 7.0549116208011210e-09);
-    p = fma(p, f, 1.0178086009239696e-07);
-    p = fma(p, f, 1.3215486790144305e-06);
-    p = fma(p, f, 1.5252733804059838e-05);
-    p = fma(p, f, 1.5403530393381606e-04);
-    p = fma(p, f, 1.3333558146428441e-03);
-    p = fma(p, f, 9.6181291076284772e-03);
-    p = fma(p, f, 5.5504108664821576e-02);
-    p = fma(p, f, 2.4022650695910070e-01);
-    p = fma(p, f, 6.9314718055994531e-01);
+    double p = scalar(4.4455382718708110e-10);
+    p = fma(p, f, scalar(7.0549116208011210e-09));
+    p = fma(p, f, scalar(1.0178086009239696e-07));
+    p = fma(p, f, scalar(1.3215486790144305e-06));
+    p = fma(p, f, scalar(1.5252733804059838e-05));
+    p = fma(p, f, scalar(1.5403530393381606e-04));
+    p = fma(p, f, scalar(1.3333558146428441e-03));
+    p = fma(p, f, scalar(9.6181291076284772e-03));
+    p = fma(p, f, scalar(5.5504108664821576e-02));
+    p = fma(p, f, scalar(2.4022650695910070e-01));
+    p = fma(p, f, scalar(6.9314718055994531e-01));
     p = fma(p, f, 1.0);
     return p * __longlong_as_double((long long)(1023 + SHIFT + (int)n) << 52);
 }
@@ -199,7 +225,8 @@ __device__ __forceinline__ void kth_largest(const unsigned (&key)[E], int k, uns
 // The keys of a group in descending order by place (lane 0's first is the largest): a bitonic network.  Blocks that sort the
 // other way hold their keys complemented, so that every exchange puts the larger key first; an exchange between lanes is a
 // lane permutation and a median with 0 or the largest key (that is: the larger, or the smaller).
-template <int X> __device__ __forceinline__ unsigned exchanged(unsigned v, unsigned keep_larger) {
+// Keys of 64 bits (a key and its place) are compared and selected instead.
+template <int X> __device__ __forceinline__ unsigned exchanged(unsigned v, bool keep_larger) {
     unsigned a = v, b;
     if constexpr (X == 1) b = dpp<0xB1>(v);
     if constexpr (X == 2) b = dpp<0x4E>(v);
@@ -215,21 +242,37 @@ template <int X> __device__ __forceinline__ unsigned exchanged(unsigned v, unsig
         a = r[0];
         b = r[1];
     }
-    return max(min(a, b), min(max(a, b), keep_larger));
+    return max(min(a, b), min(max(a, b), keep_larger ? 0xFFFFFFFFu : 0u));
 }
-template <int X, int E> __device__ __forceinline__ void exchange_lanes(unsigned (&k)[E], int lane) {
-    const unsigned keep_larger = lane & X ? 0u : 0xFFFFFFFFu;
+typedef unsigned long long wide_key;
+template <int X> __device__ __forceinline__ wide_key exchanged(wide_key v, bool keep_larger) {
+    const unsigned lo = (unsigned)v, hi = (unsigned)(v >> 32);
+    wide_key a = v, b;
+    if constexpr (X == 1) b = (wide_key)dpp<0xB1>(hi) << 32 | dpp<0xB1>(lo);
+    if constexpr (X == 2) b = (wide_key)dpp<0x4E>(hi) << 32 | dpp<0x4E>(lo);
+    if constexpr (X == 4) b = (wide_key)dpp<0x1B>(dpp<0x141>(hi)) << 32 | dpp<0x1B>(dpp<0x141>(lo));
+    if constexpr (X == 8) b = (wide_key)dpp<0x128>(hi) << 32 | dpp<0x128>(lo);
+    if constexpr (X == 16 || X == 32) {
+        const auto l = X == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+        const auto h = X == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+        a = (wide_key)(unsigned)h[0] << 32 | (unsigned)l[0];
+        b = (wide_key)(unsigned)h[1] << 32 | (unsigned)l[1];
+    }
+    return (a > b) == keep_larger ? a : b;
+}
+template <int X, int E, typename K> __device__ __forceinline__ void exchange_lanes(K (&k)[E], int lane) {
+    const bool keep_larger = (lane & X) == 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) k[e] = exchanged<X>(k[e], keep_larger);
     if constexpr (X > 1) exchange_lanes<X / 2, E>(k, lane);
 }
-__device__ __forceinline__ void exchange_places(unsigned& a, unsigned& b) {
-    const unsigned larger = max(a, b);
-    b = min(a, b);
+template <typename K> __device__ __forceinline__ void exchange_places(K& a, K& b) {
+    const K larger = a > b ? a : b;
+    b = a > b ? b : a;
     a = larger;
 }
 // places D, D/2, .. 1 apart inside a lane; blocks of SIZE alternate in direction (SIZE = E: one block)
-template <int D, int SIZE, int E> __device__ __forceinline__ void exchange_inside(unsigned (&k)[E]) {
+template <int D, int SIZE, int E, typename K> __device__ __forceinline__ void exchange_inside(K (&k)[E]) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if ((e & D) == 0) {
@@ -238,23 +281,23 @@ template <int D, int SIZE, int E> __device__ __forceinline__ void exchange_insid
         }
     if constexpr (D > 1) exchange_inside<D / 2, SIZE, E>(k);
 }
-template <int SIZE, int E> __device__ __forceinline__ void sort_inside(unsigned (&k)[E]) {
+template <int SIZE, int E, typename K> __device__ __forceinline__ void sort_inside(K (&k)[E]) {
     if constexpr (SIZE < E) {
         exchange_inside<SIZE / 2, SIZE, E>(k);
         sort_inside<SIZE * 2, E>(k);
     }
 }
-template <int L, int G, int E> __device__ __forceinline__ void sort_lanes(unsigned (&k)[E], int lane) {
-    const unsigned m = (lane & (L / 2) ? 0xFFFFFFFFu : 0u) ^ (L < G && (lane & L) ? 0xFFFFFFFFu : 0u);
+template <int L, int G, int E, typename K> __device__ __forceinline__ void sort_lanes(K (&k)[E], int lane) {
+    const K m = ((lane & (L / 2)) != 0) != (L < G && (lane & L) != 0) ? ~K(0) : K(0);
 #pragma unroll
     for (int e = 0; e < E; ++e) k[e] ^= m;
     exchange_lanes<L / 2, E>(k, lane);
     exchange_inside<E / 2, E, E>(k);
     if constexpr (L < G) sort_lanes<L * 2, G, E>(k, lane);
 }
-template <int G, int E> __device__ __forceinline__ void sort_keys(unsigned (&k)[E], int lane) {
+template <int G, int E, typename K> __device__ __forceinline__ void sort_keys(K (&k)[E], int lane) {
     sort_inside<2, E>(k);
-    const unsigned m = lane & 1 ? 0xFFFFFFFFu : 0u;
+    const K m = lane & 1 ? ~K(0) : K(0);
 #pragma unroll
     for (int e = 0; e < E; ++e) k[e] ^= m;
     exchange_inside<E / 2, E, E>(k);

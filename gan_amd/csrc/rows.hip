@@ -1,4 +1,6 @@
 // Operators on rows of logits: sampling from given random numbers, and the largest logits of a row.
+#include <type_traits>
+
 #include "rows.h"
 
 namespace aig {
@@ -907,7 +909,7 @@ struct TopArgs {
     long long rows, ld;
     int width, m, vec;
     const int* counts;
-    float temperature;
+    float temperature, per;      // per: log2(e) / temperature
     float* values;
     int* index;
     float* lse;
@@ -915,76 +917,105 @@ struct TopArgs {
 };
 constexpr int TOP_MAX = AIG_ROWS_MAX_TOP;
 
-// Orders `have` kept places (key, place; place order) and writes them, the rest of the m entries as absent: a place's rank is
-// the number of places in front of it.
-template <int THREADS>
-__device__ __forceinline__ void write_ranked(const TopArgs& a, long long r, const unsigned* key, const int* place, int have, int t) {
-    for (int j = t; j < a.m; j += THREADS) {
-        if (j >= have) {
-            a.values[r * a.m + j] = -__builtin_inff();
-            a.index[r * a.m + j] = -1;
-            continue;
-        }
-        const unsigned k = key[j];
-        int rank = 0;
-        for (int i = 0; i < have; ++i) rank += key[i] > k || (key[i] == k && i < j);
-        a.values[r * a.m + rank] = value_of(k);
-        a.index[r * a.m + rank] = place[j];
-    }
-}
+// A key with its place in the order that is wanted: larger key first, then the lower place.
+__device__ __forceinline__ wide_key with_place(unsigned key, int place) { return (wide_key)key << 32 | (unsigned)~place; }
 
-template <typename T, int G, int E>
+// The group's row sorted, whole (rows to 64 places; any row of bf16, whose key and place share 32 bits), or the m largest
+// picked out first and those sorted, M places a lane.
+template <typename T, int G, int E, int M>
 __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a) {
-    extern __shared__ unsigned lds[];            // per group: m keys, m places
+    constexpr bool PACKED = std::is_same<T, __hip_bfloat16>::value, WHOLE = PACKED || M == 0;
+    __shared__ wide_key lds[WHOLE ? 1 : 256 / G][WHOLE ? 1 : G * (M ? M : 1)];
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
     if (r >= a.rows) return;
-    const int lane = threadIdx.x & (G - 1);
-    unsigned* lkey = lds + (size_t)(threadIdx.x / G) * 2 * a.m;
-    int* lplace = reinterpret_cast<int*>(lkey + a.m);
-    const int n = a.count(r);
-    float v[E];
+    const int lane = threadIdx.x & (G - 1), n = a.count(r);
+    float v[E], m = -__builtin_inff();
     load_values<T, E>(x + r * a.ld, n, a.width, a.vec, lane, v);
-    unsigned key[E], top = 0;
-    int held = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        key[e] = key_of(or_nothing(v[e]));
-        top = max(top, key[e]);
-        held += key[e] > NO_KEY;
+        v[e] = or_nothing(v[e]);
+        m = fmaxf(m, v[e]);
     }
-    top = all<G>(top, Max());
-    held = all<G>(held, Add());
-    unsigned thr = NO_KEY;
-    int quota = 0;
-    if (a.m < held) kth_largest<G, E>(key, a.m, thr, quota);
-    int ties = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) ties += key[e] == thr;
-    int tie = before<G>(ties), mine = 0;
-    bool stays[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        stays[e] = key[e] > thr || (key[e] == thr && tie < quota);
-        tie += key[e] == thr;
-        mine += stays[e];
-    }
-    int at = before<G>(mine);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (stays[e]) {
-            lkey[at] = key[e];
-            lplace[at++] = lane * E + e;
-        }
-    const float m = value_of(top), per = (float)(LOG2E / (double)a.temperature);
+    m = all<G>(m, Max());
     float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += key[e] <= NO_KEY ? 0.0f : key[e] == top ? 1.0f : __builtin_amdgcn_exp2f((value_of(key[e]) - m) * per);
+    for (int e = 0; e < E; ++e) s += v[e] == m ? 1.0f : __builtin_amdgcn_exp2f((v[e] - m) * a.per);
     s = all<G>(s, Add());
-    if (lane == 0) a.lse[r] = top <= NO_KEY ? -__builtin_inff() : m / a.temperature + logf(s);
-    // (the group's own wave wrote the list: its lanes see it once their writes are through)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    write_ranked<G>(a, r, lkey, lplace, min(a.m, held), lane);
+    if (lane == 0) a.lse[r] = m > -__builtin_inff() ? m / a.temperature + logf(s) : -__builtin_inff();
+
+    float* values = a.values + r * a.m;
+    int* index = a.index + r * a.m;
+    if constexpr (PACKED) {
+        unsigned k[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) k[e] = (key_of(v[e]) & 0xFFFF0000u) | (unsigned)(0xFFFF - (lane * E + e));
+        sort_keys<G, E>(k, lane);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int rank = lane * E + e;
+            if (rank < a.m) {
+                // (a bf16's low half: zeros under a key of a positive value, ones under one of a negative)
+                const unsigned key = (k[e] & 0xFFFF0000u) | ((int)k[e] < 0 ? 0u : 0xFFFFu);
+                values[rank] = value_of(key);
+                index[rank] = key > NO_KEY ? 0xFFFF - (int)(k[e] & 0xFFFFu) : -1;
+            }
+        }
+        for (int j = G * E + lane; j < a.m; j += G) {
+            values[j] = -__builtin_inff();
+            index[j] = -1;
+        }
+    } else {
+        auto write = [&](wide_key k, int rank) {
+            const unsigned key = (unsigned)(k >> 32);
+            values[rank] = key > NO_KEY ? value_of(key) : -__builtin_inff();
+            index[rank] = key > NO_KEY ? (int)~(unsigned)k : -1;
+        };
+        constexpr int PER = WHOLE ? E : M;
+        wide_key k[PER];
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) k[e] = with_place(key_of(v[e]), lane * E + e);
+        } else {
+            wide_key* list = lds[threadIdx.x / G];
+#pragma unroll
+            for (int e = 0; e < M; ++e) list[lane * M + e] = 0;
+            unsigned key[E];
+            int held = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                key[e] = key_of(v[e]);
+                held += key[e] > NO_KEY;
+            }
+            held = all<G>(held, Add());
+            unsigned thr = NO_KEY;
+            int quota = 0;
+            if (a.m < held) kth_largest<G, E>(key, a.m, thr, quota);
+            int over = 0, ties = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                over += key[e] > thr;
+                ties += key[e] == thr;
+            }
+            // (places over the threshold from the list's start, those at it behind all of them)
+            int at = before<G>(over), tie = before<G>(ties);
+            const int all_over = all<G>(over, Add());
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (key[e] > thr) list[at++] = with_place(key[e], lane * E + e);
+                if (key[e] == thr && tie < quota) list[all_over + tie] = with_place(key[e], lane * E + e);
+                tie += key[e] == thr;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int e = 0; e < M; ++e) k[e] = list[lane * M + e];
+        }
+        sort_keys<G, PER>(k, lane);
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            if (lane * PER + e < a.m) write(k[e], lane * PER + e);
+        for (int j = G * PER + lane; j < a.m; j += G) write(0, j);
+    }
 }
 
 // A workgroup per row: the places that can be among the m largest are picked out into a list and ranked there.
@@ -1003,13 +1034,12 @@ __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, To
     m = block.all(m, Max());
     if (t == 0) list.count = 0;
     __syncthreads();
-    const float per = (float)(LOG2E / (double)a.temperature);
     double s = 0.0;
     int held = 0;
     each_place(row, [&](int i, float raw) {
         const float v = or_nothing(raw);
         const unsigned k = key_of(v);
-        s += v == m ? 1.0 : (double)__builtin_amdgcn_exp2f((v - m) * per);
+        s += v == m ? 1.0 : (double)__builtin_amdgcn_exp2f((v - m) * a.per);
         held += k > NO_KEY;
         if (k >= low && k > NO_KEY) list.add(k, i);
     });
@@ -1102,19 +1132,21 @@ template <typename T> int top_rows(hipStream_t s, const T* x, TopArgs a) {
         return (int)(reinterpret_cast<uintptr_t>(x) % align == 0 && (a.ld * sizeof(T)) % align == 0);
     };
     auto blocks = [&](int g) { return dim3((unsigned)((a.rows * g + 255) / 256)); };
-    auto lds = [&](int g) { return (size_t)(256 / g) * 2 * a.m * 4; };      // at most 32 KB
     if (a.width <= 64) {
         a.vec = vec(4);
-        hipLaunchKernelGGL((k_top<T, 16, 4>), blocks(16), dim3(256), lds(16), s, x, a);
+        hipLaunchKernelGGL((k_top<T, 16, 4, 0>), blocks(16), dim3(256), 0, s, x, a);
     } else if (a.width <= 256) {
         a.vec = vec(16);
-        hipLaunchKernelGGL((k_top<T, 16, 16>), blocks(16), dim3(256), lds(16), s, x, a);
+        if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 16, 16, 4>), blocks(16), dim3(256), 0, s, x, a);
+        else hipLaunchKernelGGL((k_top<T, 16, 16, 16>), blocks(16), dim3(256), 0, s, x, a);
     } else if (a.width <= 512) {
         a.vec = vec(8);
-        hipLaunchKernelGGL((k_top<T, 64, 8>), blocks(64), dim3(256), lds(64), s, x, a);
+        if (a.m <= 128) hipLaunchKernelGGL((k_top<T, 64, 8, 2>), blocks(64), dim3(256), 0, s, x, a);
+        else hipLaunchKernelGGL((k_top<T, 64, 8, 4>), blocks(64), dim3(256), 0, s, x, a);
     } else if (a.width <= NARROW) {
         a.vec = vec(16);
-        hipLaunchKernelGGL((k_top<T, 64, 16>), blocks(64), dim3(256), lds(64), s, x, a);
+        if (a.m <= 128) hipLaunchKernelGGL((k_top<T, 64, 16, 2>), blocks(64), dim3(256), 0, s, x, a);
+        else hipLaunchKernelGGL((k_top<T, 64, 16, 4>), blocks(64), dim3(256), 0, s, x, a);
     } else {
         hipLaunchKernelGGL(k_top_wide<T>, dim3((unsigned)a.rows), dim3(WIDE_T), 0, s, x, a);
     }
@@ -1177,6 +1209,7 @@ extern "C" int aig_top_rows(int64_t rows, int64_t width, int64_t ld, int dtype, 
     AIG_REQUIRE(logits && values && index && lse, "aig_top_rows: null pointer");
     TopArgs a{};
     a.rows = rows; a.ld = ld; a.width = (int)width; a.m = (int)m; a.counts = counts; a.temperature = temperature;
+    a.per = (float)(rows::LOG2E / (double)temperature);
     a.values = values; a.index = index; a.lse = lse;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == AIG_F32) return top_rows(s, static_cast<const float*>(logits), a);
