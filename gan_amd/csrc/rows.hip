@@ -556,25 +556,40 @@ __device__ __forceinline__ void general_draws(const T* __restrict__ x, const Sam
     }
 }
 
-// Lists of places picked out of a row, in LDS.
+// A key with its place in the order that is wanted: larger key first, then the lower place.
+__device__ __forceinline__ wide_key with_place(unsigned key, int place) { return (wide_key)key << 32 | (unsigned)~place; }
+
+// Places picked out of a row, in LDS.
 constexpr int LIST = 1024, LIST_K = 512;
 struct List {
-    unsigned key[LIST];
-    int place[LIST];
+    wide_key key[LIST], sorted[LIST];
     double q[LIST];
     int count;
     __device__ __forceinline__ void add(unsigned k, int i) {
         const int at = atomicAdd(&count, 1);
-        if (at < LIST) {
-            key[at] = k;
-            place[at] = i;
-        }
+        if (at < LIST) key[at] = with_place(k, i);
     }
-    // places in front of (k, i) in the order of the keys, then of the places
-    __device__ __forceinline__ int rank(unsigned k, int i, int n) const {
-        int before = 0;
-        for (int j = 0; j < n; ++j) before += key[j] > k || (key[j] == k && place[j] < i);
-        return before;
+    // key[0 .. n) into sorted[0 .. n), largest first.  All keys differ.  A wave sorts up to 256 of them; of more, every thread
+    // counts the keys in front of its own.
+    __device__ __forceinline__ void sort(int n) {
+        __syncthreads();
+        if (n <= 256) {
+            if (threadIdx.x < 64) {
+                wide_key k[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) k[e] = (int)threadIdx.x * 4 + e < n ? key[threadIdx.x * 4 + e] : 0ull;
+                sort_keys<64, 4>(k, threadIdx.x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sorted[threadIdx.x * 4 + e] = k[e];
+            }
+        } else if ((int)threadIdx.x < n) {
+            const wide_key mine = key[threadIdx.x];
+            int front = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) front += key[j] > mine;
+            sorted[front] = mine;
+        }
+        __syncthreads();
     }
 };
 
@@ -735,38 +750,33 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     if (t == 0) list.count = 0;
 
     if (by_k) {
-        const unsigned low = bound_of_top(my_top, how.top_k, list.key, &shared_key);
+        const unsigned low = bound_of_top(my_top, how.top_k, reinterpret_cast<unsigned*>(list.key), &shared_key);
+        const float low_value = value_of(low);
         each_place(row, [&](int i, float v) {
-            const unsigned k = key_of(or_nothing(v));
-            if (k >= low) list.add(k, i);
+            if (v >= low_value) list.add(key_of(v), i);
         });
         __syncthreads();
         const int have = list.count;
         if (have > LIST) return general_draws<T>(x, a);
-        const bool mine = t < have;
-        const unsigned key = mine ? list.key[t] : 0u;
-        const int place = mine ? list.place[t] : -1, rank = mine ? list.rank(key, place, have) : LIST, keep = min(how.top_k, have);
-        double q = rank < keep ? weight(value_of(key)) : 0.0;
-        if (rank < keep) hist[rank] = q;          // in the order of the keys
-        __syncthreads();
+        list.sort(have);
+        const int keep = min(how.top_k, have);
+        const wide_key mine = t < have ? list.sorted[t] : 0ull;
+        double q = t < keep ? weight(value_of((unsigned)(mine >> 32))) : 0.0, total;
         if (by_p) {
-            double front = 0.0, total = 0.0;
-            for (int j = 0; j < keep; ++j) {
-                const double w = hist[j];
-                front += j < rank ? w : 0.0;
-                total += w;
-            }
-            if (rank > 0 && !(front < how.mass(total))) q = 0.0;
+            const double front = block.before(q, total);
+            if (t > 0 && !(front < how.mass(total))) q = 0.0;
         }
         if (q < least) q = 0.0;
-        list.q[t] = q;
-        __syncthreads();
-        double upto = 0.0, total = 0.0;           // in the order of the places
-        for (int j = 0; j < have; ++j) {
-            const double w = list.q[j];
-            upto += list.place[j] < place ? w : 0.0;
-            total += w;
+        // and in the order of the places
+        if (t < have) {
+            list.q[t] = q;
+            list.key[t] = mine << 32 | (unsigned)t;
         }
+        list.sort(have);
+        const wide_key here = t < have ? list.sorted[t] : 0ull;
+        const int place = t < have ? (int)~(unsigned)(here >> 32) : -1;
+        q = t < have ? list.q[(unsigned)here] : 0.0;
+        double upto = block.before(q, total);
         for (int d = 0; d < a.draws; ++d) {
             if (!(total > 0.0)) return none(d);
             const double u = (double)a.uniform(r, d) * total;
@@ -838,24 +848,19 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     if (wave == 0) part_sum(0);
     if (wave == 1) part_sum(1 + 16 * parts.sweeps);
     __syncthreads();
-    unsigned thr = 0xFFFFFFFFu;
-    int last = -1;
+    wide_key edge = ~0ull;          // the last place of the border's bin that stays
     if (by_p) {
         const int have = list.count;
         if (have > LIST) return general_draws<T>(x, a);
-        const bool mine = t < have;
-        const unsigned key = mine ? list.key[t] : 0u;
-        const int place = mine ? list.place[t] : -1;
-        const double q = mine ? weight(value_of(key)) : 0.0;
-        list.q[t] = q;
-        __syncthreads();
-        double front = above;
-        if (mine)
-            for (int j = 0; j < have; ++j) front += list.key[j] > key || (list.key[j] == key && list.place[j] < place) ? list.q[j] : 0.0;
-        const bool stays = mine && (front == 0.0 || front < p);
-        thr = block.all(stays ? key : 0xFFFFFFFFu, Min());
-        last = block.all(stays && key == thr ? place : -1, Max());
-        if (stays && q >= least) unsafeAtomicAdd(&part_mass[parts.of(place)], q);
+        list.sort(have);
+        const wide_key mine = t < have ? list.sorted[t] : 0ull;
+        const double q = t < have ? weight(value_of((unsigned)(mine >> 32))) : 0.0;
+        double sum;
+        const double front = above + block.before(q, sum);
+        const bool stays = t < have && (front == 0.0 || front < p);
+        const int keep = block.all((int)stays, Add());
+        if (keep > 0) edge = list.sorted[keep - 1];
+        if (stays && q >= least) unsafeAtomicAdd(&part_mass[parts.of((int)~(unsigned)mine)], q);
         __syncthreads();
     }
     for (int d = 0; d < a.draws; ++d) {
@@ -879,9 +884,8 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int b = bin_of(v[j]);
-                const unsigned k = key_of(v[j]);
                 // (without branches: as a chain of || this compiler left the assignment of 0 out)
-                const bool stays = (b < border_bin) | ((b == border_bin) & ((k > thr) | ((k == thr) & (at + j <= last))));
+                const bool stays = (b < border_bin) | ((b == border_bin) & (with_place(key_of(v[j]), at + j) >= edge));
                 const double w = weight(v[j]);
                 bool taken = j >= here;
                 for (int i = 0; i < d; ++i) taken |= picked[i] == at + j;
@@ -916,9 +920,6 @@ struct TopArgs {
     __device__ __forceinline__ int count(long long r) const { return counts ? min(max(counts[r], 0), width) : width; }
 };
 constexpr int TOP_MAX = AIG_ROWS_MAX_TOP;
-
-// A key with its place in the order that is wanted: larger key first, then the lower place.
-__device__ __forceinline__ wide_key with_place(unsigned key, int place) { return (wide_key)key << 32 | (unsigned)~place; }
 
 // The group's row sorted, whole (rows to 64 places; any row of bf16, whose key and place share 32 bits), or the m largest
 // picked out first and those sorted, M places a lane.
@@ -1030,24 +1031,35 @@ __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, To
     const Span<T> row(x + r * a.ld, n);
     float m = -__builtin_inff();
     each_place(row, [&](int, float v) { m = fmaxf(m, or_nothing(v)); });
-    unsigned low = bound_of_top(key_of(m), a.m, list.key, &shared_key);
+    unsigned low = bound_of_top(key_of(m), a.m, reinterpret_cast<unsigned*>(list.key), &shared_key);
     m = block.all(m, Max());
     if (t == 0) list.count = 0;
     __syncthreads();
     double s = 0.0;
-    int held = 0;
-    each_place(row, [&](int i, float raw) {
-        const float v = or_nothing(raw);
-        const unsigned k = key_of(v);
-        s += v == m ? 1.0 : (double)__builtin_amdgcn_exp2f((v - m) * a.per);
-        held += k > NO_KEY;
-        if (k >= low && k > NO_KEY) list.add(k, i);
-    });
+    const float low_value = value_of(low);
+    auto one = [&](int i, float v) {
+        if (v >= low_value) list.add(key_of(v), i);
+        return __builtin_amdgcn_exp2f((or_nothing(v) - m) * a.per);
+    };
+    if (n <= BY_PLACE) {
+        for (int i = t; i < n; i += WIDE_T) s += (double)one(i, as_float(row.x[i]));
+    } else {
+        row.each(t, WIDE_T, [&](int i, const float (&v)[Span<T>::PER], int count) {
+            float of_vector = 0.0f;
+#pragma unroll
+            for (int j = 0; j < Span<T>::PER; ++j)
+                if (j < count) of_vector += one(i + j, v[j]);
+            s += (double)of_vector;
+        });
+    }
     s = block.all(s, Add());
-    held = block.all(held, Add());
-    if (t == 0) a.lse[r] = m > -__builtin_inff() ? m / a.temperature + logf((float)s) : -__builtin_inff();
+    // (beside an infinite largest logit there is nothing to sum)
+    if (t == 0) a.lse[r] = fabsf(m) < __builtin_inff() ? m / a.temperature + logf((float)s) : m;
     int have = list.count;
     if (have > LIST) {
+        int held = 0;
+        each_place(row, [&](int, float v) { held += v > -__builtin_inff(); });
+        held = block.all(held, Add());
         // thousands of equal logits at the border, or a row of few threads' places: the border bit by bit, then the list by place
         double above;
         const unsigned thr = held > a.m ? border_key(n, (double)a.m, hist, found, [&](int i) { return key_of(or_nothing(as_float(row.x[i]))); },
@@ -1075,27 +1087,17 @@ __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, To
             int at = kept_so_far + block.before(mine, kept_here);
 #pragma unroll
             for (int e = 0; e < WIDE_E; ++e)
-                if (stays[e] && at < LIST) {
-                    list.key[at] = k[e];
-                    list.place[at++] = base + e;
-                }
+                if (stays[e] && at < LIST) list.key[at++] = with_place(k[e], base + e);
             ties_so_far += ties_here;
             kept_so_far += kept_here;
         }
         have = min(held, a.m);
-        __syncthreads();
     }
-    if (t < have) {
-        const unsigned k = list.key[t];
-        const int place = list.place[t], rank = list.rank(k, place, have);
-        if (rank < a.m) {
-            a.values[r * a.m + rank] = value_of(k);
-            a.index[r * a.m + rank] = place;
-        }
-    }
-    for (int j = have + t; j < a.m; j += WIDE_T) {
-        a.values[r * a.m + j] = -__builtin_inff();
-        a.index[r * a.m + j] = -1;
+    list.sort(have);
+    for (int j = t; j < a.m; j += WIDE_T) {
+        const wide_key k = j < have ? list.sorted[j] : 0ull;
+        a.values[r * a.m + j] = j < have ? value_of((unsigned)(k >> 32)) : -__builtin_inff();
+        a.index[r * a.m + j] = j < have ? (int)~(unsigned)k : -1;
     }
 }
 
