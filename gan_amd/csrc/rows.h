@@ -328,7 +328,7 @@ template <typename T> struct Span {
             const float v[PER] = {as_float(x[first])};
             f(first, v, 1);
         }
-#pragma unroll 4
+#pragma unroll 2
         for (int k = first; k < vecs; k += step) {
             union { uint4 w; T t[PER]; } u;
             u.w = reinterpret_cast<const uint4*>(x + head)[k];

@@ -673,6 +673,53 @@ template <typename T> struct Parts {
         first = row.head + k * PER;
         return k < row.vecs ? PER : 0;
     }
+    // f(part) for every part, by the wave that has it
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        const int wave = threadIdx.x >> 6;
+        for (int s = 0; s < sweeps; ++s) f(1 + 16 * s + wave);
+        if (wave == 0) f(0);
+        if (wave == 1) f(1 + 16 * sweeps);
+    }
+    // The places that hold `value`, in order: their number in front of each part goes to front[part], and f(place, number in
+    // order, part) is called for those numbered below `quota` (a lane's own, by that lane).  ties: [count()] in LDS.
+    template <typename F> __device__ __forceinline__ void ties_of(float value, int quota, int* ties, int* front, const Block& block, F f) const {
+        const int lane = lane_id();
+        __syncthreads();
+        each([&](int part) {
+            int at;
+            const int here = places(part, lane, at);
+            float v[PER];
+            load(at, here, v);
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) c += (j < here) & (v[j] == value);
+            c = all<64>(c, Add());
+            if (lane == 0) ties[part] = c;
+        });
+        __syncthreads();
+        int total;
+        const int before_part = block.before((int)threadIdx.x < count() ? ties[threadIdx.x] : 0, total);
+        if ((int)threadIdx.x < count()) front[threadIdx.x] = before_part;
+        __syncthreads();
+        each([&](int part) {
+            if (front[part] >= quota || ties[part] == 0) return;
+            int at;
+            const int here = places(part, lane, at);
+            float v[PER];
+            load(at, here, v);
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) c += (j < here) & (v[j] == value);
+            int number = front[part] + before<64>(c);
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if ((j < here) & (v[j] == value)) {
+                    if (number < quota) f(at + j, number, part);
+                    ++number;
+                }
+        });
+        __syncthreads();
+    }
     __device__ __forceinline__ void load(int first, int n, float (&v)[PER]) const {
 #pragma unroll
         for (int j = 0; j < PER; ++j) v[j] = -__builtin_inff();
@@ -687,9 +734,28 @@ template <typename T> struct Parts {
     }
 };
 
+// The list after it has overflowed: fewer than k places lie over `low`, so those are listed, and the first of the many at it.
+// (Where thousands lie over it - rows of a few threads' places - the list stays too long.)
+template <typename T>
+__device__ __forceinline__ void list_with_ties(const Span<T>& row, const Parts<T>& parts, List& list, unsigned low, int k, const Block& block) {
+    __syncthreads();
+    if (threadIdx.x == 0) list.count = 0;
+    __syncthreads();
+    const float value = value_of(low);
+    each_place(row, [&](int i, float v) {
+        if (v > value) list.add(key_of(v), i);
+    });
+    __syncthreads();
+    const int over = list.count;
+    if (over >= k) return;
+    int* ties = reinterpret_cast<int*>(list.q);
+    parts.ties_of(value, k - over, ties, ties + PARTS, block, [&](int place, int, int) { list.add(low, place); });
+}
+
 // A workgroup per row.  Weights are whole numbers in f64 throughout, so their sums do not depend on how the row is split.
 //   top-k (to LIST_K): the places that can be among the k largest are picked out into a list, everything else happens there.
-//   otherwise: top-p's border from a histogram of the weights over BINS steps of the logit, the places of its bin in a list;
+//   otherwise: top-p's border from a histogram of the weights over BINS steps of the logit (from the row's smallest, or the
+//   smallest that has a weight), the places of its bin in a list, or counted where they are thousands of one value;
 //   then the sum of what stays in each part of the row, and for each draw a look through the one part that holds it.
 constexpr int BINS = 4096;
 constexpr float OCTAVES = 37.0f;          // a weight under 2^-37 is 0
@@ -736,17 +802,25 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
             for (int d = from; d < a.draws; ++d) a.store(r, d, -1, first, n);
     };
 
-    float m = -__builtin_inff();
-    each_place(row, [&](int, float v) { m = fmaxf(m, or_nothing(v)); });
+    const bool by_k = how.top_k > 0 && how.top_k < n, by_p = how.top_p < 1.0f;
+    float m = -__builtin_inff(), low_end = __builtin_inff();
+    if (by_p && !by_k)
+        each_place(row, [&](int, float v) {
+            m = fmaxf(m, or_nothing(v));
+            low_end = v > -__builtin_inff() ? fminf(low_end, v) : low_end;
+        });
+    else
+        each_place(row, [&](int, float v) { m = fmaxf(m, or_nothing(v)); });
     const unsigned my_top = key_of(m);
     m = block.all(m, Max());
     if (!(m > -__builtin_inff())) return none(0);
+    low_end = block.all(low_end, Min());
     const double m64 = (double)m, per = LOG2E / (double)how.temperature;
     auto weight = [&](float v) { return v == m ? UNIT : v > -__builtin_inff() ? weight_of(((double)v - m64) * per) : 0.0; };
     const double least = how.floor();
-    const bool by_k = how.top_k > 0 && how.top_k < n, by_p = how.top_p < 1.0f;
-    const float bins_per = (float)per * ((float)BINS / OCTAVES);
-    if ((by_k && how.top_k > LIST_K) || !(bins_per > 0.0f && bins_per < 1e30f && m < __builtin_inff())) return general_draws<T>(x, a);
+    const float octaves = fminf((m - low_end) * (float)per, OCTAVES);
+    const float bins_per = by_p && !by_k && octaves > 0.0f ? (float)per * ((float)BINS / octaves) : 1.0f;
+    if ((by_k && how.top_k > LIST_K) || !((float)per > 0.0f && bins_per < 1e30f && m < __builtin_inff())) return general_draws<T>(x, a);
     if (t == 0) list.count = 0;
 
     if (by_k) {
@@ -756,6 +830,7 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
             if (v >= low_value) list.add(key_of(v), i);
         });
         __syncthreads();
+        if (list.count > LIST) list_with_ties(row, Parts<T>(row), list, low, how.top_k, block);
         const int have = list.count;
         if (have > LIST) return general_draws<T>(x, a);
         list.sort(have);
@@ -844,24 +919,47 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
         sum = all<64>(sum, Add());
         if (lane == 0) part_mass[part] = sum;
     };
-    for (int s = 0; s < parts.sweeps; ++s) part_sum(1 + 16 * s + wave);
-    if (wave == 0) part_sum(0);
-    if (wave == 1) part_sum(1 + 16 * parts.sweeps);
+    parts.each(part_sum);
     __syncthreads();
     wide_key edge = ~0ull;          // the last place of the border's bin that stays
     if (by_p) {
         const int have = list.count;
-        if (have > LIST) return general_draws<T>(x, a);
-        list.sort(have);
-        const wide_key mine = t < have ? list.sorted[t] : 0ull;
-        const double q = t < have ? weight(value_of((unsigned)(mine >> 32))) : 0.0;
-        double sum;
-        const double front = above + block.before(q, sum);
-        const bool stays = t < have && (front == 0.0 || front < p);
-        const int keep = block.all((int)stays, Add());
-        if (keep > 0) edge = list.sorted[keep - 1];
-        if (stays && q >= least) unsafeAtomicAdd(&part_mass[parts.of((int)~(unsigned)mine)], q);
-        __syncthreads();
+        if (have > LIST) {
+            // thousands of places in the border's bin: of one value, or there is no help but the general form
+            unsigned highest = 0u, lowest = 0xFFFFFFFFu;
+            each_place(row, [&](int, float v) {
+                if (v > -__builtin_inff() && bin_of(v) == border_bin) {
+                    highest = max(highest, key_of(v));
+                    lowest = min(lowest, key_of(v));
+                }
+            });
+            highest = block.all(highest, Max());
+            lowest = block.all(lowest, Min());
+            if (highest != lowest) return general_draws<T>(x, a);
+            const double q = weight(value_of(highest));
+            int keep = (int)fmin((p - above) / q, (double)n);          // places i = 0, 1, .. stay while above + i q < p
+            while (keep > 0 && !(above + (double)(keep - 1) * q < p)) --keep;
+            while (keep < n && above + (double)keep * q < p) ++keep;
+            int* ties = reinterpret_cast<int*>(list.q);
+            if (t == 0) list.sorted[0] = 0ull;
+            parts.ties_of(value_of(highest), keep, ties, ties + PARTS, block, [&](int place, int number, int) {
+                if (number == keep - 1) list.sorted[0] = with_place(highest, place);
+            });
+            edge = list.sorted[0];            // (0: fewer ties than would stay, all of them do)
+            if (t < parts.count() && q >= least) part_mass[t] += q * (double)min(max(keep - ties[PARTS + t], 0), ties[t]);
+            __syncthreads();
+        } else {
+            list.sort(have);
+            const wide_key mine = t < have ? list.sorted[t] : 0ull;
+            const double q = t < have ? weight(value_of((unsigned)(mine >> 32))) : 0.0;
+            double sum;
+            const double front = above + block.before(q, sum);
+            const bool stays = t < have && (front == 0.0 || front < p);
+            const int keep = block.all((int)stays, Add());
+            if (keep > 0) edge = list.sorted[keep - 1];
+            if (stays && q >= least) unsafeAtomicAdd(&part_mass[parts.of((int)~(unsigned)mine)], q);
+            __syncthreads();
+        }
     }
     for (int d = 0; d < a.draws; ++d) {
         const double mass = t < parts.count() ? part_mass[t] : 0.0;
@@ -889,7 +987,7 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
                 const double w = weight(v[j]);
                 bool taken = j >= here;
                 for (int i = 0; i < d; ++i) taken |= picked[i] == at + j;
-                q[j] = stays & !taken & (w >= least) ? w : 0.0;
+                q[j] = (stays & !taken & (w >= least)) ? w : 0.0;
                 sum += q[j];
             }
             double end = found[0] + before<64>(sum);
@@ -919,7 +1017,6 @@ struct TopArgs {
     float* lse;
     __device__ __forceinline__ int count(long long r) const { return counts ? min(max(counts[r], 0), width) : width; }
 };
-constexpr int TOP_MAX = AIG_ROWS_MAX_TOP;
 
 // The group's row sorted, whole (rows to 64 places; any row of bf16, whose key and place share 32 bits), or the m largest
 // picked out first and those sorted, M places a lane.
@@ -1056,6 +1153,10 @@ __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, To
     // (beside an infinite largest logit there is nothing to sum)
     if (t == 0) a.lse[r] = fabsf(m) < __builtin_inff() ? m / a.temperature + logf((float)s) : m;
     int have = list.count;
+    if (have > LIST) {
+        list_with_ties(row, Parts<T>(row), list, low, a.m, block);
+        have = list.count;
+    }
     if (have > LIST) {
         int held = 0;
         each_place(row, [&](int, float v) { held += v > -__builtin_inff(); });

@@ -90,13 +90,22 @@ def _side(t: Optional[torch.Tensor], shape: tuple, dtype: torch.dtype, device: t
     return t.data_ptr()
 
 
+_entry: dict = {}      # entry points by name, once looked up
+
+
 def _call(name: str, device: torch.device, *args, meta=None) -> None:
     """An entry point of the library on the current stream of ``device`` (the last argument of all of them)."""
-    fn = getattr(_abi.lib(), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_abi.lib(), name)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _abi.check(_abi.timed(name, fn, *args, _abi.stream(), meta=meta), name)
-    rc = _abi.timed(name, fn, *args, _abi.stream(), meta=meta)
+    t = _abi.timeline
+    if t.enabled or t.sizes_of is not None:
+        rc = _abi.timed(name, fn, *args, _abi.stream(), meta=meta)
+    else:
+        rc = fn(*args, _abi.stream())
     if rc:
         _abi.check(rc, name)
 
