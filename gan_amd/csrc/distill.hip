@@ -372,7 +372,8 @@ template <typename T, int G, int E> void launch_narrow(hipStream_t s, const T* x
 }
 
 template <typename T> int distill(hipStream_t s, const T* x, T* grad, const DistillArgs& a) {
-    if (a.width <= 64) launch_narrow<T, 16, 4>(s, x, grad, a);
+    if (a.width <= 16) launch_narrow<T, 4, 4>(s, x, grad, a);
+    else if (a.width <= 64) launch_narrow<T, 4, 16>(s, x, grad, a);
     else if (a.width <= 256) launch_narrow<T, 16, 16>(s, x, grad, a);
     else if (a.width <= 512) launch_narrow<T, 64, 8>(s, x, grad, a);
     else if (a.width <= NARROW) launch_narrow<T, 64, 16>(s, x, grad, a);

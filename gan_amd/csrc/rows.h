@@ -1,7 +1,8 @@
-// Rows of logits: what the kernels on them share (rows.hip, distill.hip).  A row is held by a GROUP of 16 or 64 lanes,
-// lane L of which owns the E consecutive places L*E .. L*E + E - 1 in registers, so that an order by place is an order by
-// lane: one scan over the group's lanes orders everything.  Sixteen lanes are one row of the vector unit's lane
-// permutations, so their sums and scans are vector instructions alone, for four rows of logits at once.
+// Rows of logits: what the kernels on them share (rows.hip, distill.hip).  A row is held by a GROUP of 4, 16 or 64 lanes, lane
+// L of which owns the E consecutive places L*E .. L*E + E - 1 in registers, so that an order by place is an order by lane: one
+// scan over the group's lanes orders everything.  What is done once a row - sums and scans over its lanes - is done for
+// the 64 / G rows of a wave at once, so the narrowest group whose registers hold the row is the fastest (64 places: 4
+// lanes of 16 rather than 16 lanes of 4, twice as fast); up to sixteen lanes, sums and scans are vector instructions alone.
 #pragma once
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -53,7 +54,7 @@ struct Add { template <typename V> __device__ __forceinline__ V operator()(V a, 
 struct Max {
     template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; }
 };
-// The larger of v and the value N lanes round in the row of 16, as one vector instruction: from fmaxf the compiler makes a
+// The larger of v and the value N lanes round in the row of 16 (N < 0: -N apart in each four; -8: mirrored in each eight), as one vector instruction: from fmaxf the compiler makes a
 // move and two maxima, the first to make the moved value canonical.  (Two wait states between a vector write and a lane
 // permutation that reads it: the s_nop.)
 template <int N> __device__ __forceinline__ float max_rotated(float v) {
@@ -61,6 +62,9 @@ template <int N> __device__ __forceinline__ float max_rotated(float v) {
     if constexpr (N == 8) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:8 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
     if constexpr (N == 4) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:4 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
     if constexpr (N == 2) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:2 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
+    if constexpr (N == -2) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
+    if constexpr (N == -1) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
+    if constexpr (N == -8) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
     if constexpr (N == 1) asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 row_ror:1 row_mask:0xf bank_mask:0xf" : "=v"(r) : "v"(v));
     return r;
 }
@@ -90,7 +94,12 @@ template <int X, typename OP> __device__ __forceinline__ double across(double v,
 
 // v over the lanes of a group, in every lane of it
 template <int G, typename V, typename OP> __device__ __forceinline__ V all(V v, OP op) {
-    static_assert(G == 16 || G == 64, "groups of 16 or 64 lanes");
+    static_assert(G == 4 || G == 8 || G == 16 || G == 64, "groups of 4, 8, 16 or 64 lanes");
+    if constexpr (G <= 8) {
+        v = op(v, dpp<0x4E>(v));
+        v = op(v, dpp<0xB1>(v));
+        return G == 8 ? op(v, dpp<0x141>(v)) : v;        // (the other four's, by the mirror of eight)
+    }
     v = op(v, dpp<0x128>(v));
     v = op(v, dpp<0x124>(v));
     v = op(v, dpp<0x122>(v));
@@ -102,6 +111,10 @@ template <int G, typename V, typename OP> __device__ __forceinline__ V all(V v, 
     return v;
 }
 template <int G> __device__ __forceinline__ float all(float v, Max op) {
+    if constexpr (G <= 8) {
+        v = max_rotated<-1>(max_rotated<-2>(v));
+        return G == 8 ? max_rotated<-8>(v) : v;
+    }
     v = max_rotated<1>(max_rotated<2>(max_rotated<4>(max_rotated<8>(v))));
     if (G == 64) {
         v = across<16>(v, op);
@@ -112,6 +125,24 @@ template <int G> __device__ __forceinline__ float all(float v, Max op) {
 // sum over the lanes of the group in front of this one
 template <int G, typename V> __device__ __forceinline__ V before(V v) {
     V s = v;
+    if constexpr (G == 4) {
+        const int lane = lane_id() & 3;
+        const V one = dpp<0x90>(s);          // lanes 0 0 1 2 of each four
+        s += lane > 0 ? one : V(0);
+        const V two = dpp<0x40>(s);          // lanes 0 0 0 1
+        s += lane > 1 ? two : V(0);
+        return s - v;
+    }
+    if constexpr (G == 8) {
+        const int lane = lane_id() & 7;
+        const V one = dpp<0x111>(s);
+        s += lane > 0 ? one : V(0);
+        const V two = dpp<0x112>(s);
+        s += lane > 1 ? two : V(0);
+        const V four = dpp<0x114>(s);
+        s += lane > 3 ? four : V(0);
+        return s - v;
+    }
     s += dpp<0x111>(s);
     s += dpp<0x112>(s);
     s += dpp<0x114>(s);

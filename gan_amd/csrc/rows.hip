@@ -68,23 +68,28 @@ template <int G, int E, typename W> __device__ __forceinline__ void keep_first(c
 template <int G, int E>
 __device__ __forceinline__ void exact_draws(const SampleRows& a, const RowSettings& how, long long r, int lane, int n, int want,
                                             const unsigned (&key)[E], unsigned top, unsigned guess) {
-    const double m = (double)value_of(top), per = LOG2E / (double)how.temperature;
+    const float m = value_of(top);
+    const double m64 = (double)m, per = LOG2E / (double)how.temperature;
     double q[E];
-    int held = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        q[e] = key[e] == top ? UNIT : weight_of(((double)value_of(key[e]) - m) * per);
-        q[e] = key[e] > NO_KEY ? q[e] : 0.0;
-        held += key[e] > NO_KEY;
+        // (no branch: the places' chains of products run side by side.  The largest place, infinite or not, has weight 1, and
+        //  a place that holds nothing, at -inf, has none)
+        const float v = value_of(key[e]);
+        q[e] = weight_of(v == m ? 0.0 : ((double)v - m64) * per);
     }
-    held = all<G>(held, Add());
-    if (how.top_k > 0 && how.top_k < held) {
-        unsigned thr;
-        int quota;
-        kth_largest<G, E>(key, how.top_k, thr, quota);
-        keep_first<G, E>(key, q, thr, quota);
+    if (how.top_k > 0 && how.top_k < a.width) {
+        unsigned s[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[e] = key[e];
+        sort_keys<G, E>(s, lane);
+        const unsigned thr = at_rank<G, E>(s, how.top_k - 1);
+        int over = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) over += key[e] > thr;
+        keep_first<G, E>(key, q, thr, how.top_k - all<G>(over, Add()));
     }
-    if (how.top_p < 1.0f && held > 0) {
+    if (how.top_p < 1.0f) {
         double total = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) total += q[e];
@@ -239,8 +244,9 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
     if (!all<G>((int)sure, Min())) return false;
 
     // Draws.  The lane whose places hold t is found from the lanes' sums; its places are then looked through by the group, from
-    // LDS (one a lane).  A lane with few places looks through them by itself.
+    // LDS.  A lane with few places looks through them by itself.
     constexpr bool BY_GROUP = E > 4;
+    constexpr int EACH = E > G ? E / G : 1;       // places of it a lane
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) sum += w[e];
@@ -260,15 +266,27 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
         int at = -1;
         if (BY_GROUP) {
             const int owner = all<G>(t >= upto && t < upto + sum ? lane : -1, Max());
-            const int place = max(owner, 0) * E + (lane & (E - 1));
-            float here = lds[place];
-            here = lane < E ? here : 0.0f;
-            upto = __shfl(upto, max(owner, 0), G);
-            upto += before<G>(here);
-            const bool mine = owner >= 0 && lane < E && t - upto > margin && upto + here - t > margin;
-            at = all<G>(mine ? place : -1, Max());
-            if (mine) lds[place] = 0.0f;
-            const float gone = all<G>(mine ? here : 0.0f, Add());
+            const int place = max(owner, 0) * E + (lane * EACH & (E - 1));
+            const bool has = lane * EACH < E;
+            float here[EACH], end = __shfl(upto, max(owner, 0), G), mine = 0.0f;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                here[e] = lds[place + e];
+                here[e] = has ? here[e] : 0.0f;
+                mine += here[e];
+            }
+            end += before<G>(mine);
+            float gone = 0.0f;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const bool clear = (owner >= 0) & has & (t - end > margin) & (end + here[e] - t > margin);
+                at = clear ? place + e : at;
+                gone = clear ? here[e] : gone;
+                end += here[e];
+            }
+            if (at >= 0) lds[at] = 0.0f;
+            at = all<G>(at, Max());
+            gone = all<G>(gone, Add());
             sum = lane == owner ? fmaxf(sum - gone, 0.0f) : sum;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
             __builtin_amdgcn_wave_barrier();
@@ -816,7 +834,7 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     if (!(m > -__builtin_inff())) return none(0);
     low_end = block.all(low_end, Min());
     const double m64 = (double)m, per = LOG2E / (double)how.temperature;
-    auto weight = [&](float v) { return v == m ? UNIT : v > -__builtin_inff() ? weight_of(((double)v - m64) * per) : 0.0; };
+    auto weight = [&](float v) { return weight_of(v == m ? 0.0 : ((double)v - m64) * per); };      // (-inf: 0)
     const double least = how.floor();
     const float octaves = fminf((m - low_end) * (float)per, OCTAVES);
     const float bins_per = by_p && !by_k && octaves > 0.0f ? (float)per * ((float)BINS / octaves) : 1.0f;
@@ -1210,9 +1228,12 @@ template <typename T> int sample_rows(hipStream_t s, const T* x, SampleRows a) {
         return (int)(reinterpret_cast<uintptr_t>(x) % align == 0 && (a.ld * sizeof(T)) % align == 0);
     };
     auto blocks = [&](int g) { return dim3((unsigned)((a.rows * g + 255) / 256)); };
-    if (a.width <= 64) {
+    if (a.width <= 16) {
         a.vec = vec(4);
-        hipLaunchKernelGGL((k_sample<T, 16, 4>), blocks(16), dim3(256), 0, s, x, a);
+        hipLaunchKernelGGL((k_sample<T, 4, 4>), blocks(4), dim3(256), 0, s, x, a);
+    } else if (a.width <= 64) {
+        a.vec = vec(8);
+        hipLaunchKernelGGL((k_sample<T, 8, 8>), blocks(8), dim3(256), 0, s, x, a);
     } else if (a.width <= 256) {
         a.vec = vec(16);
         hipLaunchKernelGGL((k_sample<T, 16, 16>), blocks(16), dim3(256), 0, s, x, a);
@@ -1235,9 +1256,12 @@ template <typename T> int top_rows(hipStream_t s, const T* x, TopArgs a) {
         return (int)(reinterpret_cast<uintptr_t>(x) % align == 0 && (a.ld * sizeof(T)) % align == 0);
     };
     auto blocks = [&](int g) { return dim3((unsigned)((a.rows * g + 255) / 256)); };
-    if (a.width <= 64) {
+    if (a.width <= 16) {
         a.vec = vec(4);
-        hipLaunchKernelGGL((k_top<T, 16, 4, 0>), blocks(16), dim3(256), 0, s, x, a);
+        hipLaunchKernelGGL((k_top<T, 4, 4, 0>), blocks(4), dim3(256), 0, s, x, a);
+    } else if (a.width <= 64) {
+        a.vec = vec(8);
+        hipLaunchKernelGGL((k_top<T, 8, 8, 0>), blocks(8), dim3(256), 0, s, x, a);
     } else if (a.width <= 256) {
         a.vec = vec(16);
         if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 16, 16, 4>), blocks(16), dim3(256), 0, s, x, a);
