@@ -160,8 +160,8 @@ template <int G, typename V> __device__ __forceinline__ V before(V v) {
 // and are exact in f64 in whatever order they are taken - by lanes, by blocks, by atomics - so a draw is a function of its
 // row alone.  What is lost is a weight's 2^-37, far below the 2^-24 steps of the random numbers.
 constexpr double UNIT = 68719476736.0;          // 2^36
-// 2^(d + SHIFT), d in [-900, 900].  2^f on |f| <= 1/2 by its series ln2^k / k!, k = 11 .. 0: the first term left out is below
-// 7e-15 (ln2^12 / (12! 2^12)), a hundredth of a step of what it is used for (2^-36 here, 2^-24 elsewhere).  The coefficients are
+// 2^(d + SHIFT), d in [-900, 900], to 4e-14 of itself (2^-44; what it is used for has steps of 2^-36 and 2^-24): on |f| <= 1/2,
+// 2^f = 1 + f P(f) with the P of degree 8 whose largest error is least (Remez exchange).  Exact at d = 0.  The coefficients are
 // held in scalar registers: as literals each costs two vector moves beside its product.
 __device__ __forceinline__ double scalar(double c) {
     asm("" : "+s"(c));
@@ -169,17 +169,15 @@ __device__ __forceinline__ double scalar(double c) {
 }
 template <int SHIFT> __device__ __forceinline__ double pow2(double d) {
     const double n = __builtin_rint(d), f = d - n;
-    double p = scalar(4.4455382718708110e-10);
-    p = fma(p, f, scalar(7.0549116208011210e-09));
-    p = fma(p, f, scalar(1.0178086009239696e-07));
-    p = fma(p, f, scalar(1.3215486790144305e-06));
-    p = fma(p, f, scalar(1.5252733804059838e-05));
-    p = fma(p, f, scalar(1.5403530393381606e-04));
-    p = fma(p, f, scalar(1.3333558146428441e-03));
-    p = fma(p, f, scalar(9.6181291076284772e-03));
-    p = fma(p, f, scalar(5.5504108664821576e-02));
-    p = fma(p, f, scalar(2.4022650695910070e-01));
-    p = fma(p, f, scalar(6.9314718055994531e-01));
+    double p = scalar(1.0208624985451055e-07);
+    p = fma(p, f, scalar(1.3255224921011604e-06));
+    p = fma(p, f, scalar(1.5252659326736988e-05));
+    p = fma(p, f, scalar(1.5403455852016875e-04));
+    p = fma(p, f, scalar(1.3333558222014398e-03));
+    p = fma(p, f, scalar(9.6181291594041980e-03));
+    p = fma(p, f, scalar(5.5504108664546310e-02));
+    p = fma(p, f, scalar(2.4022650695812967e-01));
+    p = fma(p, f, scalar(6.9314718055994710e-01));
     p = fma(p, f, 1.0);
     return p * __longlong_as_double((long long)(1023 + SHIFT + (int)n) << 52);
 }
@@ -359,14 +357,20 @@ template <typename T> struct Span {
             const float v[PER] = {as_float(x[first])};
             f(first, v, 1);
         }
-#pragma unroll 2
-        for (int k = first; k < vecs; k += step) {
-            union { uint4 w; T t[PER]; } u;
-            u.w = reinterpret_cast<const uint4*>(x + head)[k];
-            float v[PER];
+        // (four vectors on their way at a time: one CU's share of memory is latency)
+        for (int k0 = first; k0 < vecs; k0 += 4 * step) {
+            union { uint4 w; T t[PER]; } u[4];
 #pragma unroll
-            for (int j = 0; j < PER; ++j) v[j] = as_float(u.t[j]);
-            f(head + k * PER, v, PER);
+            for (int b = 0; b < 4; ++b) u[b].w = reinterpret_cast<const uint4*>(x + head)[min(k0 + b * step, vecs - 1)];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int k = k0 + b * step;
+                if (k >= vecs) break;
+                float v[PER];
+#pragma unroll
+                for (int j = 0; j < PER; ++j) v[j] = as_float(u[b].t[j]);
+                f(head + k * PER, v, PER);
+            }
         }
         const int tail = head + vecs * PER + first;
         if (tail < n) {

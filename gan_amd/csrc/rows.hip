@@ -834,7 +834,7 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
     if (!(m > -__builtin_inff())) return none(0);
     low_end = block.all(low_end, Min());
     const double m64 = (double)m, per = LOG2E / (double)how.temperature;
-    auto weight = [&](float v) { return weight_of(v == m ? 0.0 : ((double)v - m64) * per); };      // (-inf: 0)
+    auto weight = [&](float v) { return weight_of(((double)v - m64) * per); };      // (-inf, which holds nothing: 0)
     const double least = how.floor();
     const float octaves = fminf((m - low_end) * (float)per, OCTAVES);
     const float bins_per = by_p && !by_k && octaves > 0.0f ? (float)per * ((float)BINS / octaves) : 1.0f;
