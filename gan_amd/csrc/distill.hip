@@ -399,7 +399,7 @@ extern "C" int aig_distill_rows(const aig_distill* d, float* loss, void* grad, i
     AIG_REQUIRE(d->dtype == AIG_F32 || d->dtype == AIG_F16 || d->dtype == AIG_BF16, "aig_distill_rows: unknown dtype %d", d->dtype);
     if (const int rc = check_row_limits("aig_distill_rows", d->rows, d->width)) return rc;
     AIG_REQUIRE(d->m >= 1 && d->m <= AIG_ROWS_MAX_TOP, "aig_distill_rows: m=%lld is not in 1..%d", (long long)d->m, AIG_ROWS_MAX_TOP);
-    AIG_REQUIRE(d->temperature > 0.0f && d->temperature < __builtin_inff(), "aig_distill_rows: the temperature must be positive and finite");
+    AIG_REQUIRE(d->temperature >= 1e-6f && d->temperature <= 1e6f, "aig_distill_rows: the temperature %g is not in 1e-6..1e6", (double)d->temperature);
     AIG_REQUIRE(!grad || grad_ld >= d->width, "aig_distill_rows: rows of the gradient overlap (grad_ld=%lld)", (long long)grad_ld);
     AIG_REQUIRE(upstream_stride == 0 || upstream_stride == 1, "aig_distill_rows: upstream_stride is 0 or 1");
     if (d->rows == 0) return AIG_OK;

@@ -1331,7 +1331,7 @@ extern "C" int aig_top_rows(int64_t rows, int64_t width, int64_t ld, int dtype, 
                             int64_t m, float temperature, float* values, int32_t* index, float* lse, void* stream) {
     if (const int rc = check_rows("aig_top_rows", rows, width, ld, dtype)) return rc;
     AIG_REQUIRE(m >= 1 && m <= AIG_ROWS_MAX_TOP, "aig_top_rows: m=%lld is not in 1..%d", (long long)m, AIG_ROWS_MAX_TOP);
-    AIG_REQUIRE(temperature > 0.0f, "aig_top_rows: the temperature must be positive");
+    AIG_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, "aig_top_rows: the temperature %g is not in 1e-6..1e6", (double)temperature);
     if (rows == 0) return AIG_OK;
     AIG_REQUIRE(logits && values && index && lse, "aig_top_rows: null pointer");
     TopArgs a{};

@@ -17,7 +17,6 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
-import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -177,8 +176,8 @@ def top_rows(logits: torch.Tensor, m: int, counts: Optional[torch.Tensor] = None
     m, temperature = int(m), float(temperature)
     if not 1 <= m <= MAX_TOP:
         raise ValueError(f"top_rows keeps 1 to {MAX_TOP} logits a row, got {m}")
-    if not 0 < temperature < math.inf:
-        raise ValueError(f"the temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"the temperature must be within 1e-6 and 1e6, got {temperature}")
     device = logits.device
     counts_ptr = _side(counts, (rows,), torch.int32, device, "counts")
     values = torch.empty((rows, m), dtype=torch.float32, device=device)
@@ -194,8 +193,8 @@ def _teacher(logits, top, counts, weight, temperature, tail, scale=1.0):
     """The argument block of a distillation, and the tensors it points to (they must outlive the calls that take it)."""
     rows, width, ld, dtype = _rows_of(logits, "distill_loss")
     temperature = float(temperature)
-    if not 0 < temperature < math.inf:
-        raise ValueError(f"the temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"the temperature must be within 1e-6 and 1e6, got {temperature}")
     values, index, lse = top[0], top[1], top[2]
     if not torch.is_tensor(values) or values.dim() != 2 or not 1 <= int(values.size(1)) <= MAX_TOP:
         raise _abi.AigAbiError(f"a teacher's values are [rows, 1 to {MAX_TOP}]")
@@ -232,6 +231,13 @@ def _sum_rows(v: torch.Tensor) -> torch.Tensor:
     ws = _abi.workspace(need, v.device) if need else None
     _call("aig_sum_rows", v.device, v.numel(), v.data_ptr(), 1.0, out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out
+
+
+def _refuse_recording(t: torch.Tensor, what: str, instead: str) -> None:
+    """A recorded backward pass accumulates into its leaves on the stream that they were first used on; where an eager graph of
+    the same leaves lives, that is not the recording's, and the runtime ends the process."""
+    if t.requires_grad and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        raise _abi.AigAbiError(f"{what} builds an autograd graph, which is not recorded into a HIP graph: record {instead}, which needs none")
 
 
 def _refuse_second_derivative(what: str) -> None:
@@ -280,13 +286,15 @@ def distill_loss(logits: torch.Tensor, top: TopRows, counts: Optional[torch.Tens
     are not listed, as one outcome with the teacher's remaining probability.  False: ``q`` is normalised over the listed
     entries and the second term is left out.  Entries whose place is not one of the student row's valid places (-1 among
     them) are left out; a row without valid places or without entries has loss 0 and gradient 0.  ``reduction`` is "none"
-    (float32 ``[rows]``), "sum" or "mean" (over the rows)."""
+    (float32 ``[rows]``), "sum" or "mean" (over the rows).  ``temperature`` is within 1e-6 and 1e6.  Differentiable once; into a
+    HIP graph, record ``distill_loss_and_grad``."""
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"reduction is 'none', 'sum' or 'mean', got {reduction!r}")
     rows = int(logits.size(0)) if torch.is_tensor(logits) and logits.dim() else 0
     if reduction == "mean" and rows == 0:
         raise ValueError("the mean over no rows")
     arg, held = _teacher(logits, top, counts, weight, temperature, tail, 1.0 / rows if reduction == "mean" else 1.0)
+    _refuse_recording(logits, "distill_loss of logits that require a gradient", "distill_loss_and_grad")
     return _DistillLoss.apply(logits, arg, held, reduction != "none")
 
 
@@ -356,11 +364,12 @@ def class_scores_grad(grad: torch.Tensor, windows: ScoreWindows, kinds: int, cla
 
 def class_scores(table: torch.Tensor, windows: ScoreWindows) -> torch.Tensor:
     """Logits ``[rows, width]`` looked up in ``table`` (float32 ``[kinds, classes]``) by the kind of the row and the class of
-    the candidate, differentiable in the table: nodes with equal feature rows score alike, so a template's candidate
+    the candidate, differentiable (once) in the table: nodes with equal feature rows score alike, so a template's candidate
     logits are a table of a few entries.  Places past a row's count, and candidates, classes or kinds outside their range,
     are ``-inf``."""
     if not torch.is_tensor(table) or not table.is_cuda:
         raise _abi.AigAbiError("class_scores needs the table on a HIP device (no CPU path exists)")
     if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
         raise _abi.AigAbiError(f"class_scores takes a contiguous float32 table [kinds, classes], got {table.dtype} {tuple(table.shape)}")
+    _refuse_recording(table, "class_scores of a table that requires a gradient", "class_scores(table.detach()) and class_scores_grad")
     return _ClassScores.apply(table, windows, _windows_arg(table, int(table.size(0)), int(table.size(1)), windows))

@@ -666,8 +666,9 @@ int aig_pad_batch(int64_t B, int64_t n, int64_t ecap, const int32_t* ecount, con
  * rows of `width` places, row r at logits + r*ld elements (f32, IEEE halfs or bf16), of which the first counts[r] are
  * valid (counts NULL: all; a count outside 0..width is taken as the nearer bound).  A valid place holds nothing when
  * its logit is -inf; what lies past a row's count is never read as a value.  Widths to AIG_ROWS_MAX_WIDTH; rows of up
- * to 1024 places are held in registers, wider ones are a workgroup's each.  The reference has none of these
- * (its generator takes torch.topk, models/generator.py:162-168, and never receives a gradient, train.py:297-299).
+ * to 1024 places are held in registers (at most 2^26 - 1 of them), wider ones are a workgroup's each (2^22 - 1).
+ * The reference has none of these (its generator takes torch.topk, models/generator.py:162-168, and never receives a
+ * gradient, train.py:297-299).
  * ------------------------------------------------------------------------------------------- */
 #define AIG_F32 0
 #define AIG_F16 1
@@ -708,7 +709,7 @@ int aig_gen_wire_batch_sampled(const aig_gen_wire_set* a, const aig_sampling* ho
 
 /* The m largest logits of each row (NaN and -inf never), largest first, equal ones by lowest place:
  *   values [rows,m] f32, index [rows,m] (places; absent entries -inf and -1), lse[r] = log sum exp(l / temperature)
- *   over the row's valid places (-inf for none) - what aig_distill_rows takes of a teacher. */
+ *   over the row's valid places (-inf for none) - what aig_distill_rows takes of a teacher.  temperature 1e-6 .. 1e6. */
 int aig_top_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const void* logits, const int32_t* counts, int64_t m,
                  float temperature, float* values, int32_t* index, float* lse, void* stream);
 
@@ -725,7 +726,7 @@ int aig_top_rows(int64_t rows, int64_t width, int64_t ld, int dtype, const void*
 typedef struct aig_distill {
     int64_t rows, width, ld, m;
     int32_t dtype;
-    float temperature;            /* positive, finite */
+    float temperature;            /* 1e-6 .. 1e6 */
     float scale;                  /* factor of every loss and gradient (1, or 1/rows for a mean) */
     const void* logits;
     const int32_t* counts;        /* may be NULL */

@@ -28,7 +28,8 @@ def test_sample_sizes(rows, width, ld, dtype, draws, rc):
     assert _abi.lib().aig_sample_rows(4, 4, 4, 0, None, None, None, C.byref(how), 1, P, P, None) == -1
 
 
-@pytest.mark.parametrize("m,temperature,rc", [(0, 1.0, -1), (257, 1.0, -1), (4, 0.0, -1), (4, -2.0, -1), (4, float("nan"), -1)])
+@pytest.mark.parametrize("m,temperature,rc", [(0, 1.0, -1), (257, 1.0, -1), (4, 0.0, -1), (4, -2.0, -1), (4, float("nan"), -1), (4, 1e-7, -1),
+                                              (4, float("inf"), -1)])
 def test_top_arguments(m, temperature, rc):
     assert _abi.lib().aig_top_rows(4, 8, 8, 0, P, None, m, temperature, P, P, P, None) == rc
 
@@ -41,7 +42,7 @@ def distill(**kw):
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(rows=-1), -1), (dict(width=0), -1), (dict(m=0), -1), (dict(m=257), -1), (dict(dtype=7), -1),
-                                   (dict(temperature=0.0), -1), (dict(temperature=float("inf")), -1), (dict(logits=None), -1),
+                                   (dict(temperature=0.0), -1), (dict(temperature=float("inf")), -1), (dict(temperature=2e6), -1), (dict(logits=None), -1),
                                    (dict(values=None), -1), (dict(width=1 << 20, ld=1 << 20), -4), (dict(rows=0), 0)])
 def test_distill_arguments(kw, rc):
     assert _abi.lib().aig_distill_rows(C.byref(distill(**kw)), P, None, 0, None, 0, None) == rc

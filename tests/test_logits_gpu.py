@@ -508,6 +508,33 @@ def test_on_another_stream_and_recorded(width):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
 
 
+def test_an_autograd_graph_is_not_recorded():
+    x = make_logits(8, 20, F32, seed=1).to(DEV).requires_grad_(True)
+    top = L.top_rows(x, 4)
+    cand, counts, cls, kind = make_windows(8, 20, 30, 2, 3, seed=2, counts=False)
+    w = L.ScoreWindows.of(cand.to(DEV), None, cls.to(DEV), kind.to(DEV), 2)
+    table = torch.zeros(2, 3, device=DEV, requires_grad=True)
+    alive = L.distill_loss(x, top), L.class_scores(table, w)         # an eager graph of the same leaves
+    want = L.distill_loss_and_grad(x, top)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        for call in (lambda: L.distill_loss(x, top), lambda: L.class_scores(table, w)):
+            with pytest.raises(_abi.AigAbiError, match="not recorded"):
+                call()
+        held = L.distill_loss_and_grad(x, top)
+    for _ in range(3):
+        for v in held:
+            v.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+    alive[0].backward()
+    assert x.grad is not None
+    loss = L.distill_loss(x, top)
+    with pytest.raises(RuntimeError, match="once"):
+        loss.backward(create_graph=True)
+
+
 def test_rows_far_apart():
     """Rows whose offsets pass 32 bits."""
     ld, width = 2 ** 31 + 1000, 2000
@@ -557,7 +584,7 @@ def test_refused_on_the_device():
             (lambda: L.sample_rows(x, u, temperature=torch.ones(3, device=DEV)), bad),
             (lambda: L.sample_rows(torch.zeros(1, L.MAX_WIDTH + 1, device=DEV), u[:1]), bad),
             (lambda: L.top_rows(x, 0), ValueError), (lambda: L.top_rows(x, 257), ValueError),
-            (lambda: L.top_rows(x, 2, temperature=0.0), ValueError),
+            (lambda: L.top_rows(x, 2, temperature=0.0), ValueError), (lambda: L.top_rows(x, 2, temperature=1e7), ValueError),
             (lambda: L.distill_loss(x, top, temperature=2.0), ValueError),              # lse taken at another temperature
             (lambda: L.distill_loss(x, L.TopRows(top.values, top.index, None)), ValueError),
             (lambda: L.distill_loss(x, top, reduction="max"), ValueError),
