@@ -41,8 +41,10 @@ __device__ __forceinline__ float probability(double log2_q) { return log2_q > 0.
 constexpr double FAINT = 1e-30;
 
 // A listed entry's probability is added to its place in LDS as a whole number of 2^-30, at least one: entries that name one
-// place twice add up to the same bits in any order, and a place is listed where the sum is not 0.
-constexpr float Q_UNIT = 1073741824.0f;
+// place twice add up to the same bits in any order, and a place is listed where the sum is not 0.  Only entries that repeat a
+// place can add up to the 4 that 32 bits do not hold: where a row's entries come near it, they are added again in steps of
+// 2^-23 (256 of them reach 2^31).
+constexpr float Q_UNIT = 1073741824.0f, Q_COARSE = 8388608.0f;
 
 template <typename T, int G, int E, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __restrict__ grad, DistillArgs a) {
@@ -109,6 +111,19 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
     sum_q = all<G>(sum_q, Add());
     const bool live = z != 0.0 && sum_q != 0.0;        // (a NaN among the logits is not nothing: it shows in the loss)
     sum_q -= NAMED * __builtin_floor(sum_q * (1.0 / NAMED));
+    float q_step = 1.0f / Q_UNIT;
+    if (GRAD && sum_q >= 3.5) {
+        q_step = 1.0f / Q_COARSE;
+#pragma unroll
+        for (int e = 0; e < E; ++e) listed[lane * E + e] = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        for (int j = lane; j < a.m; j += G)
+            if (names(index[j], values[j], n)) {
+                const float q = probability((double)values[j] * a.per - lse);
+                atomicAdd(&listed[index[j]], max((unsigned)__float2int_rn(q * Q_COARSE), 1u));
+            }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
 
@@ -152,7 +167,7 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             float d = faint && !q_here[e] ? exp2_fast((v[e] - rest_top) * per) : ex[e];
-            d = q_here[e] ? (float)q_here[e] * (1.0f / Q_UNIT) : d * outside;
+            d = q_here[e] ? (float)q_here[e] * q_step : d * outside;
             g[e] = from_float<T>(lane * E + e < n && live ? c * (ex[e] * full - d) : 0.0f);
         }
         grad += r * a.grad_ld;
@@ -328,14 +343,14 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
             });
         for (int i = (live ? n : 0) + t; i < a.width; i += WIDE_T) grad[i] = from_float<T>(0.0f);
         if (live && i_mine >= 0) {        // a listed place is written by the first entry that names it, for all of them
-            float s = 0.0f;
+            double s = 0.0;
             bool is_first = true;
             for (int j = 0; j < a.m; ++j)
                 if (place[j] == i_mine) {
                     is_first = is_first && j >= t;
-                    s += prob[j];
+                    s += (double)prob[j];
                 }
-            if (is_first) grad[i_mine] = from_float<T>(c * (exp2_fast((as_float(x[i_mine]) - base) * per) * full - s));
+            if (is_first) grad[i_mine] = from_float<T>(c * (exp2_fast((as_float(x[i_mine]) - base) * per) * full - (float)s));
         }
     }
 }

@@ -329,6 +329,24 @@ def test_distill_every_unmasked_place_listed(width):
     assert torch.isfinite(loss).all() and torch.isfinite(grad).all() and not grad[:, 1::9].any()
 
 
+@pytest.mark.parametrize("width", [5, 48, 200, 500, 1000, 1500])
+def test_distill_one_place_named_many_times(width):
+    """Entries that repeat a place add up to more than a row's probability.  (The bounds hold: entries of q each, added in
+    steps of 2^-23, are off by 2^-24 each; 16 half steps of their sum are more than that from a q of 1/16.)"""
+    x = make_logits(6, width, F32, seed=width)
+    for m in (4, 5, 8, 256):
+        i = torch.full((6, m), 3, dtype=torch.int32)
+        i[1, -1] = 1
+        i[2, ::2] = 0
+        v = torch.full((6, m), 1.5)
+        v[3] -= 0.25 * torch.rand(m, generator=rng(m))
+        v[4, 1:] = -3.0
+        s = torch.full((6,), 1.5)
+        s[5] = 1.0                               # (a log-sum-exp below the entries: probabilities stay at 1)
+        check_distill(x, v, i, s, 1.0)
+        check_distill(x, v, i, None, 1.0)
+
+
 def test_distill_listed_everywhere_has_no_rest():
     x = make_logits(7, 8, F32, seed=2)
     v, i, s = make_teacher(x, 8, 1.0, 1, None, True)
