@@ -240,7 +240,9 @@ def _refuse_recording(t: torch.Tensor, what: str, instead: str) -> None:
         raise _abi.AigAbiError(f"{what} builds an autograd graph, which is not recorded into a HIP graph: record {instead}, which needs none")
 
 
-def _refuse_second_derivative(what: str) -> None:
+def _check_backward(what: str) -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise _abi.AigAbiError(f"the backward pass of {what} is not recorded into a HIP graph")
     if torch.is_grad_enabled():        # (a backward pass runs with it on only when its own graph is asked for)
         raise RuntimeError(f"{what} can be differentiated once: call backward without create_graph")
 
@@ -259,7 +261,7 @@ class _DistillLoss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        _refuse_second_derivative("distill_loss")
+        _check_backward("distill_loss")
         logits, *held = ctx.saved_tensors
         a = ctx.arg
         a.logits = logits.data_ptr()       # (hooks on saved tensors may hand out copies)
@@ -335,7 +337,7 @@ class _ClassScores(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        _refuse_second_derivative("class_scores")
+        _check_backward("class_scores")
         a, held = ctx.arg, ctx.saved_tensors
         for name, v in zip(ScoreWindows._fields, held):
             if v is not None:

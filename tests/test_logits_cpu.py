@@ -85,3 +85,12 @@ def test_sampling_flags():
     for bad in (("--temperature", "-1"), ("--temperature", "nan"), ("--top-k", "-2"), ("--top-p", "1.5"), ("--min-p", "-0.1")):
         with pytest.raises(SystemExit):
             parse(*bad)
+
+
+def test_a_backward_pass_is_not_recorded(monkeypatch):
+    with torch.no_grad():
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        L._check_backward("distill_loss")
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(_abi.AigAbiError, match="not recorded"):
+            L._check_backward("distill_loss")
