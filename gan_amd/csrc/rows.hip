@@ -172,7 +172,7 @@ constexpr float MARGIN = 1.0f / 262144.0f;
 
 template <int G, int E>
 __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettings& how, long long r, int lane, int n, int want,
-                                            const float (&v)[E], float m, float* lds, unsigned& guess) {
+                                            const float (&v)[E], float m, float* lds, float& guess) {
     const float per = how.per;
     bool sure = per > 0.0f && per < 1e30f && m < __builtin_inff();
     float w[E];
@@ -180,56 +180,67 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
     for (int e = 0; e < E; ++e) w[e] = __builtin_amdgcn_exp2f((v[e] - m) * per);
     const bool by_p = how.top_p < 1.0f;
     if (by_p || (how.top_k > 0 && how.top_k < a.width)) {
-        // in the order of the keys the places that stay are the first `keep`
-        unsigned key[E], s[E];
+        // In the order of the weights the places that stay are the first `keep`.  That is the order of the logits but for the
+        // last bit of an exponential, and for logits whose weights round to one number: see below.
+        unsigned s[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[e] = key[e] = key_of(v[e]);
+        for (int e = 0; e < E; ++e) s[e] = __float_as_uint(w[e]);
         sort_keys<G, E>(s, lane);
         int keep = how.top_k > 0 ? min(how.top_k, a.width) : a.width;
         if (by_p) {
+            const bool by_k = keep < G * E;
             float ws[E], sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                ws[e] = __builtin_amdgcn_exp2f((value_of(s[e]) - m) * per);
-                ws[e] = lane * E + e < keep ? ws[e] : 0.0f;
+                ws[e] = __uint_as_float(s[e]);
+                if (by_k) ws[e] = lane * E + e < keep ? ws[e] : 0.0f;
                 sum += ws[e];
             }
-            const float total = all<G>(sum, Add()), p = how.top_p * total, margin = MARGIN * total;
+            const float total = all<G>(sum, Add()), p = how.top_p * total;
             float upto = before<G>(sum), nearest = 1e30f;
             int stay = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                // (the first place always stays; past the last one there is nothing to decide)
-                const float gap = lane * E + e > 0 && lane * E + e < keep ? upto - p : -1e30f;
-                nearest = fminf(nearest, fabsf(gap));
-                stay += gap < 0.0f;
+                // (the first place always stays; behind the last one the whole of the total is in front)
+                nearest = e > 0 || lane > 0 ? fminf(nearest, fabsf(upto - p)) : nearest;
+                stay += upto < p;
                 upto += ws[e];
             }
-            sure = sure && nearest > margin;
-            // (places past `keep` were counted as staying)
-            keep = min(keep, all<G>(stay, Add()) - (G * E - keep));
+            sure = sure && nearest > MARGIN * total;
+            keep = max(min(keep, all<G>(stay, Add())), 1);
         }
-        const unsigned thr = at_rank<G, E>(s, keep - 1);
-        if (thr > NO_KEY) {
+        const float thr = __uint_as_float(at_rank<G, E>(s, keep - 1));
+        if (thr > 0.0f) {       // (else every weight stays)
             guess = thr;
-            int over = 0, here = 0;       // places over the threshold, and at it
+            // Places whose weight is within a few last bits of the border's: all of them stay, or their logits are equal and the
+            // first of them do - or the exact form has to tell them apart.
+            const float high = thr * (1.0f + 1.0f / 1048576.0f), low = thr * (1.0f - 1.0f / 1048576.0f);
+            int over = 0, from = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                over += key[e] > thr;
-                here += key[e] == thr;
+                over += w[e] > high;
+                from += w[e] >= low;
             }
-            const int both = all<G>(over | here << 16, Add()), quota = keep - (both & 0xFFFF);
-            if ((both >> 16) > quota) {
+            const int both = all<G>(over | from << 16, Add()), quota = keep - (both & 0xFFFF);
+            if ((both >> 16) > keep) {
+                float border = -__builtin_inff();           // the largest logit that is not over it
+#pragma unroll
+                for (int e = 0; e < E; ++e) border = w[e] > high ? border : fmaxf(border, v[e]);
+                border = all<G>(border, Max());
+                int here = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) here += v[e] == border;
                 int tie = before<G>(here);
+                sure = sure && all<G>(here, Add()) == (both >> 16) - (both & 0xFFFF);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const bool at = key[e] == thr;
-                    w[e] = key[e] > thr || (at && tie < quota) ? w[e] : 0.0f;
+                    const bool at = v[e] == border;
+                    w[e] = (v[e] > border) | (at & (tie < quota)) ? w[e] : 0.0f;
                     tie += at;
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) w[e] = key[e] >= thr ? w[e] : 0.0f;
+                for (int e = 0; e < E; ++e) w[e] = w[e] >= low ? w[e] : 0.0f;
             }
         }
     }
@@ -358,12 +369,14 @@ __global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleR
             if (lane == 0) a.store(r, d, -1, first, n);
         return;
     }
-    unsigned guess = 0;
+    float guess = 0.0f;
     if (!quick_draws<G, E>(a, how, r, lane, n, want, v, m, lds[E > 4 ? threadIdx.x / G : 0], guess)) {
         unsigned key[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) key[e] = key_of(v[e]);
-        exact_draws<G, E>(a, how, r, lane, n, want, key, key_of(m), guess);
+        // (the logit that has the border's weight, or one near it)
+        const unsigned near = guess > 0.0f ? key_of(m + __builtin_amdgcn_logf(guess) / how.per) : 0u;
+        exact_draws<G, E>(a, how, r, lane, n, want, key, key_of(m), near);
     }
 }
 
