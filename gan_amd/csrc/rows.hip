@@ -170,6 +170,97 @@ __device__ __forceinline__ void exact_draws(const SampleRows& a, const RowSettin
 // instructions a place, and sums in f32 take their lane permutations along.
 constexpr float MARGIN = 1.0f / 262144.0f;
 
+// Weights that cannot be told apart by their order: exponentials of different logits are in order but for two last bits (2^-22).
+__device__ __forceinline__ float band_high(float thr) { return thr * (1.0f + 1.0f / 1048576.0f); }
+__device__ __forceinline__ float band_low(float thr) { return thr * (1.0f - 1.0f / 1048576.0f); }
+
+// Top-p's border without sorting the row.  What goes is (1 - p) of the total on fewer than n places, none larger than the last
+// place that stays: that one's weight is at least lo = (1 - p) total / n.  The bits between lo and the largest weight are halved
+// (a comparison, a selection and an addition a place each time; the bits of a float are nearly its logarithm) until few places
+// lie between, and those are sorted.  152,896 rows of 256: two halvings do for most, 89 -> SORT us.
+// lds: [LISTED].  Returns false where places do not get few (hundreds of equal ones); keep, over and from count inside the list.
+constexpr int LISTED_A_LANE_16 = 4, LISTED_A_LANE_64 = 2, HALVINGS = 12;
+template <int G, int E>
+__device__ __forceinline__ bool border_by_mass(const float (&w)[E], float top_p, int n, int lane, float* lds, bool& sure, float& thr,
+                                               int& keep, int& over, int& from) {
+    constexpr int M = G == 16 ? LISTED_A_LANE_16 : LISTED_A_LANE_64;
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += w[e];
+    const float total = all<G>(sum, Add()), p = top_p * total, margin = MARGIN * total;
+    unsigned lo = __float_as_uint(fmaxf((total - p) / (float)n * 0.999f, 1e-30f)), hi = __float_as_uint(1.0f) + 1u;
+    float front = 0.0f;          // the mass of the places from hi on: below p; that from lo on is not
+    auto halve = [&]() {
+        const unsigned mid = lo + (hi - lo) / 2;
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += __float_as_uint(w[e]) >= mid ? w[e] : 0.0f;
+        s = all<G>(s, Add());
+        const bool enough = s >= p;
+        lo = enough ? mid : lo;
+        hi = enough ? hi : mid;
+        front = enough ? front : s;
+    };
+    halve();
+    int count = 0, here, round = 0;
+    do {
+        halve();
+        here = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) here += __float_as_uint(w[e]) - lo < hi - lo;
+        count = all<G>(here, Add());
+    } while (count > G * M && ++round < HALVINGS);
+    if (count > G * M) return false;
+    int at = before<G>(here);
+#pragma unroll
+    for (int e = 0; e < M; ++e) lds[lane * M + e] = 0.0f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (__float_as_uint(w[e]) - lo < hi - lo) lds[at++] = w[e];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    unsigned s[M];
+    float mine = 0.0f;
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+        const float v = lds[lane * M + e];
+        s[e] = __float_as_uint(v);
+        mine += v;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    const float end = front + all<G>(mine, Add());
+    sort_keys<G, M>(s, lane);
+    mine = 0.0f;
+#pragma unroll
+    for (int e = 0; e < M; ++e) mine += __uint_as_float(s[e]);
+    float upto = front + before<G>(mine), nearest = end - p;       // (negative: the list ends too early)
+    int stay = 0;
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+        // (the first place of the row always stays)
+        nearest = e > 0 || lane > 0 || front > 0.0f ? fminf(nearest, fabsf(upto - p)) : nearest;
+        stay += upto < p;
+        upto += __uint_as_float(s[e]);
+    }
+    sure = sure && all<G>(nearest, Min()) > margin;
+    keep = max(all<G>(stay, Add()), 1);
+    thr = __uint_as_float(at_rank<G, M>(s, keep - 1));
+    const float high = band_high(thr), low = band_low(thr);
+    sure = sure && __float_as_uint(low) >= lo && __float_as_uint(high) < hi;       // (else the band is not all in the list)
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+        over += __uint_as_float(s[e]) > high;
+        from += __uint_as_float(s[e]) >= low;
+    }
+    const int both = all<G>(over | from << 16, Add());
+    over = both & 0xFFFF;
+    from = both >> 16;
+    return true;
+}
+
 template <int G, int E>
 __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettings& how, long long r, int lane, int n, int want,
                                             const float (&v)[E], float m, float* lds, float& guess) {
@@ -178,51 +269,59 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
     float w[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) w[e] = __builtin_amdgcn_exp2f((v[e] - m) * per);
-    const bool by_p = how.top_p < 1.0f;
-    if (by_p || (how.top_k > 0 && how.top_k < a.width)) {
-        // In the order of the weights the places that stay are the first `keep`.  That is the order of the logits but for the
+    const bool by_p = how.top_p < 1.0f, by_k = how.top_k > 0 && how.top_k < a.width;
+    if (by_p || by_k) {
+        // In the order of the weights the places that stay are the first ones.  That is the order of the logits but for the
         // last bit of an exponential, and for logits whose weights round to one number: see below.
-        unsigned s[E];
+        float thr = 0.0f;                       // the weight of the last place that stays
+        int keep = 0, over = 0, from = 0;       // of some run of the order around it: places that stay, over the band below, and not under it
+        bool found = false;
+        if constexpr (G >= 16) found = by_p && !by_k && border_by_mass<G, E>(w, how.top_p, n, lane, lds, sure, thr, keep, over, from);
+        if (!found) {
+            unsigned s[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[e] = __float_as_uint(w[e]);
-        sort_keys<G, E>(s, lane);
-        int keep = how.top_k > 0 ? min(how.top_k, a.width) : a.width;
-        if (by_p) {
-            const bool by_k = keep < G * E;
-            float ws[E], sum = 0.0f;
+            for (int e = 0; e < E; ++e) s[e] = __float_as_uint(w[e]);
+            sort_keys<G, E>(s, lane);
+            keep = by_k ? how.top_k : G * E;
+            if (by_p) {
+                float ws[E], sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                ws[e] = __uint_as_float(s[e]);
-                if (by_k) ws[e] = lane * E + e < keep ? ws[e] : 0.0f;
-                sum += ws[e];
+                for (int e = 0; e < E; ++e) {
+                    ws[e] = __uint_as_float(s[e]);
+                    if (by_k) ws[e] = lane * E + e < keep ? ws[e] : 0.0f;
+                    sum += ws[e];
+                }
+                const float total = all<G>(sum, Add()), p = how.top_p * total;
+                float upto = before<G>(sum), nearest = 1e30f;
+                int stay = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    // (the first place always stays; behind the last one the whole of the total is in front)
+                    nearest = e > 0 || lane > 0 ? fminf(nearest, fabsf(upto - p)) : nearest;
+                    stay += upto < p;
+                    upto += ws[e];
+                }
+                sure = sure && nearest > MARGIN * total;
+                keep = max(min(keep, all<G>(stay, Add())), 1);
             }
-            const float total = all<G>(sum, Add()), p = how.top_p * total;
-            float upto = before<G>(sum), nearest = 1e30f;
-            int stay = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                // (the first place always stays; behind the last one the whole of the total is in front)
-                nearest = e > 0 || lane > 0 ? fminf(nearest, fabsf(upto - p)) : nearest;
-                stay += upto < p;
-                upto += ws[e];
-            }
-            sure = sure && nearest > MARGIN * total;
-            keep = max(min(keep, all<G>(stay, Add())), 1);
-        }
-        const float thr = __uint_as_float(at_rank<G, E>(s, keep - 1));
-        if (thr > 0.0f) {       // (else every weight stays)
-            guess = thr;
-            // Places whose weight is within a few last bits of the border's: all of them stay, or their logits are equal and the
-            // first of them do - or the exact form has to tell them apart.
-            const float high = thr * (1.0f + 1.0f / 1048576.0f), low = thr * (1.0f - 1.0f / 1048576.0f);
-            int over = 0, from = 0;
+            thr = __uint_as_float(at_rank<G, E>(s, keep - 1));
+            const float high = band_high(thr), low = band_low(thr);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 over += w[e] > high;
                 from += w[e] >= low;
             }
-            const int both = all<G>(over | from << 16, Add()), quota = keep - (both & 0xFFFF);
-            if ((both >> 16) > keep) {
+            const int both = all<G>(over | from << 16, Add());
+            over = both & 0xFFFF;
+            from = both >> 16;
+        }
+        if (thr > 0.0f) {       // (else every weight stays)
+            guess = thr;
+            // Places whose weight is within a few last bits of the border's: all of them stay, or their logits are equal and the
+            // first of them do - or the exact form has to tell them apart.
+            const float high = band_high(thr), low = band_low(thr);
+            if (from > keep) {
+                const int quota = keep - over;
                 float border = -__builtin_inff();           // the largest logit that is not over it
 #pragma unroll
                 for (int e = 0; e < E; ++e) border = w[e] > high ? border : fmaxf(border, v[e]);
@@ -231,7 +330,7 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
 #pragma unroll
                 for (int e = 0; e < E; ++e) here += v[e] == border;
                 int tie = before<G>(here);
-                sure = sure && all<G>(here, Add()) == (both >> 16) - (both & 0xFFFF);
+                sure = sure && all<G>(here, Add()) == from - over;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const bool at = v[e] == border;
