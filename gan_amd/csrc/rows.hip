@@ -174,43 +174,69 @@ constexpr float MARGIN = 1.0f / 262144.0f;
 __device__ __forceinline__ float band_high(float thr) { return thr * (1.0f + 1.0f / 1048576.0f); }
 __device__ __forceinline__ float band_low(float thr) { return thr * (1.0f - 1.0f / 1048576.0f); }
 
-// Top-p's border without sorting the row.  What goes is (1 - p) of the total on fewer than n places, none larger than the last
-// place that stays: that one's weight is at least lo = (1 - p) total / n.  The bits between lo and the largest weight are halved
-// (a comparison, a selection and an addition a place each time; the bits of a float are nearly its logarithm) until few places
-// lie between, and those are sorted.  152,896 rows of 256: two halvings do for most, 89 -> SORT us.
-// lds: [LISTED].  Returns false where places do not get few (hundreds of equal ones); keep, over and from count inside the list.
-constexpr int LISTED_A_LANE_16 = 4, LISTED_A_LANE_64 = 2, HALVINGS = 12;
+// The border of top-p, or of a top-k of few places and then top-p, without sorting the row: the bits between a lower bound of
+// it and the largest weight are halved (the bits of a float are nearly its logarithm) until few places lie between, and those
+// are sorted.  Top-p: what goes is (1 - p) of the total on fewer than n places, none larger than the last place that stays, so
+// that one's weight is at least (1 - p) total / n; a halving is a comparison, a selection and an addition a place, and two do
+// for most rows of 256.  Top-k: by the number of places, from their mean weight; the list is all places from lo on.
+// 152,896 rows of 256, top-p 0.9: 89 us sorted whole, 64 like this.
+// lds: [G M].  Returns false where places do not get few (hundreds of equal ones); keep, over and from count inside the list.
+constexpr int HALVINGS = 12;
+template <int G> __device__ __host__ constexpr int listed_a_lane() { return G == 16 ? 4 : 2; }
 template <int G, int E>
-__device__ __forceinline__ bool border_by_mass(const float (&w)[E], float top_p, int n, int lane, float* lds, bool& sure, float& thr,
-                                               int& keep, int& over, int& from) {
-    constexpr int M = G == 16 ? LISTED_A_LANE_16 : LISTED_A_LANE_64;
+__device__ __forceinline__ bool border_in_list(const float (&w)[E], int top_k, float top_p, int n, int lane, float* lds, bool& sure,
+                                               float& thr, int& keep, int& over, int& from) {
+    constexpr int M = listed_a_lane<G>();
+    const bool by_k = top_k > 0, by_p = top_p < 1.0f;
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) sum += w[e];
-    const float total = all<G>(sum, Add()), p = top_p * total, margin = MARGIN * total;
-    unsigned lo = __float_as_uint(fmaxf((total - p) / (float)n * 0.999f, 1e-30f)), hi = __float_as_uint(1.0f) + 1u;
-    float front = 0.0f;          // the mass of the places from hi on: below p; that from lo on is not
-    auto halve = [&]() {
-        const unsigned mid = lo + (hi - lo) / 2;
-        float s = 0.0f;
+    float total = all<G>(sum, Add()), p = top_p * total;
+    constexpr float LEAST = 1e-30f;
+    constexpr unsigned TOP = 0x3F800001u;        // over the bits of 1, the largest weight
+    unsigned lo = __float_as_uint(by_k ? LEAST : fmaxf((total - p) / (float)n * 0.999f, LEAST)), hi = TOP;
+    float front = 0.0f;          // top-p: the mass of the places from hi on: below p; that from lo on is not
+    int count = n, here = 0;
+    if (by_k) {                  // fewer than top_k places from hi on; from lo on there are as many, or lo is LEAST
+        unsigned mid = __float_as_uint(fmaxf(total / (float)n, 2.0f * LEAST));
+        for (int round = 0; count > G * M && round < HALVINGS; ++round) {
+            int c = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += __float_as_uint(w[e]) >= mid ? w[e] : 0.0f;
-        s = all<G>(s, Add());
-        const bool enough = s >= p;
-        lo = enough ? mid : lo;
-        hi = enough ? hi : mid;
-        front = enough ? front : s;
-    };
-    halve();
-    int count = 0, here, round = 0;
-    do {
+            for (int e = 0; e < E; ++e) c += __float_as_uint(w[e]) >= mid;
+            c = all<G>(c, Add());
+            const bool enough = c >= top_k;
+            lo = enough ? mid : lo;
+            hi = enough ? hi : mid;
+            count = enough ? c : count;
+            mid = lo + (hi - lo) / 2;
+        }
+        hi = TOP;
+        if (count > G * M) return false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) here += __float_as_uint(w[e]) >= lo;
+    } else {
+        auto halve = [&]() {
+            const unsigned mid = lo + (hi - lo) / 2;
+            float s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += __float_as_uint(w[e]) >= mid ? w[e] : 0.0f;
+            s = all<G>(s, Add());
+            const bool enough = s >= p;
+            lo = enough ? mid : lo;
+            hi = enough ? hi : mid;
+            front = enough ? front : s;
+        };
         halve();
-        here = 0;
+        int round = 0;
+        do {
+            halve();
+            here = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) here += __float_as_uint(w[e]) - lo < hi - lo;
-        count = all<G>(here, Add());
-    } while (count > G * M && ++round < HALVINGS);
-    if (count > G * M) return false;
+            for (int e = 0; e < E; ++e) here += __float_as_uint(w[e]) - lo < hi - lo;
+            count = all<G>(here, Add());
+        } while (count > G * M && ++round < HALVINGS);
+        if (count > G * M) return false;
+    }
     int at = before<G>(here);
 #pragma unroll
     for (int e = 0; e < M; ++e) lds[lane * M + e] = 0.0f;
@@ -222,34 +248,37 @@ __device__ __forceinline__ bool border_by_mass(const float (&w)[E], float top_p,
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
     unsigned s[M];
-    float mine = 0.0f;
 #pragma unroll
-    for (int e = 0; e < M; ++e) {
-        const float v = lds[lane * M + e];
-        s[e] = __float_as_uint(v);
-        mine += v;
-    }
+    for (int e = 0; e < M; ++e) s[e] = __float_as_uint(lds[lane * M + e]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
-    const float end = front + all<G>(mine, Add());
     sort_keys<G, M>(s, lane);
-    mine = 0.0f;
+    keep = by_k ? top_k : G * M;
+    if (by_p) {
+        float ws[M], mine = 0.0f;
 #pragma unroll
-    for (int e = 0; e < M; ++e) mine += __uint_as_float(s[e]);
-    float upto = front + before<G>(mine), nearest = end - p;       // (negative: the list ends too early)
-    int stay = 0;
+        for (int e = 0; e < M; ++e) {
+            ws[e] = lane * M + e < keep ? __uint_as_float(s[e]) : 0.0f;
+            mine += ws[e];
+        }
+        const float listed = all<G>(mine, Add());
+        if (by_k) p = top_p * (total = listed);
+        float upto = front + before<G>(mine), nearest = front + listed - p;       // (negative: the list ends too early)
+        int stay = 0;
 #pragma unroll
-    for (int e = 0; e < M; ++e) {
-        // (the first place of the row always stays)
-        nearest = e > 0 || lane > 0 || front > 0.0f ? fminf(nearest, fabsf(upto - p)) : nearest;
-        stay += upto < p;
-        upto += __uint_as_float(s[e]);
+        for (int e = 0; e < M; ++e) {
+            // (the first place of the row always stays; behind the last one the whole of the list is in front)
+            nearest = e > 0 || lane > 0 || front > 0.0f ? fminf(nearest, fabsf(upto - p)) : nearest;
+            stay += upto < p;
+            upto += ws[e];
+        }
+        sure = sure && nearest > MARGIN * total;
+        keep = max(min(keep, all<G>(stay, Add())), 1);
     }
-    sure = sure && all<G>(nearest, Min()) > margin;
-    keep = max(all<G>(stay, Add()), 1);
     thr = __uint_as_float(at_rank<G, M>(s, keep - 1));
     const float high = band_high(thr), low = band_low(thr);
-    sure = sure && __float_as_uint(low) >= lo && __float_as_uint(high) < hi;       // (else the band is not all in the list)
+    // (a band that is not all in the list)
+    sure = sure && (thr == 0.0f || (__float_as_uint(low) >= lo && (__float_as_uint(high) < hi || hi == TOP)));
 #pragma unroll
     for (int e = 0; e < M; ++e) {
         over += __uint_as_float(s[e]) > high;
@@ -276,7 +305,10 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
         float thr = 0.0f;                       // the weight of the last place that stays
         int keep = 0, over = 0, from = 0;       // of some run of the order around it: places that stay, over the band below, and not under it
         bool found = false;
-        if constexpr (G >= 16) found = by_p && !by_k && border_by_mass<G, E>(w, how.top_p, n, lane, lds, sure, thr, keep, over, from);
+        if constexpr (G >= 16) {
+            if (!by_k || how.top_k <= G * listed_a_lane<G>() / 2)
+                found = border_in_list<G, E>(w, by_k ? how.top_k : 0, how.top_p, n, lane, lds, sure, thr, keep, over, from);
+        }
         if (!found) {
             unsigned s[E];
 #pragma unroll
