@@ -1239,31 +1239,60 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
             wide_key* list = lds[threadIdx.x / G];
 #pragma unroll
             for (int e = 0; e < M; ++e) list[lane * M + e] = 0;
-            unsigned key[E];
-            int held = 0;
+            // the bits between the smallest and the largest logit are halved until the places above are at least m and at most
+            // the list's (first try: what lies far below the largest at this temperature is most likely masked)
+            float least = __builtin_inff();
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                key[e] = key_of(v[e]);
-                held += key[e] > NO_KEY;
+            for (int e = 0; e < E; ++e) least = v[e] > -__builtin_inff() ? fminf(least, v[e]) : least;
+            least = all<G>(least, Min());
+            float lo = least, hi = m, mid = fmaxf(0.5f * lo + 0.5f * hi, m - 16.0f * a.temperature);
+            int count = n;
+            for (int round = 0; count > G * M && round < HALVINGS; ++round) {
+                int c = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) c += v[e] >= mid;
+                c = all<G>(c, Add());
+                const bool enough = c >= a.m;
+                lo = enough ? mid : lo;
+                hi = enough ? hi : mid;
+                count = enough ? c : count;
+                mid = 0.5f * lo + 0.5f * hi;
             }
-            held = all<G>(held, Add());
-            unsigned thr = NO_KEY;
-            int quota = 0;
-            if (a.m < held) kth_largest<G, E>(key, a.m, thr, quota);
-            int over = 0, ties = 0;
+            if (count <= G * M) {
+                int here = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                over += key[e] > thr;
-                ties += key[e] == thr;
-            }
-            // (places over the threshold from the list's start, those at it behind all of them)
-            int at = before<G>(over), tie = before<G>(ties);
-            const int all_over = all<G>(over, Add());
+                for (int e = 0; e < E; ++e) here += v[e] >= lo;
+                int at = before<G>(here);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (key[e] > thr) list[at++] = with_place(key[e], lane * E + e);
-                if (key[e] == thr && tie < quota) list[all_over + tie] = with_place(key[e], lane * E + e);
-                tie += key[e] == thr;
+                for (int e = 0; e < E; ++e)
+                    if (v[e] >= lo) list[at++] = with_place(key_of(v[e]), lane * E + e);
+            } else {
+                unsigned key[E];
+                int held = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    key[e] = key_of(v[e]);
+                    held += key[e] > NO_KEY;
+                }
+                held = all<G>(held, Add());
+                unsigned thr = NO_KEY;
+                int quota = 0;
+                if (a.m < held) kth_largest<G, E>(key, a.m, thr, quota);
+                int over = 0, ties = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    over += key[e] > thr;
+                    ties += key[e] == thr;
+                }
+                // (places over the threshold from the list's start, those at it behind all of them)
+                int at = before<G>(over), tie = before<G>(ties);
+                const int all_over = all<G>(over, Add());
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (key[e] > thr) list[at++] = with_place(key[e], lane * E + e);
+                    if (key[e] == thr && tie < quota) list[all_over + tie] = with_place(key[e], lane * E + e);
+                    tie += key[e] == thr;
+                }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
             __builtin_amdgcn_wave_barrier();
@@ -1405,18 +1434,20 @@ template <typename T> int top_rows(hipStream_t s, const T* x, TopArgs a) {
         hipLaunchKernelGGL((k_top<T, 4, 4, 0>), blocks(4), dim3(256), 0, s, x, a);
     } else if (a.width <= 64) {
         a.vec = vec(8);
-        hipLaunchKernelGGL((k_top<T, 8, 8, 0>), blocks(8), dim3(256), 0, s, x, a);
+        if (a.m <= 16) hipLaunchKernelGGL((k_top<T, 8, 8, 4>), blocks(8), dim3(256), 0, s, x, a);
+        else hipLaunchKernelGGL((k_top<T, 8, 8, 0>), blocks(8), dim3(256), 0, s, x, a);
     } else if (a.width <= 256) {
         a.vec = vec(16);
-        if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 16, 16, 4>), blocks(16), dim3(256), 0, s, x, a);
+        if (a.m <= 32) hipLaunchKernelGGL((k_top<T, 16, 16, 4>), blocks(16), dim3(256), 0, s, x, a);
+        else if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 16, 16, 8>), blocks(16), dim3(256), 0, s, x, a);
         else hipLaunchKernelGGL((k_top<T, 16, 16, 16>), blocks(16), dim3(256), 0, s, x, a);
     } else if (a.width <= 512) {
         a.vec = vec(8);
-        if (a.m <= 128) hipLaunchKernelGGL((k_top<T, 64, 8, 2>), blocks(64), dim3(256), 0, s, x, a);
+        if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 64, 8, 2>), blocks(64), dim3(256), 0, s, x, a);
         else hipLaunchKernelGGL((k_top<T, 64, 8, 4>), blocks(64), dim3(256), 0, s, x, a);
     } else if (a.width <= NARROW) {
         a.vec = vec(16);
-        if (a.m <= 128) hipLaunchKernelGGL((k_top<T, 64, 16, 2>), blocks(64), dim3(256), 0, s, x, a);
+        if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 64, 16, 2>), blocks(64), dim3(256), 0, s, x, a);
         else hipLaunchKernelGGL((k_top<T, 64, 16, 4>), blocks(64), dim3(256), 0, s, x, a);
     } else {
         hipLaunchKernelGGL(k_top_wide<T>, dim3((unsigned)a.rows), dim3(WIDE_T), 0, s, x, a);
