@@ -1184,7 +1184,8 @@ struct TopArgs {
 // picked out first and those sorted, M places a lane.
 template <typename T, int G, int E, int M>
 __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a) {
-    constexpr bool PACKED = std::is_same<T, __hip_bfloat16>::value, WHOLE = PACKED || M == 0;
+    constexpr int TRIES = 5;
+    constexpr bool WHOLE = M == 0, PACKED = WHOLE && std::is_same<T, __hip_bfloat16>::value;
     __shared__ wide_key lds[WHOLE ? 1 : 256 / G][WHOLE ? 1 : G * (M ? M : 1)];
     const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
     if (r >= a.rows) return;
@@ -1239,27 +1240,48 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
             wide_key* list = lds[threadIdx.x / G];
 #pragma unroll
             for (int e = 0; e < M; ++e) list[lane * M + e] = 0;
-            // the bits between the smallest and the largest logit are halved until the places above are at least m and at most
-            // the list's (first try: what lies far below the largest at this temperature is most likely masked)
+            // What lies between the smallest and the largest logit is halved until the places from lo on are at least m and at
+            // most the list's (the first try: what lies far below the largest at this temperature is most likely masked).  A few
+            // tries on the next value below hi is looked at itself: if there are enough of it, the first by place do.
             float least = __builtin_inff();
 #pragma unroll
             for (int e = 0; e < E; ++e) least = v[e] > -__builtin_inff() ? fminf(least, v[e]) : least;
             least = all<G>(least, Min());
-            float lo = least, hi = m, mid = fmaxf(0.5f * lo + 0.5f * hi, m - 16.0f * a.temperature);
-            int count = n;
-            for (int round = 0; count > G * M && round < HALVINGS; ++round) {
+            float lo = least, hi = m, mid = fmaxf(0.5f * lo + 0.5f * m, m - 16.0f * a.temperature);
+            bool all_below = true;                        // (no hi yet that places are left out from)
+            int count = n, over = 0, quota = G * E;       // places from lo on; from hi on (fewer than m); of those at lo that go on the list
+            for (int round = 0; count > G * M; ++round) {
                 int c = 0;
+                const bool look = round >= TRIES && (round & 1);
+                if (!look) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) c += v[e] >= mid;
+                    for (int e = 0; e < E; ++e) c += v[e] >= mid;
+                } else {
+                    mid = -__builtin_inff();
+#pragma unroll
+                    for (int e = 0; e < E; ++e) mid = all_below | (v[e] < hi) ? fmaxf(mid, v[e]) : mid;
+                    mid = all<G>(mid, Max());
+#pragma unroll
+                    for (int e = 0; e < E; ++e) c += v[e] >= mid;
+                }
                 c = all<G>(c, Add());
-                const bool enough = c >= a.m;
-                lo = enough ? mid : lo;
-                hi = enough ? hi : mid;
-                count = enough ? c : count;
+                if (c >= a.m) {
+                    lo = mid;
+                    count = c;
+                    if (look) {
+                        quota = a.m - over;
+                        break;
+                    }
+                } else {
+                    hi = mid;
+                    over = c;
+                    all_below = false;
+                    if (!(mid > least)) break;            // (all that is held is fewer than m)
+                }
                 mid = 0.5f * lo + 0.5f * hi;
             }
-            if (count <= G * M) {
-                int here = 0;
+            int here = 0;
+            if (quota == G * E) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) here += v[e] >= lo;
                 int at = before<G>(here);
@@ -1267,31 +1289,17 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
                 for (int e = 0; e < E; ++e)
                     if (v[e] >= lo) list[at++] = with_place(key_of(v[e]), lane * E + e);
             } else {
-                unsigned key[E];
-                int held = 0;
+                int ties = 0;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    key[e] = key_of(v[e]);
-                    held += key[e] > NO_KEY;
+                    here += v[e] > lo;
+                    ties += v[e] == lo;
                 }
-                held = all<G>(held, Add());
-                unsigned thr = NO_KEY;
-                int quota = 0;
-                if (a.m < held) kth_largest<G, E>(key, a.m, thr, quota);
-                int over = 0, ties = 0;
+                int at = before<G>(here), tie = before<G>(ties);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    over += key[e] > thr;
-                    ties += key[e] == thr;
-                }
-                // (places over the threshold from the list's start, those at it behind all of them)
-                int at = before<G>(over), tie = before<G>(ties);
-                const int all_over = all<G>(over, Add());
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (key[e] > thr) list[at++] = with_place(key[e], lane * E + e);
-                    if (key[e] == thr && tie < quota) list[all_over + tie] = with_place(key[e], lane * E + e);
-                    tie += key[e] == thr;
+                    if (v[e] > lo) list[at++] = with_place(key_of(v[e]), lane * E + e);
+                    if (v[e] == lo && tie++ < quota) list[over + tie - 1] = with_place(key_of(v[e]), lane * E + e);
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
@@ -1429,26 +1437,37 @@ template <typename T> int top_rows(hipStream_t s, const T* x, TopArgs a) {
         return (int)(reinterpret_cast<uintptr_t>(x) % align == 0 && (a.ld * sizeof(T)) % align == 0);
     };
     auto blocks = [&](int g) { return dim3((unsigned)((a.rows * g + 255) / 256)); };
+    constexpr bool PACKED = std::is_same<T, __hip_bfloat16>::value;
+    // Lists of G M places, the smallest that leave room over m (a list of exactly m needs its border exactly: 50k x 512, m 64,
+    // 113 us on one place a lane, 60 on two; m 48: 54 and 60), and the whole row where that is as fast: 64 places from m = 17 on
+    // (m 32: 24 us whole, 28 on four a lane), 32-bit keys from m = 65 on (100k x 256, m 200: 184 us packed, 240 listed).
+#define LAUNCH_TOP(G, E, M) hipLaunchKernelGGL((k_top<T, G, E, M>), blocks(G), dim3(256), 0, s, x, a)
     if (a.width <= 16) {
         a.vec = vec(4);
-        hipLaunchKernelGGL((k_top<T, 4, 4, 0>), blocks(4), dim3(256), 0, s, x, a);
+        LAUNCH_TOP(4, 4, 0);
     } else if (a.width <= 64) {
         a.vec = vec(8);
-        if (a.m <= 16) hipLaunchKernelGGL((k_top<T, 8, 8, 4>), blocks(8), dim3(256), 0, s, x, a);
-        else hipLaunchKernelGGL((k_top<T, 8, 8, 0>), blocks(8), dim3(256), 0, s, x, a);
+        if constexpr (PACKED) LAUNCH_TOP(8, 8, 0);
+        else if (a.m > 16) LAUNCH_TOP(8, 8, 0);
+        else if (a.m > 8) LAUNCH_TOP(8, 8, 4);
+        else LAUNCH_TOP(8, 8, 2);
     } else if (a.width <= 256) {
         a.vec = vec(16);
-        if (a.m <= 32) hipLaunchKernelGGL((k_top<T, 16, 16, 4>), blocks(16), dim3(256), 0, s, x, a);
-        else if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 16, 16, 8>), blocks(16), dim3(256), 0, s, x, a);
-        else hipLaunchKernelGGL((k_top<T, 16, 16, 16>), blocks(16), dim3(256), 0, s, x, a);
+        if (a.m > (PACKED ? 64 : 128)) LAUNCH_TOP(16, 16, 0);
+        else if (a.m > 32) LAUNCH_TOP(16, 16, 8);
+        else if (a.m > 16) LAUNCH_TOP(16, 16, 4);
+        else LAUNCH_TOP(16, 16, 2);
     } else if (a.width <= 512) {
         a.vec = vec(8);
-        if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 64, 8, 2>), blocks(64), dim3(256), 0, s, x, a);
-        else hipLaunchKernelGGL((k_top<T, 64, 8, 4>), blocks(64), dim3(256), 0, s, x, a);
+        if (a.m <= 48) LAUNCH_TOP(64, 8, 1);
+        else if (a.m > (PACKED ? 64 : 96)) LAUNCH_TOP(64, 8, PACKED ? 0 : 4);
+        else LAUNCH_TOP(64, 8, 2);
     } else if (a.width <= NARROW) {
         a.vec = vec(16);
-        if (a.m <= 64) hipLaunchKernelGGL((k_top<T, 64, 16, 2>), blocks(64), dim3(256), 0, s, x, a);
-        else hipLaunchKernelGGL((k_top<T, 64, 16, 4>), blocks(64), dim3(256), 0, s, x, a);
+        if (a.m <= 48) LAUNCH_TOP(64, 16, 1);
+        else if (a.m > (PACKED ? 64 : 96)) LAUNCH_TOP(64, 16, PACKED ? 0 : 4);
+        else LAUNCH_TOP(64, 16, 2);
+#undef LAUNCH_TOP
     } else {
         hipLaunchKernelGGL(k_top_wide<T>, dim3((unsigned)a.rows), dim3(WIDE_T), 0, s, x, a);
     }

@@ -154,6 +154,30 @@ def test_sample_decisions_on_a_border(width):
     check_sample(x, u, top_k=width // 2, top_p=0.5, min_p=1.0)
 
 
+@pytest.mark.parametrize("width", [20, 64, 65, 200, 256, 500, 512, 777, 1024])
+def test_sample_borders_among_places_that_do_not_part(width):
+    """Equal logits, logits a last bit apart, masks of the lowest value, places of no weight, one place with all of it."""
+    x = make_logits(12, width, F32, seed=width)
+    x[0] = 2.5
+    x[1] = torch.where(torch.rand(width, generator=rng(1)) < 0.5, 2.0, 1.0)
+    x[2] = 3.0 + torch.arange(width) * 2.0 ** -22
+    x[3, 5:] = torch.finfo(F32).min
+    x[4, 3:] = -math.inf
+    x[5, 0] = 60.0
+    x[6] = torch.randint(0, 4, (width,), generator=rng(2)).float()
+    x[7] = -20.0
+    x[7, -1] = 0.0
+    x[8] = torch.linspace(0.0, -30.0, width)
+    x[9] = torch.where(torch.rand(width, generator=rng(3)) < 0.7, -math.inf, 1.0)
+    x[10] = 1e-7 * x[10]
+    x[11, : width // 2] = x[11].max()
+    u = torch.rand(12, 3, generator=rng(4))
+    for k in (0, 1, 7, 16, 32, 33, 64, 65, 130):
+        for p in (1.0, 0.0, 0.3, 0.9, 0.999, 1.0 - 2.0 ** -20):
+            if k or p < 1:
+                check_sample(x, u, top_k=k, top_p=p, temperature=0.9)
+
+
 @pytest.mark.parametrize("width", [1500, 8200, 40000])
 @pytest.mark.parametrize("ties", [False, True])
 def test_sample_wide_rows_every_way(width, ties):
@@ -222,6 +246,36 @@ def test_top(width):
             else:      # 32 bits: sums of up to width/1024 numbers a thread and a tree over them, an exponential and a log
                 y = np.abs(xs[r, :n][np.isfinite(xs[r, :n])] / t).max()
                 assert abs(g - lse) <= 2.0 ** -24 * (4 * min(y, abs(lse) + 200) + 4 * abs(lse) + 64 + width / 1024), (g, lse)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [16, 33, 64, 130, 256, 400, 512, 900, 1024])
+def test_top_of_rows_whose_places_do_not_part(width, dtype):
+    """Equal and infinite logits, masks of the lowest value, fewer places than are asked for, for every length of the list."""
+    inf = float("inf")
+    x = make_logits(12, width, F32, seed=width)
+    x[0] = 2.5
+    x[1] = inf
+    x[2, ::2] = inf
+    x[3, 5:] = torch.finfo(dtype).min
+    x[4, 3:] = -inf
+    x[5] = torch.randint(0, 2, (width,), generator=rng(1)).float()
+    x[6] = -inf
+    x[7, : width // 2] = x[7].max()
+    x[8] = torch.where(torch.rand(width, generator=rng(2)) < 0.5, -inf, 1.0)
+    x[9, 1:] = 1e-3 * x[9, 1:]
+    x[9, 0] = 1e6
+    x[10] = torch.linspace(1.0, 1.0 + 2.0 ** -20, width)
+    x[11] = torch.finfo(dtype).min
+    x = x.to(dtype)
+    y = x.float().numpy().astype(np.float64)
+    for m in (1, 5, 8, 9, 16, 17, 32, 33, 48, 49, 64, 65, 96, 97, 128, 129, 200, 256):
+        top = L.top_rows(x.to(DEV), m, temperature=1.0)
+        values, index = top.values.cpu().numpy(), top.index.cpu().numpy()
+        for r in range(12):
+            v, i, _ = top_row(y[r], m, 1.0)
+            assert np.array_equal(index[r], i), (m, r)
+            assert np.array_equal(values[r].astype(np.float64), v), (m, r)
 
 
 def make_teacher(x, m, t, seed, counts, tail):
