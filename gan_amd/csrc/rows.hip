@@ -18,7 +18,8 @@ struct RowSettings {
     int top_k;
     __device__ __forceinline__ RowSettings(const Settings& s, long long r)
         : temperature(s.temperature_rows ? s.temperature_rows[r] : s.temperature), top_p(s.top_p_rows ? s.top_p_rows[r] : s.top_p),
-          min_p(s.min_p_rows ? s.min_p_rows[r] : s.min_p), per(s.temperature_rows ? (float)(LOG2E / (double)temperature) : s.per), top_k(s.top_k_rows ? s.top_k_rows[r] : s.top_k) {}
+          min_p(s.min_p_rows ? s.min_p_rows[r] : s.min_p), per(s.temperature_rows ? (float)(LOG2E / (double)temperature) : s.per),
+          top_k(s.top_k_rows ? s.top_k_rows[r] : s.top_k) {}
     // the smallest weight that min-p and the unit leave
     __device__ __forceinline__ double floor() const { return min_p > 0.0f ? fmax((double)fminf(min_p, 1.0f) * UNIT, 1.0) : 1.0; }
     // the mass that top-p keeps of `total`: a place stays while the mass in front of it is below this; the first always does
@@ -458,7 +459,10 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
     return true;
 }
 
-// A group of G lanes per row, the row in registers.
+// A group of G lanes per row, the row in registers: read once, 8 bytes a draw written.  Bound by the issue of vector
+// instructions, not by memory: 100,000 x 64 under top-k 32, top-p 0.9 and min-p (sorted whole: 300 of 878 instructions a wave)
+// 22.7 us, of which 18 are issue; 27 MB would be copied in 6.  Without filters 8.8 us.  152,896 x 256 under top-p 0.9 63 us,
+// 59 of them issue of 952 instructions a wave (157 MB: 35).  One row 4.7 us: a chain of lane exchanges.
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleRows a) {
     __shared__ __attribute__((aligned(16))) float lds[E > 4 ? 256 / G : 1][E > 4 ? G * E : 1];
@@ -919,6 +923,10 @@ __device__ __forceinline__ void list_with_ties(const Span<T>& row, const Parts<T
 //   otherwise: top-p's border from a histogram of the weights over BINS steps of the logit (from the row's smallest, or the
 //   smallest that has a weight), the places of its bin in a list, or counted where they are thousands of one value;
 //   then the sum of what stays in each part of the row, and for each draw a look through the one part that holds it.
+// Rows are as many as a batch has requests, so most CUs idle; what a row costs is its CU's time: 48 x 50,001 bf16 under top-k
+// and top-p 17.6 us (two reads of 100 KB, then sorts of a hundred places by one wave); under top-p alone 46 us, two f64
+// exponentials a place, and 75 us for 512 rows of 32,001 (two a CU); top-k beyond LIST_K over 131,072 places 700 us
+// (general_draws).
 constexpr int BINS = 4096;
 constexpr float OCTAVES = 37.0f;          // a weight under 2^-37 is 0
 
@@ -1180,8 +1188,10 @@ struct TopArgs {
     __device__ __forceinline__ int count(long long r) const { return counts ? min(max(counts[r], 0), width) : width; }
 };
 
-// The group's row sorted, whole (rows to 64 places; any row of bf16, whose key and place share 32 bits), or the m largest
-// picked out first and those sorted, M places a lane.
+// The group's row sorted with its places, whole (M = 0; bf16's key and place share 32 bits), or a list of G M places that holds
+// the m largest picked out first and sorted alone.  Bound by the issue of vector instructions: 100,000 x 64, m 16, 18 us, 15 of
+// them issue of 726 instructions a wave (39 MB read and written: 9 us at the rate of a copy); sorted whole 23 us, with the
+// m-th largest found bit by bit 28.
 template <typename T, int G, int E, int M>
 __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a) {
     constexpr int TRIES = 5;
@@ -1315,7 +1325,8 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
     }
 }
 
-// A workgroup per row: the places that can be among the m largest are picked out into a list and ranked there.
+// A workgroup per row: the places that can be among the m largest are picked out into a list and ranked there.  96 x 32,771
+// IEEE halfs, m 64: 11 us, two reads of a row by one CU and a sort by one of its waves; the 6.3 MB themselves would take 1.4.
 template <typename T>
 __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, TopArgs a) {
     __shared__ double hist[256], found[2], red[WIDE_T / 64 + 1];
