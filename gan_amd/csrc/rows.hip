@@ -925,8 +925,8 @@ __device__ __forceinline__ void list_with_ties(const Span<T>& row, const Parts<T
 //   then the sum of what stays in each part of the row, and for each draw a look through the one part that holds it.
 // Rows are as many as a batch has requests, so most CUs idle; what a row costs is its CU's time: 48 x 50,001 bf16 under top-k
 // and top-p 17.6 us (two reads of 100 KB, then sorts of a hundred places by one wave); under top-p alone 46 us, two f64
-// exponentials a place, and 75 us for 512 rows of 32,001 (two a CU); top-k beyond LIST_K over 131,072 places 700 us
-// (general_draws).
+// exponentials a place, and 75 us for 512 rows of 32,001 (two a CU); 150 rows of 131,072 under a top-k
+// beyond LIST_K 700 us (general_draws).
 constexpr int BINS = 4096;
 constexpr float OCTAVES = 37.0f;          // a weight under 2^-37 is 0
 
@@ -1190,8 +1190,7 @@ struct TopArgs {
 
 // The group's row sorted with its places, whole (M = 0; bf16's key and place share 32 bits), or a list of G M places that holds
 // the m largest picked out first and sorted alone.  Bound by the issue of vector instructions: 100,000 x 64, m 16, 18 us, 15 of
-// them issue of 726 instructions a wave (39 MB read and written: 9 us at the rate of a copy); sorted whole 23 us, with the
-// m-th largest found bit by bit 28.
+// them issue of 726 instructions a wave (39 MB read and written: 9 us at the rate of a copy); sorted whole 23 us.
 template <typename T, int G, int E, int M>
 __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a) {
     constexpr int TRIES = 5;
