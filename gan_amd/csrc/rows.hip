@@ -735,18 +735,23 @@ struct List {
         const int at = atomicAdd(&count, 1);
         if (at < LIST) key[at] = with_place(k, i);
     }
+    template <int E> __device__ __forceinline__ void sort_by_wave(int n) {
+        wide_key k[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) k[e] = (int)threadIdx.x * E + e < n ? key[threadIdx.x * E + e] : 0ull;
+        sort_keys<64, E>(k, threadIdx.x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sorted[threadIdx.x * E + e] = k[e];
+    }
     // key[0 .. n) into sorted[0 .. n), largest first.  All keys differ.  A wave sorts up to 256 of them; of more, every thread
     // counts the keys in front of its own.
     __device__ __forceinline__ void sort(int n) {
         __syncthreads();
         if (n <= 256) {
             if (threadIdx.x < 64) {
-                wide_key k[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) k[e] = (int)threadIdx.x * 4 + e < n ? key[threadIdx.x * 4 + e] : 0ull;
-                sort_keys<64, 4>(k, threadIdx.x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sorted[threadIdx.x * 4 + e] = k[e];
+                if (n <= 64) sort_by_wave<1>(n);
+                else if (n <= 128) sort_by_wave<2>(n);
+                else sort_by_wave<4>(n);
             }
         } else if ((int)threadIdx.x < n) {
             const wide_key mine = key[threadIdx.x];
