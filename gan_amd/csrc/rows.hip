@@ -726,7 +726,7 @@ __device__ __forceinline__ void general_draws(const T* __restrict__ x, const Sam
 __device__ __forceinline__ wide_key with_place(unsigned key, int place) { return (wide_key)key << 32 | (unsigned)~place; }
 
 // Places picked out of a row, in LDS.
-constexpr int LIST = 1024, LIST_K = 512;
+constexpr int LIST = 1024, LIST_K = 512;       // (a place a thread)
 struct List {
     wide_key key[LIST], sorted[LIST];
     double q[LIST];
@@ -735,34 +735,48 @@ struct List {
         const int at = atomicAdd(&count, 1);
         if (at < LIST) key[at] = with_place(k, i);
     }
-    template <int E> __device__ __forceinline__ void sort_by_wave(int n) {
-        wide_key k[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) k[e] = (int)threadIdx.x * E + e < n ? key[threadIdx.x * E + e] : 0ull;
-        sort_keys<64, E>(k, threadIdx.x);
-#pragma unroll
-        for (int e = 0; e < E; ++e) sorted[threadIdx.x * E + e] = k[e];
-    }
-    // key[0 .. n) into sorted[0 .. n), largest first.  All keys differ.  A wave sorts up to 256 of them; of more, every thread
-    // counts the keys in front of its own.
+    // key[0 .. n) into sorted[0 .. n), largest first.  All keys differ.  Each wave sorts 64 of them; a key's rank is then its own in
+    // there and, by a binary search each, that among the 64 of every other wave.
     __device__ __forceinline__ void sort(int n) {
+        const int t = threadIdx.x, wave = t >> 6;
         __syncthreads();
-        if (n <= 256) {
-            if (threadIdx.x < 64) {
-                if (n <= 64) sort_by_wave<1>(n);
-                else if (n <= 128) sort_by_wave<2>(n);
-                else sort_by_wave<4>(n);
-            }
-        } else if ((int)threadIdx.x < n) {
-            const wide_key mine = key[threadIdx.x];
-            int front = 0;
-#pragma unroll 8
-            for (int j = 0; j < n; ++j) front += key[j] > mine;
-            sorted[front] = mine;
+        wide_key mine[1] = {0ull};
+        if (wave * 64 < n) {
+            if (t < n) mine[0] = key[t];
+            sort_keys<64, 1>(mine, t & 63);
+            if (n > 64) key[t] = mine[0];
         }
+        int rank = t & 63;
+        if (n > 64) {
+            __syncthreads();
+            if (wave * 64 < n) {
+                for (int c = 0; c * 64 < n; ++c) {
+                    if (c == wave) continue;
+                    const wide_key* other = key + c * 64;
+                    int front = 0;
+#pragma unroll
+                    for (int step = 32; step; step >>= 1) front += other[front + step - 1] > mine[0] ? step : 0;
+                    rank += front + (other[front] > mine[0]);
+                }
+            }
+        }
+        if (t < n) sorted[rank] = mine[0];
         __syncthreads();
     }
 };
+
+// the k-th largest of 64 E keys, each the largest of 16 / E threads
+template <int E> __device__ __forceinline__ unsigned kth_of_groups(const unsigned* keys, int k) {
+    unsigned v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        v[e] = 0;
+#pragma unroll
+        for (int j = 0; j < 16 / E; ++j) v[e] = max(v[e], keys[(e * (16 / E) + j) * 64 + threadIdx.x]);
+    }
+    sort_keys<64, E>(v, threadIdx.x);
+    return at_rank<64, E>(v, k - 1);
+}
 
 // A key that at least k of the row's places reach, few more do: the k-th largest of the threads' own largest (mine: this
 // thread's).  NO_KEY + 1 where fewer than k threads hold a place.
@@ -770,17 +784,14 @@ __device__ __forceinline__ unsigned bound_of_top(unsigned mine, int k, unsigned*
     keys[threadIdx.x] = mine;
     __syncthreads();
     if (threadIdx.x < 64) {
-        if (k <= 128) {          // (the largest of each four: few more places reach their k-th, and 256 keys sort quickly)
-            unsigned v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[e] = max(v[e], keys[(e * 4 + j) * 64 + threadIdx.x]);
-            }
-            sort_keys<64, 4>(v, threadIdx.x);
-            const unsigned thr = max(at_rank<64, 4>(v, k - 1), NO_KEY + 1);
-            if (threadIdx.x == 0) *result = thr;
+        // (the largest of several threads: fewer keys sort quicker, and few more places reach their k-th)
+        unsigned thr;
+        if (k <= 32) {
+            thr = kth_of_groups<1>(keys, k);
+        } else if (k <= 64) {
+            thr = kth_of_groups<2>(keys, k);
+        } else if (k <= 128) {
+            thr = kth_of_groups<4>(keys, k);
         } else {
             unsigned v[16];
             int held = 0;
@@ -789,14 +800,14 @@ __device__ __forceinline__ unsigned bound_of_top(unsigned mine, int k, unsigned*
                 v[e] = keys[e * 64 + threadIdx.x];
                 held += v[e] > NO_KEY;
             }
-            unsigned thr = NO_KEY + 1;
+            thr = NO_KEY + 1;
             if (k < all<64>(held, Add())) {
                 int quota;
                 kth_largest<64, 16>(v, k, thr, quota);
                 thr += quota == 0;
             }
-            if (threadIdx.x == 0) *result = thr;
         }
+        if (threadIdx.x == 0) *result = max(thr, NO_KEY + 1);
     }
     __syncthreads();
     return *result;
