@@ -229,31 +229,6 @@ __device__ __forceinline__ void load_values(const T* __restrict__ row, int n, in
     }
 }
 
-// The k largest of a group's keys, ties by place: those with key > thr, and of those with key == thr the first `quota`.
-// 0 < k < number of places that hold something.  The threshold is found a bit at a time.
-template <int G, int E>
-__device__ __forceinline__ void kth_largest(const unsigned (&key)[E], int k, unsigned& thr, int& quota) {
-    unsigned t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned c = t | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) n += key[e] >= c;
-        n = all<G>(n, Add());
-        if (n >= k) t = c;
-        if (n == k) {
-            thr = c - 1;
-            quota = 0;
-            return;
-        }
-    }
-    int n = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) n += key[e] > t;
-    thr = t;
-    quota = k - all<G>(n, Add());
-}
-
 // The keys of a group in descending order by place (lane 0's first is the largest): a bitonic network.  Blocks that sort the
 // other way hold their keys complemented, so that every exchange puts the larger key first; an exchange between lanes is a
 // lane permutation and a median with 0 or the largest key (that is: the larger, or the smaller).

@@ -793,19 +793,33 @@ __device__ __forceinline__ unsigned bound_of_top(unsigned mine, int k, unsigned*
         } else if (k <= 128) {
             thr = kth_of_groups<4>(keys, k);
         } else {
-            unsigned v[16];
-            int held = 0;
+            // halvings between the smallest and the largest until few more than k of the threads' are over
+            float v[16], least = __builtin_inff(), most = -__builtin_inff();
+            int count = 0;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                v[e] = keys[e * 64 + threadIdx.x];
-                held += v[e] > NO_KEY;
+                v[e] = value_of(keys[e * 64 + threadIdx.x]);
+                const bool held = v[e] > -__builtin_inff();
+                count += held;
+                least = held ? fminf(least, v[e]) : least;
+                most = fmaxf(most, v[e]);
             }
-            thr = NO_KEY + 1;
-            if (k < all<64>(held, Add())) {
-                int quota;
-                kth_largest<64, 16>(v, k, thr, quota);
-                thr += quota == 0;
+            count = all<64>(count, Add());
+            float lo = all<64>(least, Min()), hi = all<64>(most, Max());
+            for (int round = 0; count > k + k / 8 && round < HALVINGS; ++round) {
+                const float mid = 0.5f * lo + 0.5f * hi;
+                int c = 0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) c += v[e] >= mid;
+                c = all<64>(c, Add());
+                lo = c >= k ? mid : lo;
+                hi = c >= k ? hi : mid;
+                count = c >= k ? c : count;
             }
+            least = __builtin_inff();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) least = v[e] >= lo ? fminf(least, v[e]) : least;
+            thr = count < k ? 0u : key_of(all<64>(least, Min()));
         }
         if (threadIdx.x == 0) *result = max(thr, NO_KEY + 1);
     }
