@@ -954,8 +954,8 @@ __device__ __forceinline__ void list_with_ties(const Span<T>& row, const Parts<T
 //   smallest that has a weight), the places of its bin in a list, or counted where they are thousands of one value;
 //   then the sum of what stays in each part of the row, and for each draw a look through the one part that holds it.
 // Rows are as many as a batch has requests, so most CUs idle; what a row costs is its CU's time: 48 x 50,001 bf16 under top-k
-// and top-p 17.6 us (two reads of 100 KB, then sorts of a hundred places by one wave); under top-p alone 46 us, two f64
-// exponentials a place, and 75 us for 512 rows of 32,001 (two a CU); 150 rows of 131,072 under a top-k
+// 50 and top-p 15 us (two reads of 100 KB, two lists sorted), top-k 500 27 us; under top-p alone 45 us, two f64
+// exponentials a place, and 69 us for 512 rows of 32,001 (two a CU); 150 rows of 131,072 under a top-k
 // beyond LIST_K 700 us (general_draws).
 constexpr int BINS = 4096;
 constexpr float OCTAVES = 37.0f;          // a weight under 2^-37 is 0
@@ -1355,7 +1355,7 @@ __global__ __launch_bounds__(256) void k_top(const T* __restrict__ x, TopArgs a)
 }
 
 // A workgroup per row: the places that can be among the m largest are picked out into a list and ranked there.  96 x 32,771
-// IEEE halfs, m 64: 11 us, two reads of a row by one CU and a sort by one of its waves; the 6.3 MB themselves would take 1.4.
+// IEEE halfs, m 64: 9.8 us, two reads of a row by one CU and a sort of some eighty places; the 6.3 MB themselves would take 1.4.
 template <typename T>
 __global__ __launch_bounds__(WIDE_T) void k_top_wide(const T* __restrict__ x, TopArgs a) {
     __shared__ double hist[256], found[2], red[WIDE_T / 64 + 1];
