@@ -205,15 +205,34 @@ template <typename V, typename OP> __device__ __forceinline__ V block_all(V v, O
     return t;
 }
 
+// two sums over the workgroup at once
+__device__ __forceinline__ void block_sums(double& a, double& b, double* red) {
+    a = all<64>(a, Add());
+    b = all<64>(b, Add());
+    __syncthreads();
+    if (lane_id() == 0) {
+        red[threadIdx.x >> 6] = a;
+        red[WIDE_T / 64 + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+    a = red[0];
+    b = red[WIDE_T / 64];
+#pragma unroll
+    for (int w = 1; w < WIDE_T / 64; ++w) {
+        a += red[w];
+        b += red[WIDE_T / 64 + w];
+    }
+}
+
 // One pass over the row for the largest place, the sum of exponentials and that of the places that are not listed (each
 // thread beside its own largest so far), a second one for the gradient.  Listed places are a bitmap in LDS, shifted so that a
 // vector's bits are one byte of it (f32: half a byte).  512 x 32,001 bf16, two rows a CU: loss 17.3 us (33 MB, 1.9 TB/s), its
-// gradient from the sums that the loss left 27 us (66 MB, 2.4 TB/s): a row's reductions over sixteen waves, ten barriers, stand
+// gradient from the sums that the loss left 27 us (66 MB, 2.4 TB/s): a row's reductions over sixteen waves, nine barriers, stand
 // between its passes, and two workgroups a CU hide them in part.
 template <typename T, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x, T* __restrict__ grad, DistillArgs a) {
     constexpr int PER = Span<T>::PER;
-    __shared__ double red[WIDE_T / 64];
+    __shared__ double red[2 * (WIDE_T / 64)];
     __shared__ unsigned bits[MAX_WIDTH / 32 + 1];
     __shared__ int place[AIG_ROWS_MAX_TOP];
     __shared__ float prob[AIG_ROWS_MAX_TOP];
@@ -237,7 +256,9 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
             v_mine = v;
         }
     }
-    const int named = block_all((int)(i_mine >= 0), Add(), red);
+    typename Span<T>::Batch ahead{};
+    if (LOSS) ahead = row.fetch(t, WIDE_T);       // (on its way under the entries' sums; a gradient alone has no pass to read it for)
+    __syncthreads();
     if (i_mine >= 0) atomicOr(&bits[(i_mine + pad) >> 5], 1u << ((i_mine + pad) & 31));
     double lse;
     if (a.lse) {
@@ -248,12 +269,12 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
     }
     const double lq = (double)v_mine * a.per - lse;
     const float q = i_mine >= 0 ? probability(lq) : 0.0f;
-    const double sum_q = block_all((double)q, Add(), red);
     if (GRAD && t < AIG_ROWS_MAX_TOP) {
         place[t] = i_mine;
         prob[t] = q;
     }
-    __syncthreads();
+    double sum_q = (double)q, named = i_mine >= 0 ? 1.0 : 0.0;
+    block_sums(sum_q, named, red);        // (its barriers are also those between the bitmap's writers and its readers)
 
     float top, rest_top;
     double z, rest;
@@ -267,7 +288,7 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
     } else {
         float mine = -__builtin_inff();
         z = rest = 0.0;
-        row.each(t, WIDE_T, [&](int i, const float (&v)[PER], int count) {
+        row.each(t, WIDE_T, LOSS ? ahead : row.fetch(t, WIDE_T), [&](int i, const float (&v)[PER], int count) {
             float here = v[0];
             for (int j = 1; j < PER; ++j) here = j < count ? fmaxf(here, v[j]) : here;
             if (here > mine) {
@@ -290,8 +311,9 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
         });
         top = block_all(mine, Max(), red);
         const float shrink = mine > -__builtin_inff() ? exp2_fast((mine - top) * per) : 1.0f;      // (1: keeps a NaN)
-        z = block_all(z * (double)shrink, Add(), red);
-        rest = block_all(rest * (double)shrink, Add(), red);
+        z *= (double)shrink;
+        rest *= (double)shrink;
+        block_sums(z, rest, red);
         rest_top = top;
         if (a.lse && rest < FAINT) {
             float u = -__builtin_inff();
@@ -311,7 +333,7 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
         }
     }
     const float base = top > -__builtin_inff() ? top : 0.0f;
-    const bool live = z != 0.0 && named > 0;
+    const bool live = z != 0.0 && named > 0.0;
     const float rest_q = a.lse && rest_top > -__builtin_inff() ? (float)fmax(1.0 - sum_q, 0.0) : 0.0f;
     const bool faint = rest_q > 0.0f && rest_top != top;
     if (LOSS) {

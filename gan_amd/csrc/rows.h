@@ -330,23 +330,34 @@ template <typename T> struct Span {
         head = min((int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T), n);
         vecs = (n - head) / PER;
     }
-    template <typename F> __device__ __forceinline__ void each(int first, int step, F f) const {
+    // four vectors on their way at a time: one CU's share of memory is latency
+    struct Batch { uint4 w[4]; };
+    __device__ __forceinline__ Batch fetch(int k0, int step) const {
+        Batch u{};
+        if (k0 < vecs) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) u.w[b] = reinterpret_cast<const uint4*>(x + head)[min(k0 + b * step, vecs - 1)];
+        }
+        return u;
+    }
+    template <typename F> __device__ __forceinline__ void each(int first, int step, F f) const { each(first, step, fetch(first, step), f); }
+    // (with the first vectors on their way already)
+    template <typename F> __device__ __forceinline__ void each(int first, int step, Batch ahead, F f) const {
         if (first < head) {
             const float v[PER] = {as_float(x[first])};
             f(first, v, 1);
         }
-        // (four vectors on their way at a time: one CU's share of memory is latency)
         for (int k0 = first; k0 < vecs; k0 += 4 * step) {
-            union { uint4 w; T t[PER]; } u[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) u[b].w = reinterpret_cast<const uint4*>(x + head)[min(k0 + b * step, vecs - 1)];
+            if (k0 != first) ahead = fetch(k0, step);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const int k = k0 + b * step;
                 if (k >= vecs) break;
+                union { uint4 w; T t[PER]; } u;
+                u.w = ahead.w[b];
                 float v[PER];
 #pragma unroll
-                for (int j = 0; j < PER; ++j) v[j] = as_float(u[b].t[j]);
+                for (int j = 0; j < PER; ++j) v[j] = as_float(u.t[j]);
                 f(head + k * PER, v, PER);
             }
         }
