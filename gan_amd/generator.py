@@ -37,7 +37,8 @@ PI, PO, AND = 0, 1, 2
 class GeneratorPlan:
     """Order, candidate windows and edge offsets of one template for one candidate_k."""
 
-    __slots__ = ("n", "K", "E", "types", "order", "rank", "want", "cnt", "cand", "fb", "eoff", "key", "C", "cls", "x_cls")
+    __slots__ = ("n", "K", "E", "types", "order", "rank", "want", "cnt", "cand", "fb", "eoff", "key", "C", "cls", "x_cls",
+                 "windows")
 
     @staticmethod
     def build(x: torch.Tensor, node_depth: Optional[torch.Tensor], K: int) -> "GeneratorPlan":
@@ -45,7 +46,7 @@ class GeneratorPlan:
         dev = x.device
         n = int(x.size(0))
         p = GeneratorPlan()
-        p.n, p.K = n, int(K)
+        p.n, p.K, p.windows = n, int(K), None
         i32 = dict(dtype=torch.int32, device=dev)
         p.types, p.order, p.rank = torch.empty(n, **i32), torch.empty(n, **i32), torch.empty(n, **i32)
         kind, dptr = 0, None
@@ -192,7 +193,8 @@ class AIGGenerator(nn.Module):
             raise TypeError("sampling is a gan_amd.logits.Sampling")
         if u is None:
             u = torch.rand((rows, 2), device=dev)
-        if not (torch.is_tensor(u) and u.device == dev and u.dtype == torch.float32 and u.numel() == 2 * rows):
+        if not (torch.is_tensor(u) and u.device == dev and u.dtype == torch.float32 and u.dim() > 1 and u.size(-1) == 2 and
+                u.numel() == 2 * rows):
             raise _abi.AigAbiError(f"the random numbers of a draw are float32 [{rows} slots, 2] on {dev}")
         return L.sampling_arg(sampling, rows, dev), u.reshape(rows, 2).contiguous()
 
@@ -202,13 +204,12 @@ class AIGGenerator(nn.Module):
     def score_windows(self, templates):
         """The candidate windows of templates of one node count, back to back, as ``class_scores`` takes them, and the
         weight that makes a sum over their slots the mean over the slots that need a fan-in.  Row ``g n + r`` is slot ``r`` of
-        template ``g``; its kind is ``g C + (class of its node)``.  The last few are kept, with the plans they are made of."""
+        template ``g``; its kind is ``g C + (class of its node)``.  They are part of the templates' plans and kept with them."""
         st = self._stacked_plans(list(templates), templates[0].x.device)
-        cache = self.__dict__.setdefault("_window_stacks", {})
-        key = tuple(id(p) for p in st["plans"])
-        hit = cache.get(key)
-        if hit is not None and all(a is b for a, b in zip(hit[0], st["plans"])):
-            return hit[1], hit[2], st
+        alone = st["plans"][0] if len(st["plans"]) == 1 else None
+        kept = st.get("windows") if alone is None else alone.windows
+        if kept is not None:
+            return (*kept, st)
         B, n, C = len(templates), st["n"], st["C"]
         if not 0 < C <= self.TRAIN_CLASS_LIMIT:
             raise ValueError(f"candidate logits can be differentiated for templates of 1 to {self.TRAIN_CLASS_LIMIT} distinct "
@@ -221,9 +222,10 @@ class AIGGenerator(nn.Module):
         needs = (st["want"].reshape(-1) > 0) & (counts > 0)
         windows = L.ScoreWindows.of(cand.contiguous(), counts, cls.reshape(-1), kind.contiguous(), B * C)
         weight = needs.float() / needs.sum().clamp(min=1)
-        if len(cache) >= 4:
-            cache.pop(next(iter(cache)))
-        cache[key] = (list(st["plans"]), windows, weight)
+        if alone is None:
+            st["windows"] = (windows, weight)
+        else:
+            alone.windows = (windows, weight)
         return windows, weight, st
 
     def score_table(self, st, zs: torch.Tensor) -> torch.Tensor:

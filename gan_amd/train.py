@@ -580,6 +580,18 @@ def _side_stream(device: torch.device) -> "torch.cuda.Stream":
     return _SIDE_STREAMS[idx]
 
 
+def check_distillation(a) -> None:
+    """The teacher's flags, before the first step (a step that raises is skipped, so a bad flag would skip every one)."""
+    if not 1 <= a.distill_top <= logits_ops.MAX_TOP:
+        raise ValueError(f"--distill-top is 1 to {logits_ops.MAX_TOP}, got {a.distill_top}")
+    if not 1e-6 <= a.distill_temperature <= 1e6:
+        raise ValueError(f"--distill-temperature is within 1e-6 and 1e6, got {a.distill_temperature}")
+    if not 0.0 <= a.distill_weight < float("inf"):
+        raise ValueError(f"--distill-weight must not be negative, got {a.distill_weight}")
+    if a.teacher_candidate_k is not None and a.teacher_candidate_k < 1:
+        raise ValueError(f"--teacher-candidate-k must be positive, got {a.teacher_candidate_k}")
+
+
 class Trainer:
     """State of one training run; ``step(batch)`` is one pass of the reference's inner loop body."""
 
@@ -773,6 +785,7 @@ class Trainer:
     # ------------------------------------------------------------------ a generator that learns from a teacher
     def _load_teacher(self) -> None:
         a = self.args
+        check_distillation(a)
         state = torch.load(a.teacher_ckpt, map_location=self.device, weights_only=True)
         z_dim = int(state["node_proj.0.weight"].size(1)) - a.g_hidden
         if z_dim != a.z_dim:

@@ -116,6 +116,29 @@ def test_drawn_fan_ins_are_refused():
         G.candidate_logits([distinct], z[None])
 
 
+def test_random_numbers_of_another_shape_are_refused():
+    G, tpl = generator(8), template(30, seed=1)
+    n, z = tpl.x.size(0), torch.zeros(128, device=DEV)
+    for shape in ((2, n), (2 * n,), (n, 2, 1)):
+        with pytest.raises(_abi.AigAbiError):
+            G(tpl, z, sampling=L.Sampling(), u=torch.zeros(shape, device=DEV))
+    assert same_graph(G(tpl, z, sampling=L.Sampling(), u=torch.zeros(n, 2, device=DEV)),
+                      G(tpl, z, sampling=L.Sampling(), u=torch.zeros(1, n, 2, device=DEV)))
+
+
+def test_windows_are_kept_with_the_plans_they_are_made_of():
+    G, a, b = generator(8), template(30, seed=1), template(30, seed=2)
+    for templates in ([a], [a, b]):
+        first, again = G.score_windows(templates), G.score_windows(templates)
+        assert first[0] is again[0] and first[1] is again[1]
+    assert not torch.equal(G.score_windows([a])[0].cls, G.score_windows([b])[0].cls)
+    z = torch.zeros(128, device=DEV)
+    before = G.candidate_logits([a], z[None]).detach()
+    other = Data(x=a.x.flip(0).contiguous(), node_depth=a.node_depth)
+    assert not torch.equal(G.candidate_logits([other], z[None]).detach(), before)
+    assert torch.equal(G.candidate_logits([a], z[None]).detach(), before)
+
+
 def reference_table(G, x_cls, z):
     """The score table in 64 bits on the CPU: ``[C, C]`` over (target class, candidate class)."""
     p = {k: v.detach().double().cpu().requires_grad_(True) for k, v in G.named_parameters()}

@@ -94,3 +94,14 @@ def test_a_backward_pass_is_not_recorded(monkeypatch):
         monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
         with pytest.raises(_abi.AigAbiError, match="not recorded"):
             L._check_backward("distill_loss")
+
+
+@pytest.mark.parametrize("flag,value", [("distill_top", 0), ("distill_top", 257), ("distill_temperature", 0.0), ("distill_temperature", float("nan")),
+                                        ("distill_weight", -1.0), ("distill_weight", float("inf")), ("teacher_candidate_k", 0)])
+def test_flags_of_a_teacher(flag, value):
+    from gan_amd import train
+    args = train.build_parser().parse_args(["--dataset-dir", "d", "--teacher-ckpt", "g.pt"])
+    train.check_distillation(args)
+    setattr(args, flag, value)
+    with pytest.raises(ValueError, match=flag.replace("_", "-")):
+        train.check_distillation(args)
