@@ -421,6 +421,7 @@ template <typename T> int distill(hipStream_t s, const T* x, T* grad, const Dist
     else if (a.width <= 256) launch_narrow<T, 16, 16>(s, x, grad, a);
     else if (a.width <= 512) launch_narrow<T, 64, 8>(s, x, grad, a);
     else if (a.width <= NARROW) launch_narrow<T, 64, 16>(s, x, grad, a);
+    else if (in_registers(a.rows, a.width)) launch_narrow<T, 64, 32>(s, x, grad, a);
     else {
         const dim3 grid((unsigned)a.rows);
         if (grad && a.loss) hipLaunchKernelGGL((k_distill_wide<T, true, true>), grid, dim3(WIDE_T), 0, s, x, grad, a);
@@ -453,7 +454,7 @@ extern "C" int aig_distill_rows(const aig_distill* d, float* loss, void* grad, i
     a.rows = d->rows; a.ld = d->ld; a.grad_ld = grad_ld; a.width = (int)d->width; a.m = (int)d->m;
     a.temperature = d->temperature; a.factor = d->scale;
     a.per = rows::LOG2E / (double)d->temperature;
-    a.stats = d->width > rows::NARROW ? d->stats : nullptr;
+    a.stats = d->stats;
     a.counts = d->counts; a.values = d->values; a.lse = d->lse; a.weight = d->weight; a.index = d->index;
     a.upstream = upstream; a.upstream_stride = upstream_stride; a.loss = loss;
     hipStream_t s = static_cast<hipStream_t>(stream);

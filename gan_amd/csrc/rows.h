@@ -17,6 +17,14 @@ namespace rows {
 
 constexpr int MAX_WIDTH = AIG_ROWS_MAX_WIDTH;
 constexpr int NARROW = 1024;            // rows up to this width are held by a group's registers
+// Wider ones have a workgroup each, but for rows to 2048 places that are more than the workgroups the chip holds at a time: 32
+// places a lane then, a wave a row.  4,000 x 2,000 in registers and by workgroups: top-p 37 and 202 us, top-k 50 36 and 145, top 16
+// 15 and 60, loss and gradient 31 and 106; 512 rows 16 and 28, 23 and 20, 9 and 9, 10 and 16; 64 rows 16 and 14, 9 and 11, 9 and 5,
+// 9 and 8.
+constexpr int NARROW_MANY = 2048, MANY_ROWS = 512;
+__host__ __device__ constexpr bool in_registers(long long rows, long long width) {
+    return width <= NARROW || (width <= NARROW_MANY && rows >= MANY_ROWS);
+}
 
 // ---------------------------------------------------------------- values
 // logits as f32, exactly, whatever they are stored in

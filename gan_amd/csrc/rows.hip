@@ -162,14 +162,14 @@ __device__ __forceinline__ void exact_draws(const SampleRows& a, const RowSettin
     }
 }
 
-// The same in f32, as long as that is certain.  A sum of weights in f32 is off by less than 2^-19 of the row's total: an
-// exponential of -d carries three roundings of d (2^-24 each, times ln 2) and its own last bit, the average of d over the
-// weights of 1024 places is at most 6.5; a sum of 16 in a lane rounds by half of 16 such steps of the lane's, the six steps
-// over the lanes by six of the total: 0.8e-6 + 0.1e-6 + 0.8e-6.  A decision between two numbers that lie further apart than
-// MARGIN of the total is therefore the exact one; a row with a closer one is drawn again in f64 (returns false): one in a
-// hundred, mostly for top-p's border among places of small weight.  What that buys: an f64 exponential alone is 26
-// instructions a place, and sums in f32 take their lane permutations along.
-constexpr float MARGIN = 1.0f / 262144.0f;
+// The same in f32, as long as that is certain.  A sum of weights in f32 is off by less than 2^-19 of the row's total (2^-18 for
+// rows of 2048 places): an exponential of -d carries three roundings of d (2^-24 each, times ln 2) and its own last bit, the
+// average of d over the weights of 1024 places is at most 6.5 (2048: 7.2); a sum of 16 (32) in a lane rounds by half of as many
+// such steps of the lane's, the six steps over the lanes by six of the total: 0.8e-6 + 0.1e-6 + 0.8e-6 (0.9 + 0.1 + 1.3).  A
+// decision between two numbers that lie further apart than margin_of of the total is therefore the exact one; a row with a
+// closer one is drawn again in f64 (returns false): one in a hundred, mostly for top-p's border among places of small weight.
+// What that buys: an f64 exponential alone is 26 instructions a place, and sums in f32 take their lane permutations along.
+template <int PLACES> __device__ __host__ constexpr float margin_of() { return PLACES <= 1024 ? 1.0f / 262144.0f : 1.0f / 131072.0f; }
 
 // Weights that cannot be told apart by their order: exponentials of different logits are in order but for two last bits (2^-22).
 __device__ __forceinline__ float band_high(float thr) { return thr * (1.0f + 1.0f / 1048576.0f); }
@@ -273,7 +273,7 @@ __device__ __forceinline__ bool border_in_list(const float (&w)[E], int top_k, f
             stay += upto < p;
             upto += ws[e];
         }
-        sure = sure && nearest > MARGIN * total;
+        sure = sure && nearest > margin_of<G * E>() * total;
         keep = max(min(keep, all<G>(stay, Add())), 1);
     }
     thr = __uint_as_float(at_rank<G, M>(s, keep - 1));
@@ -334,7 +334,7 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
                     stay += upto < p;
                     upto += ws[e];
                 }
-                sure = sure && nearest > MARGIN * total;
+                sure = sure && nearest > margin_of<G * E>() * total;
                 keep = max(min(keep, all<G>(stay, Add())), 1);
             }
             thr = __uint_as_float(at_rank<G, E>(s, keep - 1));
@@ -380,7 +380,7 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
         const float least = fminf(how.min_p, 1.0f);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            sure = sure && !(v[e] < m && fabsf(w[e] - least) <= 4.0f * MARGIN * least);
+            sure = sure && !(v[e] < m && fabsf(w[e] - least) <= 4.0f * margin_of<G * E>() * least);
             w[e] = w[e] >= least ? w[e] : 0.0f;
         }
     }
@@ -403,7 +403,7 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
     float margin = 0.0f;
     for (int d = 0; d < a.draws; ++d) {
         const float total = all<G>(sum, Add());
-        margin = fmaxf(margin, MARGIN * total);
+        margin = fmaxf(margin, margin_of<G * E>() * total);
         float upto = before<G>(sum);
         const float t = a.uniform(r, d) * total;
         int at = -1;
@@ -1464,6 +1464,9 @@ template <typename T> int sample_rows(hipStream_t s, const T* x, SampleRows a) {
     } else if (a.width <= NARROW) {
         a.vec = vec(16);
         hipLaunchKernelGGL((k_sample<T, 64, 16>), blocks(64), dim3(256), 0, s, x, a);
+    } else if (in_registers(a.rows, a.width)) {
+        a.vec = vec(32);
+        hipLaunchKernelGGL((k_sample<T, 64, 32>), blocks(64), dim3(256), 0, s, x, a);
     } else {
         hipLaunchKernelGGL(k_sample_wide<T>, dim3((unsigned)a.rows), dim3(WIDE_T), 0, s, x, a);
     }
@@ -1507,6 +1510,11 @@ template <typename T> int top_rows(hipStream_t s, const T* x, TopArgs a) {
         if (a.m <= 48) LAUNCH_TOP(64, 16, 1);
         else if (a.m > (PACKED ? 64 : 96)) LAUNCH_TOP(64, 16, PACKED ? 0 : 4);
         else LAUNCH_TOP(64, 16, 2);
+    } else if (in_registers(a.rows, a.width)) {
+        a.vec = vec(32);
+        if (a.m <= 48) LAUNCH_TOP(64, 32, 1);
+        else if (a.m > 96) LAUNCH_TOP(64, 32, 4);
+        else LAUNCH_TOP(64, 32, 2);
 #undef LAUNCH_TOP
     } else {
         hipLaunchKernelGGL(k_top_wide<T>, dim3((unsigned)a.rows), dim3(WIDE_T), 0, s, x, a);
@@ -1536,7 +1544,7 @@ using namespace aig;
 int aig::check_row_limits(const char* what, int64_t rows, int64_t width) {
     if (width > AIG_ROWS_MAX_WIDTH) return fail(AIG_ELIMIT, "%s: rows of %lld: at most %d", what, (long long)width, AIG_ROWS_MAX_WIDTH);
     // (a launch has fewer than 2^32 threads: a wave a row, a workgroup of 1024 for rows beyond a wave's registers)
-    const int64_t most = width <= rows::NARROW ? (1ll << 26) - 1 : (1ll << 22) - 1;
+    const int64_t most = rows::in_registers(rows, width) ? (1ll << 26) - 1 : (1ll << 22) - 1;
     if (rows > most) return fail(AIG_ELIMIT, "%s: %lld rows of %lld: at most %lld", what, (long long)rows, (long long)width, (long long)most);
     return AIG_OK;
 }

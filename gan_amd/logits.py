@@ -26,7 +26,7 @@ from . import _abi
 MAX_WIDTH = 131072
 MAX_DRAWS = 8
 MAX_TOP = 256
-NARROW = 1024          # rows up to this width are held in registers, wider ones are a workgroup's each
+NARROW = 1024          # rows up to this width are held in registers and keep no sums for their gradient
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 

@@ -178,6 +178,53 @@ def test_sample_borders_among_places_that_do_not_part(width):
                 check_sample(x, u, top_k=k, top_p=p, temperature=0.9)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width,ld", [(1025, 1025), (1600, 1608), (2047, 2050), (2048, 2048)])
+def test_many_rows_are_answered_like_few(width, ld, dtype):
+    """Rows of 1025 to 2048 places: what hundreds of them get is what a part of them gets, and the first few are the oracle's."""
+    rows, m, t = 530, 20, 1.5
+    x = torch.empty(rows, ld, dtype=dtype)
+    x[:, :width] = make_logits(rows, width, dtype, seed=width)
+    x[:, width:] = float("nan")
+    x = x[:, :width]
+    x[0, ::2] = -math.inf
+    x[1] = 1.0
+    x[2] = -math.inf
+    x[3, 7:] = torch.finfo(dtype).min
+    x[4, ::3] = float("nan")
+    x[5] = make_logits(1, width, dtype, seed=3, ties=True)[0]
+    x[6, 5:] = math.inf
+    counts = make_counts(rows, width, 5)
+    counts[:8] = width
+    u = torch.rand(rows, 2, generator=rng(6))
+    dx, dc, du = x.to(DEV), counts.to(DEV), u.to(DEV)
+    full = torch.empty(rows, ld, dtype=dtype, device=DEV)
+    full[:, :width] = dx
+    full[:, width:] = float("nan")
+    dx = full[:, :width]
+    parts = (slice(0, 200), slice(200, 400), slice(400, rows))
+    for how in (dict(), dict(top_p=0.9), dict(top_k=50), dict(top_k=30, top_p=0.8, min_p=0.01), dict(top_k=700, temperature=0.8), dict(temperature=0.0)):
+        many = L.sample_rows(dx, du, counts=dc, **how)
+        few = torch.cat([L.sample_rows(dx[s], du[s].contiguous(), counts=dc[s].contiguous(), **how) for s in parts])
+        assert torch.equal(many, few), how
+        for r in range(10):
+            n = int(counts[r])
+            assert many[r].tolist() == sample_row(x[r, :n].float().numpy().astype(np.float64), u[r].numpy().astype(np.float64), **how), (r, how)
+    for k in (1, m, 60, 120, 256):
+        many = L.top_rows(dx, k, counts=dc, temperature=t)
+        few = [L.top_rows(dx[s], k, counts=dc[s].contiguous(), temperature=t) for s in parts]
+        assert torch.equal(many.index, torch.cat([f.index for f in few])) and torch.equal(many.values, torch.cat([f.values for f in few]))
+        # (sums of 32 places a lane, or 2 a thread, and a tree: 64 half steps of the sum at most, and a logarithm's)
+        a, b = many.lse, torch.cat([f.lse for f in few])
+        assert torch.equal(a.isinf(), b.isinf())
+        both = a.isfinite()
+        assert ((a[both] - b[both]).abs() <= 2.0 ** -24 * (4 * b[both].abs() + 80)).all()
+    y = make_logits(rows, width, dtype, seed=width + 1)
+    v, i, s = make_teacher(y, m, t, 4, counts, True)
+    check_distill(y, v, i, s, t, counts)
+    check_distill(y, v, i, None, t, counts, torch.rand(rows, generator=rng(8)))
+
+
 @pytest.mark.parametrize("width", [1500, 8200, 40000])
 @pytest.mark.parametrize("ties", [False, True])
 def test_sample_wide_rows_every_way(width, ties):
