@@ -38,12 +38,25 @@ class Sampling(NamedTuple):
     min_p: Union[float, torch.Tensor] = 0.0
 
 
-class TopRows(NamedTuple):
-    """What ``top_rows`` keeps of a teacher's rows; ``temperature`` is the one ``lse`` was taken at (None: not known)."""
+class _TopRows(NamedTuple):
     values: torch.Tensor
     index: torch.Tensor
     lse: Optional[torch.Tensor]
+
+
+class TopRows(_TopRows):
+    """What ``top_rows`` keeps of a teacher's rows: the three tensors ``values``, ``index`` and ``lse``.  ``temperature``, an
+    attribute beside them, is the one ``lse`` was taken at (None: not known)."""
     temperature: Optional[float] = None
+
+    def __new__(cls, values, index, lse, temperature=None):
+        self = super().__new__(cls, values, index, lse)
+        self.temperature = temperature
+        return self
+
+    def _replace(self, **fields):
+        temperature = fields.pop("temperature", self.temperature)
+        return TopRows(*super()._replace(**fields), temperature)
 
 
 class ScoreWindows(NamedTuple):
