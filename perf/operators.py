@@ -307,7 +307,7 @@ def run(s):
         return L.sample_rows(s["logits"], s["u"], counts=s["counts"], temperature=s["temperature"], top_k=s["top_k"],
                              top_p=s["top_p"], min_p=s["min_p"])
     if s["op"] == "top":
-        return tuple(L.top_rows(s["logits"], s["m"], counts=s["counts"], temperature=s["temperature"])[:3])
+        return tuple(L.top_rows(s["logits"], s["m"], counts=s["counts"], temperature=s["temperature"]))
     if s["op"] == "distill":
         top = L.TopRows(s["values"], s["index"], s["lse"])
         kw = dict(counts=s["counts"], weight=s["weight"], temperature=s["temperature"], tail=s["tail"])
