@@ -171,6 +171,8 @@ __device__ __forceinline__ void exact_draws(const SampleRows& a, const RowSettin
 // What that buys: an f64 exponential alone is 26 instructions a place, and sums in f32 take their lane permutations along.
 template <int PLACES> __device__ __host__ constexpr float margin_of() { return PLACES <= 1024 ? 1.0f / 262144.0f : 1.0f / 131072.0f; }
 
+constexpr float HALF_UNIT = (float)(0.5 / UNIT);       // of the largest weight's 1: less is no whole multiple of 2^-36 but 0
+
 // Weights that cannot be told apart by their order: exponentials of different logits are in order but for two last bits (2^-22).
 __device__ __forceinline__ float band_high(float thr) { return thr * (1.0f + 1.0f / 1048576.0f); }
 __device__ __forceinline__ float band_low(float thr) { return thr * (1.0f - 1.0f / 1048576.0f); }
@@ -453,7 +455,18 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
                 sum += w[e];
             }
         }
-        if (at < 0 && total > 0.0f) return false;       // (no weight left at all: there is no place to draw)
+        if (at < 0) {
+            if (total > 0.0f) return false;
+            // No weight is left, or what is left was below the last bit of the sum that it was part of: the exact form draws a
+            // place that is there.  (The weights themselves: LDS holds 0 for the places that were drawn, and what is clearly
+            // below half a unit is none.)
+            if (BY_GROUP) {
+                int left = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) left |= lds[lane * E + e] > 0.99f * HALF_UNIT;
+                if (all<G>(left, Max())) return false;
+            }
+        }
         if (lane == 0) a.store(r, d, d < want ? at : -1, first, n);
     }
     return true;

@@ -1,0 +1,65 @@
+"""Rows of logits: calls that their operators once answered wrongly, against definitions in 64 bits."""
+import pytest
+import torch
+
+from gan_amd import logits as L
+from test_distill_gpu import generator, template
+from test_logits_gpu import BF16, F16, F32, check_sample, make_logits, rng
+from util_rows import sample_row
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+
+
+@pytest.mark.parametrize("rows,width", [(300, 9), (300, 20), (300, 64), (200, 256), (100, 512), (100, 1024), (12, 1500), (530, 2048)])
+def test_places_of_little_weight_are_drawn_when_they_are_what_is_left(rows, width):
+    """Few places, most of them far below the largest: once the largest is drawn, what is left is below the last bit of the
+    sum that held it - and is drawn all the same."""
+    g = rng(width)
+    counts = torch.randint(2, min(width, 8) + 1, (rows,), generator=g, dtype=torch.int32)
+    u = torch.rand(rows, 4, generator=g)
+    for i, t in enumerate((0.05, 0.1, 0.2, 0.3)):
+        x = make_logits(rows, width, (F32, BF16, F16)[i % 3], seed=width + i)
+        x[0, :2] = torch.tensor([0.0, -18.0 * t])          # one place beside the largest, in the same lane
+        counts[0] = 2
+        x[1] = -50.0                                       # ... at the lane's end, and in the one beside it
+        x[1, :8] = torch.tensor([0.0, -17.0, -17.5, -18.0, -19.0, -20.0, -21.0, -22.0]) * t
+        counts[1] = min(8, width)
+        x[2, :2] = torch.tensor([0.0, -26.0]) * t          # below a multiple of 2^-36: nothing is left
+        counts[2] = 2
+        x[3, :3] = torch.tensor([0.0, -24.5, -24.0]) * t
+        counts[3] = 3
+        for how in (dict(), dict(top_k=2), dict(top_k=3)):
+            check_sample(x, u, counts=counts, temperature=t, **how)
+    # all of a row's places that stay in one lane, among many that do not
+    x = make_logits(rows, width, F32, seed=3) - 8.0
+    x[:, 0], x[:, 1], x[:, 2] = 9.0, -8.0, -8.5
+    x[:, 3:] -= 20.0
+    check_sample(x, u, top_k=3)
+    check_sample(x, u[:, :2].contiguous(), top_k=2)
+    check_sample(x, u)
+
+
+@pytest.mark.parametrize("K", [8, 40, 300])
+def test_fan_ins_drawn_at_a_low_temperature(K):
+    """A slot's second fan-in is its second draw, however little of the weight that has."""
+    G, tpl = generator(K, seed=3), template(150, seed=4)
+    n, g = tpl.x.size(0), rng(K)
+    z, u = torch.randn(128, generator=g).to(DEV), torch.rand(n, 2, generator=g).to(DEV)
+    logits = G(tpl, z, return_debug=True, sampling=L.Sampling(), u=u)._debug["logits"].cpu().double()
+    plan = G.plan_for(tpl, tpl.x, tpl.node_depth)
+    cnt, want = plan.cnt.cpu(), plan.want.cpu()
+    t = torch.ones(n)
+    for r in range(n):                       # what is below the largest logit of a slot has e^-20 of its weight and less
+        v = logits[r, :cnt[r]].unique()
+        t[r] = (v[-1] - v[-2]) / 20.0 if want[r] > 0 and len(v) > 1 else 1.0
+    sel = G(tpl, z, return_debug=True, sampling=L.Sampling(temperature=t.to(DEV)), u=u)._debug["sel"].cpu()
+    seconds = 0
+    for r in range(n):
+        if want[r] == 0 or cnt[r] == 0:
+            continue
+        first, second = sample_row(logits[r, :cnt[r]].numpy(), u[r].double().cpu().numpy(), temperature=float(t[r]))
+        second = first if want[r] < 2 or second < 0 else second
+        seconds += first != second
+        assert sel[r].tolist() == [first, second], (r, int(cnt[r]), float(t[r]))
+    assert seconds > 0
