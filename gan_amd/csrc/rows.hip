@@ -378,11 +378,12 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
             }
         }
     }
-    if (how.min_p > 0.0f) {
-        const float least = fminf(how.min_p, 1.0f);
+    if (how.min_p > 2.0f * HALF_UNIT) {       // (a smaller one takes nothing out that is not 0 anyway)
+        // (a weight is compared as a multiple of 2^-36: up to half a unit beside itself)
+        const float least = fminf(how.min_p, 1.0f), near = 4.0f * margin_of<G * E>() * least + HALF_UNIT;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            sure = sure && !(v[e] < m && fabsf(w[e] - least) <= 4.0f * margin_of<G * E>() * least);
+            sure = sure && !(v[e] < m && fabsf(w[e] - least) <= near);
             w[e] = w[e] >= least ? w[e] : 0.0f;
         }
     }

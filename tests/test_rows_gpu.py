@@ -40,6 +40,23 @@ def test_places_of_little_weight_are_drawn_when_they_are_what_is_left(rows, widt
     check_sample(x, u)
 
 
+@pytest.mark.parametrize("rows,width", [(400, 9), (400, 64), (200, 256), (100, 512), (100, 1024), (12, 1500), (530, 2048)])
+def test_min_p_is_compared_with_weights_in_whole_units(rows, width):
+    """A min-p of a few units of 2^-36: the half that a weight is rounded by decides who reaches it."""
+    g, unit = rng(width + 1), 2.0 ** -36
+    n = min(width, 8)
+    counts = torch.full((rows,), n, dtype=torch.int32)
+    u = torch.rand(rows, 4, generator=g)
+    for i, share in enumerate((1e-9, 68.5 * unit, 5.4 * unit, 2.5 * unit, 1.5 * unit, unit, 1e-12)):
+        x = make_logits(rows, width, F32, seed=width + i)
+        # weights from a little under the share to a little over it, beside the largest
+        x[:, :n] = torch.log(torch.tensor(share * 0.98)) + 0.04 * torch.rand(rows, n, generator=g)
+        x[:, 0] = 0.0
+        x[: rows // 2, 1:n] = torch.log(torch.tensor(share)) + 0.6 * (torch.rand(rows // 2, n - 1, generator=g) - 0.5)
+        check_sample(x, u, counts=counts, min_p=share)
+        check_sample(x, u, counts=counts, min_p=share, top_k=5)
+
+
 @pytest.mark.parametrize("K", [8, 40, 300])
 def test_fan_ins_drawn_at_a_low_temperature(K):
     """A slot's second fan-in is its second draw, however little of the weight that has."""
