@@ -232,6 +232,25 @@ def _teacher(logits, top, counts, weight, temperature, tail, scale=1.0):
 _HELD = ("counts", "values", "index", "lse", "weight")
 
 
+_OPERANDS = {"counts": (("rows",), torch.int32), "values": (("rows", "m"), torch.float32), "index": (("rows", "m"), torch.int32),
+             "lse": (("rows",), torch.float32), "weight": (("rows",), torch.float32), "cand": (("rows", "width"), torch.int32),
+             "cls": (("nodes",), torch.int32), "row_kind": (("rows",), torch.int32), "by_kind": (("rows",), torch.int32),
+             "kind_start": ((), torch.int32)}
+
+
+def _handed_back(a, names, tensors, device) -> list:
+    """Saved operands where an argument block looks for them, and the tensors that must outlive the launch.  (Hooks on saved
+    tensors may hand out copies, which are checked as the operands themselves were.)"""
+    out = list(tensors)
+    for i, (name, v) in enumerate(zip(names, tensors)):
+        sizes, dtype = _OPERANDS[name]
+        if v is not None and (v.data_ptr() != getattr(a, name) or v.dtype is not dtype or not v.is_contiguous()):
+            out[i] = v.contiguous()
+            shape = (a.kinds + 1,) if name == "kind_start" else tuple(getattr(a, n) for n in sizes)
+            setattr(a, name, _side(out[i], shape, dtype, device, "saved " + name))
+    return out
+
+
 def _distill(device, a: _abi.Distill, loss, grad, upstream=None) -> None:
     _call("aig_distill_rows", device, C.byref(a), None if loss is None else loss.data_ptr(), None if grad is None else grad.data_ptr(),
           a.width, None if upstream is None else upstream.data_ptr(), 0 if upstream is None or upstream.numel() == 1 else 1,
@@ -269,18 +288,22 @@ class _DistillLoss(torch.autograd.Function):
             arg.stats = ctx.stats.data_ptr()
         _distill(logits.device, arg, loss, None)
         ctx.save_for_backward(logits, *held)
-        ctx.arg = arg
+        ctx.arg, ctx.stride, ctx.dtype = arg, logits.stride(), logits.dtype
         return _sum_rows(loss) if reduce else loss
 
     @staticmethod
     def backward(ctx, g):
         _check_backward("distill_loss")
         logits, *held = ctx.saved_tensors
-        a = ctx.arg
-        a.logits = logits.data_ptr()       # (hooks on saved tensors may hand out copies)
-        for name, v in zip(_HELD, held):
-            if v is not None:
-                setattr(a, name, v.data_ptr())
+        a = _abi.Distill.from_buffer_copy(ctx.arg)
+        if logits.data_ptr() != a.logits or logits.stride() != ctx.stride or logits.dtype is not ctx.dtype:
+            # (a hook's copy has strides of its own)
+            logits = logits if logits.stride(1) == 1 else logits.contiguous()
+            if logits.dtype is not ctx.dtype or logits.shape != (a.rows, a.width) or logits.device != g.device:
+                raise _abi.AigAbiError(f"saved logits must be {ctx.dtype} {(a.rows, a.width)} on {g.device}, got {logits.dtype} "
+                                       f"{tuple(logits.shape)} on {logits.device}")
+            a.logits, a.ld = logits.data_ptr(), _rows_of(logits, "distill_loss")[2]
+        held = _handed_back(a, _HELD, held, logits.device)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
@@ -351,10 +374,8 @@ class _ClassScores(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         _check_backward("class_scores")
-        a, held = ctx.arg, ctx.saved_tensors
-        for name, v in zip(ScoreWindows._fields, held):
-            if v is not None:
-                setattr(a, name, v.data_ptr())
+        a = _abi.ScoreWindowsArg.from_buffer_copy(ctx.arg)
+        held = _handed_back(a, ScoreWindows._fields, ctx.saved_tensors, g.device)
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
         return _table_grad(g, a), None, None

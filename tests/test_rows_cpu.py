@@ -25,3 +25,58 @@ def test_a_teachers_rows_are_three_tensors():
         top._replace(places=index)
     for other in (copy.copy(top), copy.deepcopy(top), pickle.loads(pickle.dumps(top))):
         assert type(other) is L.TopRows and other.temperature == 2.0 and torch.equal(other.lse, lse)
+
+
+@pytest.mark.parametrize("seen", ["slice", "expanded", "dense"])
+@pytest.mark.parametrize("copy_of", ["dense", "by columns", "wider", "none"])
+def test_a_copy_of_saved_logits_has_strides_of_its_own(monkeypatch, seen, copy_of):
+    """The backward pass passes the kernel what a hook on saved tensors hands back, with that tensor's strides.  (What would be
+    launched is looked at instead.)"""
+    rows, width, wide = 6, 5, 12
+    launched = []
+    monkeypatch.setattr(L, "_rows_of", lambda t, what: (t.size(0), t.size(1), t.stride(0), 0))
+    monkeypatch.setattr(L, "_call", lambda name, device, *args, meta=None: launched.append((name, args[0]._obj)) if name == "aig_distill_rows" else None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    whole = torch.randn(rows, wide).requires_grad_(True)
+    x = whole[:, :width] if seen == "slice" else whole[:1, :width].expand(rows, width) if seen == "expanded" else whole[:, :width].contiguous()
+    top = L.TopRows(torch.randn(rows, 2), torch.zeros(rows, 2, dtype=torch.int32), torch.zeros(rows), 1.0)
+    handed = {}
+
+    def unpack(t):
+        if not t.is_floating_point() or t.shape != (rows, width):
+            return t if copy_of == "none" else t.clone()
+        if copy_of == "dense":
+            t = t.clone(memory_format=torch.contiguous_format)
+        elif copy_of == "by columns":
+            t = t.t().contiguous().t()
+        elif copy_of == "wider":
+            t = torch.cat([t, torch.zeros(rows, 3)], dim=1)[:, :width]
+        handed["x"] = t
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        loss = L.distill_loss(x, top, reduction="none")
+    loss.backward(torch.ones(rows))
+    (_, forth), (_, back) = launched
+    assert forth.ld == x.stride(0) and forth.logits == x.data_ptr()
+    t = handed["x"]
+    if copy_of == "by columns":          # rows whose logits are apart are laid out anew
+        assert back.logits != t.data_ptr() and back.ld == width
+    else:
+        assert back.logits == t.data_ptr() and back.ld == t.stride(0)
+    assert (back.rows, back.width, back.m) == (rows, width, 2)
+    assert forth.logits == x.data_ptr() and forth.ld == x.stride(0)        # (what was kept stays what it was)
+
+
+@pytest.mark.parametrize("change", [lambda t: t.bfloat16(), lambda t: t[:-1].clone(), lambda t: t[:, :-1].clone()])
+def test_saved_tensors_that_come_back_as_others_are_refused(monkeypatch, change):
+    monkeypatch.setattr(L, "_rows_of", lambda t, what: (t.size(0), t.size(1), t.stride(0), 0))
+    monkeypatch.setattr(L, "_call", lambda *args, **kw: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    x, values = torch.randn(6, 5, requires_grad=True), torch.randn(6, 2)
+    top = L.TopRows(values, torch.zeros(6, 2, dtype=torch.int32), torch.zeros(6), 1.0)
+    for shape in ((6, 5), (6, 2)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.is_floating_point() and t.shape == shape else t):
+            loss = L.distill_loss(x, top, reduction="none")
+        with pytest.raises(L._abi.AigAbiError, match="saved (logits|values) must be"):
+            loss.backward(torch.ones(6))

@@ -4,7 +4,7 @@ import torch
 
 from gan_amd import logits as L
 from test_distill_gpu import generator, template
-from test_logits_gpu import BF16, F16, F32, check_sample, make_logits, rng
+from test_logits_gpu import BF16, F16, F32, check_sample, make_logits, make_windows, rng
 from util_rows import sample_row
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,46 @@ def test_fan_ins_drawn_at_a_low_temperature(K):
         seconds += first != second
         assert sel[r].tolist() == [first, second], (r, int(cnt[r]), float(t[r]))
     assert seconds > 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width", [(9, 64), (9, 300), (530, 2000), (9, 2000), (5, 5000)])
+def test_gradient_of_logits_that_hooks_hand_back_as_copies(rows, width, dtype):
+    """Saved on the host, cloned, or laid out by columns: the gradient is that without hooks."""
+    whole = make_logits(rows, width + 24, dtype, seed=width).to(DEV)
+    whole[:, width:] = float("nan")                # (what lies beside the rows is none of theirs)
+    teacher = make_logits(rows, width, F32, seed=width + 1).to(DEV)
+    top = L.top_rows(teacher, 8, temperature=2.0)
+    counts = torch.full((rows,), width - 1, dtype=torch.int32, device=DEV)
+    weight, up = torch.rand(rows, generator=rng(1)).to(DEV), torch.randn(rows, generator=rng(2)).to(DEV)
+    hooks = (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.clone()),
+             torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t))
+
+    def gradient(view):
+        leaf = whole.detach().clone().requires_grad_(True)
+        loss = L.distill_loss(view(leaf), top, counts=counts, weight=weight, temperature=2.0, reduction="none")
+        return leaf, loss
+
+    for view in (lambda v: v[:, :width], lambda v: v[:, :width].contiguous(), lambda v: v[1:2, :width].expand(rows, width)):
+        leaf, loss = gradient(view)
+        loss.backward(up)
+        for hook in hooks:
+            with hook:
+                other, again = gradient(view)
+            assert torch.equal(again, loss)
+            again.backward(up)
+            assert torch.equal(other.grad, leaf.grad)      # (a place's slope depends on its row's sums, which the loss left, alone)
+
+
+def test_gradient_of_a_table_whose_windows_are_saved_elsewhere():
+    cand, counts, cls, kind = make_windows(300, 40, 100, 5, 9, seed=2)
+    w = L.ScoreWindows.of(*(v.to(DEV) for v in (cand, counts, cls, kind)), 5)
+    table, g = torch.randn(5, 9, generator=rng(1)).to(DEV).requires_grad_(True), torch.randn(300, 40, generator=rng(2)).to(DEV)
+    L.class_scores(table, w).backward(g)
+    want, table.grad = table.grad, None
+    for hook in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.clone())):
+        with hook:
+            out = L.class_scores(table, w)
+        out.backward(g)
+        assert torch.equal(table.grad, want)
+        table.grad = None
