@@ -836,8 +836,8 @@ class Trainer:
         try:
             return self._step(real_padded, epoch, save_dir)
         finally:
-            # (a gradient that was exchanged is stepped on by every rank, whatever happened behind it, so their generators
-            #  stay equal; nothing in the step reads the weights any more)
+            # (reached with a step due where something raised behind the exchange of the generator's gradient: every rank steps
+            #  on it, so their generators stay equal; nothing in the step reads the weights any more)
             if self._g_step_due:
                 self._g_step_due = False
                 torch.cuda.current_stream(self.device).wait_stream(self.raw_stream)
@@ -1197,7 +1197,7 @@ class Trainer:
                 raise
             if self.exchange:
                 self.g_reducer.reduce(True)
-            self._g_step_due = True
+                self._g_step_due = True
         early_raw = early_raw and raw_set is not None
         pen_stream = self.raw_stream if early_raw else self.side_stream
         if early_raw:
@@ -1271,8 +1271,8 @@ class Trainer:
             terms.add_raw_gradients(sign=-1.0)
         elif raw_recorded:
             terms.add_fake_gradients(sign=-1.0)
-        if self.teacher is None:
-            self.opt_G.step()
+        self._g_step_due = False      # (the generator passes of this step, which read the weights, are behind this stream's work)
+        self.opt_G.step()
         self._probe("main: step end")
         self.last.update(loss_G=loss_G.detach(), pen=loss_pen.detach())
         if self.teacher is not None:

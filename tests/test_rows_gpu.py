@@ -3,6 +3,10 @@ import pytest
 import torch
 
 from gan_amd import logits as L
+from gan_amd import train as train_cli
+from gan_amd.data import Batch
+from gan_amd.dataset import pad_data
+from gan_amd.synth import synth_aig
 from test_distill_gpu import generator, template
 from test_logits_gpu import BF16, F16, F32, check_sample, make_logits, make_windows, rng
 from util_rows import sample_row
@@ -123,3 +127,34 @@ def test_gradient_of_a_table_whose_windows_are_saved_elsewhere():
         out.backward(g)
         assert torch.equal(table.grad, want)
         table.grad = None
+
+
+@pytest.mark.parametrize("extra", [[], ["--no-graph-capture"]])
+def test_a_step_that_raises_leaves_the_generator_alone(extra, tmp_path, monkeypatch):
+    """A skipped step is skipped for the generator too, wherever it raised; the next one moves it."""
+    graphs = [synth_aig(6, 40, 3, seed=60 + i, window=16, orientation="dataset") for i in range(2)]
+    mn, me = max(g.x.size(0) for g in graphs), max(g.edge_index.size(1) for g in graphs)
+    batch = Batch.from_data_list([pad_data(g, mn, me) for g in graphs]).to(DEV)
+    torch.save(generator(12, seed=9).state_dict(), tmp_path / "teacher.pt")
+    args = train_cli.build_parser().parse_args(["--dataset-dir", "x", "--candidate-k", "12", "--teacher-ckpt", str(tmp_path / "teacher.pt"),
+                                                "--distill-top", "4", "--n-critic", "2", "--save-every", "2"] + extra)
+    torch.manual_seed(3)
+    tr = train_cli.Trainer(args, mn, me, DEV)
+    weights = lambda: [p.detach().clone() for p in tr.G.parameters()]
+    start = weights()
+
+    def boom(*a, **k):
+        raise RuntimeError("injected failure")
+    with monkeypatch.context() as patch:
+        patch.setattr(train_cli, "validate_strict_aig", boom)          # (behind the distillation and the generator's pass)
+        with pytest.raises(RuntimeError, match="injected"):
+            tr.step(batch)
+    assert all(torch.equal(a, b) for a, b in zip(start, weights())) and not tr.opt_G.state
+    with monkeypatch.context() as patch:
+        patch.setattr(tr, "distill_loss", boom)
+        with pytest.raises(RuntimeError, match="injected"):
+            tr.step(batch)
+    assert all(torch.equal(a, b) for a, b in zip(start, weights())) and not tr.opt_G.state
+    tr.step(batch)
+    assert any(not torch.equal(a, b) for a, b in zip(start, weights()))
+    assert all(int(v["step"]) == 1 for v in tr.opt_G.state.values())
