@@ -8,7 +8,8 @@ step raised still takes part in the collective - the reference's catch-and-conti
 (train.py:349-352) would otherwise leave the other ranks waiting forever.  The flag is used on the
 device (the gradient becomes the mean over the ranks that had one), never read by the host: a host
 read per critic iteration would stop the host from enqueueing ahead of the GPU.  The generator has
-no gradient (see gan_amd/generator.py), hence no second collective.
+no gradient of the adversarial loss (see gan_amd/generator.py), hence no second collective - unless it learns from
+a teacher: its gradient then goes out the same way, once per step.
 """
 from __future__ import annotations
 

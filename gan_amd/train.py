@@ -827,6 +827,12 @@ class Trainer:
             total = loss if total is None else total + loss
         return total
 
+    def _exchange_learned(self, ok: bool) -> None:
+        """The mean of the ranks' gradients of the generator, those that report one; the step on it is due then."""
+        if self.teacher is not None and self.exchange:
+            self.g_reducer.reduce(ok)
+            self._g_step_due = True
+
     def _as_set(self, templates: List[Data]) -> bool:
         """The graphs of the minibatch go through the generator and the constraint kernels as one set when
         they all have the padded node count (the reference's default: templates keep their padding)."""
@@ -1008,8 +1014,13 @@ class Trainer:
         alphas = zs = None
         raw_set = loss_pen = raw_loaded = None
         if early_raw:
-            alphas = [self.draw_alpha() for _ in range(a.n_critic)]
-            zs = [self.draw_z() for _ in templates]
+            try:
+                alphas = [self.draw_alpha() for _ in range(a.n_critic)]
+                zs = [self.draw_z() for _ in templates]
+            except Exception as e:
+                if not self.exchange:
+                    raise
+                failed = e
             step_start = torch.cuda.Event()
             step_start.record(main_stream)       # (what the third stream writes was last read before this point)
         raw_from = min(1, a.n_critic - 1)    # from this iteration on the second stream belongs to the raw graphs
@@ -1173,31 +1184,25 @@ class Trainer:
                 if not self.exchange:
                     raise
                 failed = e
-        if failed is not None:
-            if self.teacher is not None and self.exchange:
-                self.g_reducer.reduce(False)
-                self._g_step_due = True
-            raise failed
-        self._edges_last = edges_fake + edges_real
+        # A gradient of the generator's own (extension: a teacher) is exchanged too, by every rank, whatever raised in
+        # front of it or in making it.
+        learned = None
+        try:
+            if failed is not None:
+                raise failed
+            self._edges_last = edges_fake + edges_real
 
-        # ---- generator (train.py:275-299); its output carries no gradient, so backward only touches D
-        self._mark("critic done")
-        self.opt_G.zero_grad()
-        if zs is None:
-            zs = [self.draw_z() for _ in templates]
-        if self.teacher is not None:      # (extension) the one term that reaches the generator
-            learned = None
-            try:
+            # ---- generator (train.py:275-299); its output carries no gradient, so backward only touches D
+            self._mark("critic done")
+            self.opt_G.zero_grad()
+            if zs is None:
+                zs = [self.draw_z() for _ in templates]
+            if self.teacher is not None:      # the one term that reaches the generator
                 learned = self.distill_loss(templates, zs)
-            except Exception:
-                if not self.exchange:
-                    raise
-                self.g_reducer.reduce(False)
-                self._g_step_due = True
-                raise
-            if self.exchange:
-                self.g_reducer.reduce(True)
-                self._g_step_due = True
+        except Exception:
+            self._exchange_learned(False)
+            raise
+        self._exchange_learned(True)
         early_raw = early_raw and raw_set is not None
         pen_stream = self.raw_stream if early_raw else self.side_stream
         if early_raw:

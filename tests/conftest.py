@@ -68,6 +68,31 @@ def _start_rccl_bench():
                   out_path, log_path)
 
 
+DP_TEACHER = None      # (process, result path, log path) of tests/dp_teacher.py, see pytest_configure
+
+
+def _start_dp_teacher():
+    """Two data-parallel ranks of a training step with a teacher, started like the rehearsal and after what runs in
+    front of it has ended; tests/test_parallel_teacher_gpu.py checks what it wrote."""
+    import socket
+    import subprocess
+    import tempfile
+    global DP_TEACHER
+    tmp = tempfile.mkdtemp(prefix="aig_dpt_")
+    out_path, log_path = os.path.join(tmp, "dp.json"), os.path.join(tmp, "dp.log")
+    keep = os.path.join(ROOT, "gpurun_out")
+    if os.path.isdir(keep) and os.access(keep, os.W_OK):
+        log_path = os.path.join(keep, "dp_teacher.log")
+    with socket.socket() as sock:
+        sock.bind(("127.0.0.1", 0))
+        port = sock.getsockname()[1]
+    env = dict(os.environ)
+    env.update(AIG_DIST_BACKEND="gloo", HSA_ENABLE_IPC_MODE_LEGACY="0", OMP_NUM_THREADS="4")
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr",
+           "127.0.0.1", "--master-port", str(port), os.path.join(ROOT, "tests", "dp_teacher.py"), out_path]
+    DP_TEACHER = (subprocess.Popen(cmd, env=env, stdout=open(log_path, "w"), stderr=subprocess.STDOUT, cwd=ROOT), out_path, log_path)
+
+
 WATCH = {"test": None, "since": 0.0, "trainer": None, "reported": None}
 
 
@@ -155,6 +180,16 @@ def pytest_configure(config):
                 RCCL_BENCH[0].wait(timeout=240)
             except subprocess.TimeoutExpired:
                 pass      # tests/test_parallel_gpu.py reports it
+    # (collected on its own, too: the file names what it needs)
+    teacher = all("test_" not in os.path.basename(a.split("::")[0]) for a in config.args) or "test_parallel_teacher_gpu" in names
+    ended = all(job is None or job[0].poll() is not None for job in (DP_REHEARSAL, RCCL_BENCH))
+    if wants_gpu and teacher and ended and torch.cuda.device_count() > 0 and os.environ.get("RANK") is None:
+        import subprocess
+        _start_dp_teacher()
+        try:
+            DP_TEACHER[0].wait(timeout=120)
+        except subprocess.TimeoutExpired:
+            pass          # tests/test_parallel_teacher_gpu.py reports it
     if wants_gpu and torch.cuda.device_count() > 0:
         _start_step_watchdog()
 
