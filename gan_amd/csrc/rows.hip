@@ -1557,8 +1557,8 @@ using namespace aig;
 
 int aig::check_row_limits(const char* what, int64_t rows, int64_t width) {
     if (width > AIG_ROWS_MAX_WIDTH) return fail(AIG_ELIMIT, "%s: rows of %lld: at most %d", what, (long long)width, AIG_ROWS_MAX_WIDTH);
-    // (a launch has fewer than 2^32 threads: a wave a row, a workgroup of 1024 for rows beyond a wave's registers)
-    const int64_t most = width <= rows::NARROW ? (1ll << 26) - 1 : (1ll << 22) - 1;
+    // (a launch has fewer than 2^32 threads: a wave a row, four of them a workgroup; one of 1024 for rows beyond a wave's registers)
+    const int64_t most = width <= rows::NARROW ? (1ll << 26) - 4 : (1ll << 22) - 1;
     if (rows > most) return fail(AIG_ELIMIT, "%s: %lld rows of %lld: at most %lld", what, (long long)rows, (long long)width, (long long)most);
     return AIG_OK;
 }

@@ -171,6 +171,14 @@ static int lanes_a_row(int64_t width, int per_lane, int most) {
     return bits;
 }
 
+// a launch has fewer than 2^32 threads
+static int check_launch(const char* what, const aig_score_windows* w, int64_t blocks, int64_t threads) {
+    if (blocks * threads >= (1ll << 32))
+        return fail(AIG_ELIMIT, "%s: %lld rows of %lld take %lld threads: fewer than 2^32 fit a launch", what, (long long)w->rows,
+                    (long long)w->width, (long long)(blocks * threads));
+    return AIG_OK;
+}
+
 extern "C" int aig_class_scores(const aig_score_windows* w, const float* table, float* out, void* stream) {
     if (const int rc = check_windows("aig_class_scores", w)) return rc;
     if (w->rows == 0) return AIG_OK;
@@ -178,7 +186,9 @@ extern "C" int aig_class_scores(const aig_score_windows* w, const float* table, 
     const bool vec = w->width % 4 == 0 && aligned16(w->cand) && aligned16(out);
     const int bits = lanes_a_row(w->width, vec ? 4 : 1, 8);
     const int64_t per_block = 256 >> bits;
-    const dim3 grid((unsigned)((w->rows + per_block - 1) / per_block));
+    const int64_t blocks = (w->rows + per_block - 1) / per_block;
+    if (const int rc = check_launch("aig_class_scores", w, blocks, 256)) return rc;
+    const dim3 grid((unsigned)blocks);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (vec) hipLaunchKernelGGL(k_class_scores<4>, grid, dim3(256), 0, s, windows_of(w), bits, table, out);
     else hipLaunchKernelGGL(k_class_scores<1>, grid, dim3(256), 0, s, windows_of(w), bits, table, out);
@@ -193,17 +203,19 @@ extern "C" size_t aig_class_scores_bwd_ws_bytes(int64_t rows, int64_t width, int
 
 extern "C" int aig_class_scores_bwd(const aig_score_windows* w, const float* grad, float* d_table, void* ws, size_t ws_bytes, void* stream) {
     if (const int rc = check_windows("aig_class_scores_bwd", w)) return rc;
+    const int run = run_rows(w->width), threads = w->classes <= 128 ? 256 : w->classes <= 512 ? 64 : 32;      // columns of at most 128 KB
+    const int64_t blocks = (w->rows + run - 1) / run;
+    if (const int rc = check_launch("aig_class_scores_bwd", w, blocks, threads)) return rc;
     AIG_REQUIRE(d_table && (w->rows == 0 || (grad && w->by_kind)) && w->kind_start, "aig_class_scores_bwd: null pointer");
     if (!ws || ws_bytes < aig_class_scores_bwd_ws_bytes(w->rows, w->width, w->kinds, w->classes))
         return fail(AIG_EWORKSPACE, "aig_class_scores_bwd: workspace of %zu bytes is too small", ws_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
     double* partial = static_cast<double*>(ws);
-    const int run = run_rows(w->width), threads = w->classes <= 128 ? 256 : w->classes <= 512 ? 64 : 32;      // columns of at most 128 KB
     const size_t lds = (size_t)w->classes * threads * sizeof(float);
     if (w->rows) {
         const bool vec = w->width % 4 == 0 && aligned16(w->cand) && aligned16(grad);
         const int bits = lanes_a_row(w->width, vec ? 4 : 1, threads == 256 ? 8 : threads == 64 ? 6 : 5);
-        const dim3 grid((unsigned)((w->rows + run - 1) / run));
+        const dim3 grid((unsigned)blocks);
         AIG_HIP_CHECK(ensure_dynamic_lds(vec ? reinterpret_cast<const void*>(k_class_scores_bwd<4>) : reinterpret_cast<const void*>(k_class_scores_bwd<1>), lds));
         if (vec) hipLaunchKernelGGL(k_class_scores_bwd<4>, grid, dim3(threads), lds, s, windows_of(w), run, bits, grad, partial);
         else hipLaunchKernelGGL(k_class_scores_bwd<1>, grid, dim3(threads), lds, s, windows_of(w), run, bits, grad, partial);

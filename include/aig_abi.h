@@ -667,7 +667,7 @@ int aig_pad_batch(int64_t B, int64_t n, int64_t ecap, const int32_t* ecount, con
  * valid (counts NULL: all; a count outside 0..width is taken as the nearer bound).  A valid place holds nothing when
  * its logit is -inf; what lies past a row's count is never read as a value.  Widths to AIG_ROWS_MAX_WIDTH; rows of up
  * to 1024 places - to 2048 where there are 512 of them and more - are held in registers, wider ones are a workgroup's each;
- * at most 2^26 - 1 rows, 2^22 - 1 of more than 1024 places.
+ * at most 2^26 - 4 rows, 2^22 - 1 of more than 1024 places.
  * The reference has none of these (its generator takes torch.topk, models/generator.py:162-168, and never receives a
  * gradient, train.py:297-299).
  * ------------------------------------------------------------------------------------------- */

@@ -1,11 +1,15 @@
 """Rows of logits: what can be checked of their entry points without a GPU."""
 import copy
+import ctypes as C
 import pickle
 
 import pytest
 import torch
 
+from gan_amd import _abi
 from gan_amd import logits as L
+
+P = C.c_void_p(4096)      # never read: every call that is given it is refused on its sizes
 
 
 def test_a_teachers_rows_are_three_tensors():
@@ -78,5 +82,27 @@ def test_saved_tensors_that_come_back_as_others_are_refused(monkeypatch, change)
     for shape in ((6, 5), (6, 2)):
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.is_floating_point() and t.shape == shape else t):
             loss = L.distill_loss(x, top, reduction="none")
-        with pytest.raises(L._abi.AigAbiError, match="saved (logits|values) must be"):
+        with pytest.raises(_abi.AigAbiError, match="saved (logits|values) must be"):
             loss.backward(torch.ones(6))
+
+
+@pytest.mark.parametrize("rows", [(1 << 26) - 3, (1 << 26) - 1])
+def test_rows_that_round_up_to_a_launch_too_large(rows):
+    """64 lanes a row and four rows a workgroup: 2^32 threads and more are not launched."""
+    how = _abi.Sampling(temperature=1.0, top_p=1.0)
+    lib = _abi.lib()
+    assert lib.aig_sample_rows(rows, 600, 600, 0, P, None, None, C.byref(how), 1, P, P, None) == -4
+    assert lib.aig_top_rows(rows, 600, 600, 0, P, None, 4, 1.0, P, P, P, None) == -4
+    a = _abi.Distill(rows=rows, width=600, ld=600, m=2, dtype=0, temperature=1.0, scale=1.0, logits=4096, values=4096, index=4096)
+    assert lib.aig_distill_rows(C.byref(a), P, None, 0, None, 0, None) == -4
+
+
+@pytest.mark.parametrize("rows,width,forth", [(600_000_000, 5, True), (2 ** 31 - 1, 2, True), (300_000_000, 9, True), (2 ** 31 - 1, 1, False)])
+def test_windows_that_take_a_launch_too_large(rows, width, forth):
+    """Fewer than 2^32 places, but a power of two of lanes a row (four of every row for the table's gradient)."""
+    a = _abi.ScoreWindowsArg(rows=rows, width=width, nodes=5, kinds=2, classes=3, cand=4096, cls=4096, row_kind=4096, by_kind=4096, kind_start=4096)
+    lib = _abi.lib()
+    if forth:
+        assert lib.aig_class_scores(C.byref(a), P, P, None) == -4
+    if rows > (1 << 30):
+        assert lib.aig_class_scores_bwd(C.byref(a), P, P, P, 1 << 50, None) == -4
