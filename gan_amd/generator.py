@@ -38,7 +38,7 @@ class GeneratorPlan:
     """Order, candidate windows and edge offsets of one template for one candidate_k."""
 
     __slots__ = ("n", "K", "E", "types", "order", "rank", "want", "cnt", "cand", "fb", "eoff", "key", "C", "cls", "x_cls",
-                 "windows")
+                 "windows", "sources")
 
     @staticmethod
     def build(x: torch.Tensor, node_depth: Optional[torch.Tensor], K: int) -> "GeneratorPlan":
@@ -171,8 +171,10 @@ class AIGGenerator(nn.Module):
         return w
 
     def plan_for(self, template: Data, x: torch.Tensor, nd: Optional[torch.Tensor]) -> GeneratorPlan:
-        """Cached on the template object; rebuilt when its tensors or candidate_k change."""
-        key = _plan_key(x, nd, int(self.candidate_k))
+        """Cached on the template object; rebuilt when its tensors or candidate_k change (``x``, ``nd``: the template's features
+        and depths, as the kernels take them)."""
+        sources = template.x, getattr(template, "node_depth", None)
+        key = _plan_key(*sources, int(self.candidate_k))
         plan = template.__dict__.get("_gen_plan")
         if plan is None or plan.key != key:
             # (a template that two generators with windows of their own take turns on - a teacher and its student - keeps
@@ -181,7 +183,8 @@ class AIGGenerator(nn.Module):
             plan = others.get(key[0])
             if plan is None or plan.key != key:
                 plan = GeneratorPlan.build(x, nd, int(self.candidate_k))
-                plan.key = key
+                # (the plan keeps the tensors that its key names: no other tensor has their addresses while it lives)
+                plan.key, plan.sources = key, sources
                 others[key[0]] = plan
             template.__dict__["_gen_plan"] = plan
         return plan

@@ -1,0 +1,63 @@
+"""Which plan a template gets (what a plan holds is made on the GPU; here it is a stand-in that remembers its features)."""
+import pytest
+import torch
+
+from gan_amd import generator as gen
+from gan_amd.data import Data
+
+
+class Plan:
+    def __init__(self, x, K):
+        self.features, self.K = x.clone(), K
+
+
+@pytest.fixture
+def made(monkeypatch):
+    plans = []
+
+    def build(x, nd, K):
+        plans.append(Plan(x, K))
+        return plans[-1]
+    monkeypatch.setattr(gen.GeneratorPlan, "build", staticmethod(build))
+    return plans
+
+
+def plan_of(G, tpl):
+    x = tpl.x if tpl.x.dtype == torch.float32 else tpl.x.float()
+    plan = G.plan_for(tpl, x, None)
+    assert torch.equal(plan.features, x) and plan.K == G.candidate_k
+    return plan
+
+
+def test_a_plan_is_kept_per_width(made):
+    wide, narrow, tpl = gen.AIGGenerator(candidate_k=8), gen.AIGGenerator(candidate_k=4), Data(x=torch.rand(30, 2))
+    first = [plan_of(G, tpl) for G in (wide, narrow)]
+    for _ in range(3):
+        assert [plan_of(G, tpl) for G in (wide, narrow)] == first
+    assert len(made) == 2
+    tpl.x.add_(1.0)
+    assert plan_of(wide, tpl) is not first[0] and plan_of(narrow, tpl) is not first[1]
+
+
+def test_features_that_take_the_place_of_others(made):
+    """Features replaced while one of two generators looks: the other does not take new ones at an old address for the old."""
+    wide, narrow, tpl = gen.AIGGenerator(candidate_k=8), gen.AIGGenerator(candidate_k=4), Data(x=torch.rand(5000, 2))
+    for k in range(20):
+        plan_of(wide, tpl), plan_of(narrow, tpl)
+        tpl.x = None
+        tpl.x = torch.rand(5000, 2)          # (often the address that has just become free)
+        plan_of(wide, tpl)
+        tpl.x = None
+        tpl.x = torch.rand(5000, 2)
+        plan_of(narrow, tpl)
+
+
+def test_features_in_another_type_are_followed(made):
+    """Changed in place: what they are converted to may well be made at the same address again."""
+    G, tpl = gen.AIGGenerator(candidate_k=8), Data(x=torch.rand(5000, 2, dtype=torch.float64))
+    kept = plan_of(G, tpl)
+    assert plan_of(G, tpl) is kept
+    for _ in range(5):
+        tpl.x.add_(1.0)
+        plan_of(G, tpl)
+
