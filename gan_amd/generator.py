@@ -178,14 +178,14 @@ class AIGGenerator(nn.Module):
         plan = template.__dict__.get("_gen_plan")
         if plan is None or plan.key != key:
             # (a template that two generators with windows of their own take turns on - a teacher and its student - keeps
-            #  a plan for each width)
-            others = template.__dict__.setdefault("_gen_plans", {})
+            #  a plan for each width; a dict that a clone of the template shares is left as it is)
+            others = template.__dict__.get("_gen_plans", {})
             plan = others.get(key[0])
             if plan is None or plan.key != key:
                 plan = GeneratorPlan.build(x, nd, int(self.candidate_k))
                 # (the plan keeps the tensors that its key names: no other tensor has their addresses while it lives)
                 plan.key, plan.sources = key, sources
-                others[key[0]] = plan
+                template.__dict__["_gen_plans"] = {**others, key[0]: plan}
             template.__dict__["_gen_plan"] = plan
         return plan
 

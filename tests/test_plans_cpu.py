@@ -61,3 +61,13 @@ def test_features_in_another_type_are_followed(made):
         tpl.x.add_(1.0)
         plan_of(G, tpl)
 
+
+def test_clones_do_not_displace_each_others_plans(made):
+    wide, narrow, tpl = gen.AIGGenerator(candidate_k=8), gen.AIGGenerator(candidate_k=4), Data(x=torch.rand(30, 2))
+    plan_of(wide, tpl), plan_of(narrow, tpl)
+    other = tpl.clone()
+    kept = [plan_of(G, t) for t in (tpl, other) for G in (wide, narrow)]
+    count = len(made)
+    for _ in range(3):
+        assert [plan_of(G, t) for t in (tpl, other) for G in (wide, narrow)] == kept
+    assert len(made) == count == 4
