@@ -88,6 +88,31 @@ class GeneratorPlan:
         return p
 
 
+class _Enqueued:
+    """What one stream has been given to make, for later calls on any: another stream waits for it as long as it may be
+    unfinished.  (A stream that is being recorded cannot wait for work in front of the recording.)"""
+
+    __slots__ = ("event", "stream")
+
+    def __init__(self, device: torch.device):
+        stream = torch.cuda.current_stream(device)
+        self.event, self.stream = torch.cuda.Event(), stream.cuda_stream
+        self.event.record(stream)
+
+    def wait(self, device: torch.device) -> None:
+        if self.event is None:
+            return
+        stream = torch.cuda.current_stream(device)
+        if torch.cuda.is_current_stream_capturing():
+            if stream.cuda_stream != self.stream:
+                raise _abi.AigAbiError("candidate windows that were just made on another stream cannot be waited for in a recording: "
+                                       "call score_windows once more, when they are finished, in front of it")
+        elif self.event.query():
+            self.event = None
+        elif stream.cuda_stream != self.stream:
+            stream.wait_event(self.event)
+
+
 CLASS_LIMIT = 1024      # distinct feature rows up to which a template is scored per class (pair tables of C x C entries)
 SELECT_FORMS_SCORES_MAX_K = 127     # windows up to which aig_gen_wire_batch takes logits = NULL with scores by class
 # ... and the slots of a call from which on that pays: the selection kernel then runs two full waves a block and forming
@@ -212,7 +237,11 @@ class AIGGenerator(nn.Module):
         alone = st["plans"][0] if len(st["plans"]) == 1 else None
         kept = st.get("windows") if alone is None else alone.windows
         if kept is not None:
-            return (*kept, st)
+            windows, weight, made = kept
+            made.wait(windows.cand.device)
+            return windows, weight, st
+        if torch.cuda.is_current_stream_capturing():
+            raise _abi.AigAbiError("candidate windows are kept, so they are made in front of a recording: call score_windows there once")
         B, n, C = len(templates), st["n"], st["C"]
         if not 0 < C <= self.TRAIN_CLASS_LIMIT:
             raise ValueError(f"candidate logits can be differentiated for templates of 1 to {self.TRAIN_CLASS_LIMIT} distinct "
@@ -225,10 +254,11 @@ class AIGGenerator(nn.Module):
         needs = (st["want"].reshape(-1) > 0) & (counts > 0)
         windows = L.ScoreWindows.of(cand.contiguous(), counts, cls.reshape(-1), kind.contiguous(), B * C)
         weight = needs.float() / needs.sum().clamp(min=1)
+        kept = windows, weight, _Enqueued(cls.device)
         if alone is None:
-            st["windows"] = (windows, weight)
+            st["windows"] = kept
         else:
-            alone.windows = (windows, weight)
+            alone.windows = kept
         return windows, weight, st
 
     def score_table(self, st, zs: torch.Tensor) -> torch.Tensor:

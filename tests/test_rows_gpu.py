@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from gan_amd import _abi
 from gan_amd import logits as L
 from gan_amd import train as train_cli
 from gan_amd.data import Batch
@@ -158,3 +159,56 @@ def test_a_step_that_raises_leaves_the_generator_alone(extra, tmp_path, monkeypa
     tr.step(batch)
     assert any(not torch.equal(a, b) for a, b in zip(start, weights()))
     assert all(int(v["step"]) == 1 for v in tr.opt_G.state.values())
+
+
+@pytest.mark.parametrize("count", [1, 3])
+def test_windows_made_on_one_stream_and_read_on_another(count):
+    """The second caller's stream waits for what the first caller's has been given to make."""
+    G, tpls = generator(24), [template(400, seed=70 + i) for i in range(count)]
+    z = torch.randn(count, 128, generator=rng(4)).to(DEV)
+    fresh = generator(24)
+    want = fresh.candidate_logits([t.clone() for t in tpls], z).detach()
+    G._stacked_plans(tpls, DEV)                     # (the plans themselves are there)
+    busy = torch.zeros(1 << 28, device=DEV)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(first):
+        for _ in range(60):                         # (some 30 ms)
+            busy.add_(1.0)
+        mine = G.score_windows(tpls)
+    assert not first.query()
+    with torch.cuda.stream(second), torch.no_grad():
+        theirs = G.score_windows(tpls)
+        got = G.candidate_logits(tpls, z)
+        assert theirs[0] is mine[0]
+    second.synchronize()
+    assert torch.equal(got, want)
+    again = G.candidate_logits(tpls, z).detach()
+    assert torch.equal(again, want)
+
+
+@pytest.mark.parametrize("count", [1, 2])
+def test_candidate_logits_in_a_recording(count):
+    """Windows are made in front of a recording; what is recorded then follows z."""
+    G, tpls = generator(24), [template(60, seed=80 + i) for i in range(count)]
+    z = torch.randn(count, 128, generator=rng(5)).to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    G._stacked_plans(tpls, DEV)
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+            with pytest.raises(_abi.AigAbiError, match="in front of a recording"):
+                G.score_windows(tpls)
+            kept = z * 2.0
+        for _ in range(2):
+            G.candidate_logits(tpls, z)
+            torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+            got = G.candidate_logits(tpls, z)
+        for k in range(3):
+            z.copy_(torch.randn(count, 128, generator=rng(6 + k)))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, G.candidate_logits(tpls, z)), k
