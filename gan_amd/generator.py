@@ -249,7 +249,8 @@ class AIGGenerator(nn.Module):
         cls, order = st["cls"].reshape(B, n), st["order"].reshape(B, n).long()
         graph = torch.arange(B, device=cls.device, dtype=torch.int32)[:, None]
         kind = (cls.gather(1, order) + graph * C).reshape(-1)
-        cand = (st["cand"].reshape(B, n, -1) + (graph * n)[:, :, None]).reshape(B * n, -1)
+        # (one template: its plan's own)
+        cand = st["cand"][:n] if B == 1 else (st["cand"].reshape(B, n, -1) + (graph * n)[:, :, None]).reshape(B * n, -1)
         counts = st["cnt"].reshape(-1)
         needs = (st["want"].reshape(-1) > 0) & (counts > 0)
         windows = L.ScoreWindows.of(cand.contiguous(), counts, cls.reshape(-1), kind.contiguous(), B * C)

@@ -212,3 +212,18 @@ def test_candidate_logits_in_a_recording(count):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, G.candidate_logits(tpls, z)), k
+
+
+def test_windows_of_one_template_hold_no_second_copy_of_its_candidates():
+    G, a, b = generator(24), template(60, seed=1), template(60, seed=2)
+    plan = G.plan_for(a, a.x, a.node_depth)
+    windows = G.score_windows([a])[0]
+    assert windows.cand.data_ptr() == plan.cand.data_ptr() and windows.cand.shape == (plan.n, 24)
+    both = G.score_windows([a, b])[0].cand
+    other = G.score_windows([b])[0].cand
+    for r in range(plan.n):                     # (past a row's count a window holds whatever it did)
+        k = int(plan.cnt[r])
+        assert torch.equal(both[r, :k], windows.cand[r, :k])
+    cnt = G.plan_for(b, b.x, b.node_depth).cnt
+    for r in range(plan.n):
+        assert torch.equal(both[plan.n + r, :cnt[r]], other[r, :cnt[r]] + plan.n)
