@@ -40,11 +40,13 @@ __device__ __forceinline__ float probability(double log2_q) { return log2_q > 0.
 // a sum over the rest of a row that is below this beside the row's largest place is taken again beside its own largest
 constexpr double FAINT = 1e-30;
 
-// A listed entry's probability is added to its place in LDS as a whole number of 2^-30, at least one: entries that name one
-// place twice add up to the same bits in any order, and a place is listed where the sum is not 0.  Only entries that repeat a
-// place can add up to the 4 that 32 bits do not hold: where a row's entries come near it, they are added again in steps of
-// 2^-23 (256 of them reach 2^31).
-constexpr float Q_UNIT = 1073741824.0f, Q_COARSE = 8388608.0f;
+// A listed entry's probability is added to its place in LDS as a whole number of 2^-30, shifted up by one, or as 1 where that
+// number is 0: entries that name one place twice add up to the same bits in any order, a place is listed where the sum is not
+// 0, and an entry without probability (a masked place of the teacher's) adds none.  Only entries that repeat a place can add up
+// to the 2 that 31 bits do not hold: where a row's entries come near it, they are added again in steps that their sum fits.
+// (An entry is off by half a step, 256 of them by 4 half steps of f32 of the sum at most.)
+constexpr float Q_UNIT = 1073741824.0f;
+__device__ __forceinline__ unsigned units_of(float q, float unit) { return max((unsigned)__float2int_rn(q * unit) << 1, 1u); }
 
 // A group of lanes per row, the row in registers, its listed places in LDS: the logits are read once, the gradient written once.
 // Loss and gradient of 1,000,000 x 64 f32 with 8 entries each: 588 MB in 135 us, 4.4 TB/s, where a large copy moves 4.6: bound by
@@ -106,7 +108,7 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
         const double lq = (double)t * a.per - lse;
         const float q = probability(lq);
         sum_q += NAMED + (double)q;
-        if (GRAD) atomicAdd(&listed[i], max((unsigned)__float2int_rn(q * Q_UNIT), 1u));
+        if (GRAD) atomicAdd(&listed[i], units_of(q, Q_UNIT));
         else listed[i] = 1u;
         if (LOSS) l += q > 0.0f ? (double)q * (lq - ((double)lv[i] - (double)base) * a.per) : q == 0.0f ? 0.0 : (double)q;
     };
@@ -116,17 +118,16 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
     const bool live = z != 0.0 && sum_q != 0.0;        // (a NaN among the logits is not nothing: it shows in the loss)
     sum_q -= NAMED * __builtin_floor(sum_q * (1.0 / NAMED));
     float q_step = 1.0f / Q_UNIT;
-    if (GRAD && sum_q >= 3.5) {
-        q_step = 1.0f / Q_COARSE;
+    if (GRAD && sum_q >= 1.75) {
+        const int e2 = __builtin_amdgcn_frexp_exp((float)sum_q);      // (the sum is below 2^e2, which is at most 512)
+        q_step = ldexpf(1.0f, e2 - 30);
 #pragma unroll
         for (int e = 0; e < E; ++e) listed[lane * E + e] = 0;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
         for (int j = lane; j < a.m; j += G)
-            if (names(index[j], values[j], n)) {
-                const float q = probability((double)values[j] * a.per - lse);
-                atomicAdd(&listed[index[j]], max((unsigned)__float2int_rn(q * Q_COARSE), 1u));
-            }
+            if (names(index[j], values[j], n))
+                atomicAdd(&listed[index[j]], units_of(probability((double)values[j] * a.per - lse), ldexpf(1.0f, 30 - e2)));
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(256) void k_distill(const T* __restrict__ x, T* __r
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             float d = faint && !q_here[e] ? exp2_fast((v[e] - rest_top) * per) : ex[e];
-            d = q_here[e] ? (float)q_here[e] * q_step : d * outside;
+            d = q_here[e] ? (float)(q_here[e] >> 1) * q_step : d * outside;
             g[e] = from_float<T>(lane * E + e < n && live ? c * (ex[e] * full - d) : 0.0f);
         }
         grad += r * a.grad_ld;

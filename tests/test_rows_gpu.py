@@ -9,7 +9,7 @@ from gan_amd.data import Batch
 from gan_amd.dataset import pad_data
 from gan_amd.synth import synth_aig
 from test_distill_gpu import generator, template
-from test_logits_gpu import BF16, F16, F32, check_sample, make_logits, make_windows, rng
+from test_logits_gpu import BF16, F16, F32, check_distill, check_sample, make_logits, make_windows, rng
 from util_rows import sample_row
 
 pytestmark = pytest.mark.gpu
@@ -227,3 +227,36 @@ def test_windows_of_one_template_hold_no_second_copy_of_its_candidates():
     cnt = G.plan_for(b, b.x, b.node_depth).cnt
     for r in range(plan.n):
         assert torch.equal(both[plan.n + r, :cnt[r]], other[r, :cnt[r]] + plan.n)
+
+
+@pytest.mark.parametrize("rows,width", [(6, 7), (6, 16), (6, 60), (6, 200), (6, 500), (6, 1000), (6, 1500), (530, 2000)])
+def test_listed_places_without_probability(rows, width):
+    """A teacher's masked places that are listed all the same: they are not of the rest, and a student's masked place has no
+    gradient."""
+    low = torch.finfo(F32).min
+    x = make_logits(rows, width, F32, seed=width)
+    i = torch.arange(6, dtype=torch.int32).expand(rows, 6).contiguous()
+    v = x[:, :6] + 0.5 * torch.randn(rows, 6, generator=rng(2))
+    x[:, 3:5], v[:, 3:5] = low, low
+    v[:, 5] = -200.0                              # no probability, but a student's that is not masked
+    s = torch.logsumexp(v.double() / 1.5, 1).float() + 0.5
+    for lse in (s, None):
+        _, grad = check_distill(x[:8], v[:8], i[:8], None if lse is None else lse[:8], 1.5)
+        assert not grad[:, 3:5].any()
+    _, grad = L.distill_loss_and_grad(x.to(DEV), L.TopRows(v.to(DEV), i.to(DEV), s.to(DEV)), temperature=1.5)
+    assert not grad[:, 3:5].any() and grad[:, 5].all()
+
+
+@pytest.mark.parametrize("width", [5, 48, 200, 500, 1000, 1500])
+def test_probabilities_of_many_entries_of_one_place_add_up(width):
+    """256 entries whose probabilities lie between the steps of 2^-23: their sum is not off by 256 half steps."""
+    x = make_logits(4, width, F32, seed=width)
+    i = torch.full((4, 256), 3, dtype=torch.int32)
+    q = (torch.arange(92000, 92004).double()[:, None] + torch.tensor([0.45, 0.48, 0.49, 0.47]).double()[:, None]) * 2.0 ** -23
+    v = torch.log(q).expand(4, 256).float().clone()
+    v[:, 0] = 0.0
+    v[:, 1] = 0.0
+    i[:, 1] = 1
+    s = torch.zeros(4)
+    check_distill(x, v, i, s, 1.0)
+    check_distill(x, v, i, None, 1.0)
