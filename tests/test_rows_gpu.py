@@ -62,10 +62,10 @@ def test_min_p_is_compared_with_weights_in_whole_units(rows, width):
         check_sample(x, u, counts=counts, min_p=share, top_k=5)
 
 
-@pytest.mark.parametrize("K", [8, 40, 300])
-def test_fan_ins_drawn_at_a_low_temperature(K):
+@pytest.mark.parametrize("K,n_and", [(8, 150), (40, 150), (300, 150), (700, 1100), (1024, 1600)])
+def test_fan_ins_drawn_at_a_low_temperature(K, n_and):
     """A slot's second fan-in is its second draw, however little of the weight that has."""
-    G, tpl = generator(K, seed=3), template(150, seed=4)
+    G, tpl = generator(K, seed=3), template(n_and, seed=4)
     n, g = tpl.x.size(0), rng(K)
     z, u = torch.randn(128, generator=g).to(DEV), torch.rand(n, 2, generator=g).to(DEV)
     logits = G(tpl, z, return_debug=True, sampling=L.Sampling(), u=u)._debug["logits"].cpu().double()
