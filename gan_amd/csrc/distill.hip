@@ -49,7 +49,7 @@ constexpr float Q_UNIT = 1073741824.0f;
 __device__ __forceinline__ unsigned units_of(float q, float unit) { return max((unsigned)__float2int_rn(q * unit) << 1, 1u); }
 
 // A group of lanes per row, the row in registers, its listed places in LDS: the logits are read once, the gradient written once.
-// Loss and gradient of 1,000,000 x 64 f32 with 8 entries each: 588 MB in 135 us, 4.4 TB/s, where a large copy moves 4.6: bound by
+// Loss and gradient of 1,000,000 x 64 f32 with 8 entries each: 588 MB in 119 to 127 us, where a large copy takes 128: bound by
 // memory.  26,279 x 512 bf16 with 32 entries: loss 21 us (34 MB, 1.6 TB/s), gradient 23.5 us (60 MB, 2.6 TB/s): bound by the
 // latency of a row's chain - load, largest, sum, entries, rest - at eight waves a SIMD.  243 x 16: 2.8 us, a launch.
 template <typename T, int G, int E, bool LOSS, bool GRAD>
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(WIDE_T) void k_distill_wide(const T* __restrict__ x
         }
     }
     typename Span<T>::Batch ahead{};
-    if (LOSS) ahead = row.fetch(t, WIDE_T);       // (on its way under the entries' sums; a gradient alone has no pass to read it for)
+    if (LOSS) ahead = row.fetch(t, WIDE_T);       // (on its way under the entries' sums; a gradient alone reads the row behind them)
     __syncthreads();
     if (i_mine >= 0) atomicOr(&bits[(i_mine + pad) >> 5], 1u << ((i_mine + pad) & 31));
     double lse;

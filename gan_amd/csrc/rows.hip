@@ -167,7 +167,10 @@ __device__ __forceinline__ void exact_draws(const SampleRows& a, const RowSettin
 // average of d over the weights of 1024 places is at most 6.5 (2048: 7.2); a sum of 16 (32) in a lane rounds by half of as many
 // such steps of the lane's, the six steps over the lanes by six of the total: 0.8e-6 + 0.1e-6 + 0.8e-6 (0.9 + 0.1 + 1.3).  A
 // decision between two numbers that lie further apart than margin_of of the total is therefore the exact one; a row with a
-// closer one is drawn again in f64 (returns false): one in a hundred, mostly for top-p's border among places of small weight.
+// closer one is drawn again in f64 (returns false).  So is a min-p within half a unit of 2^-36 of a weight, and a draw that finds no
+// weight left in the sums while a place still has some.  How many rows that is, of normal logits of deviation 2 at T 0.8, two
+// draws: under top-p 0.9 0.1 % of 64 places, 0.3 % of 256, 1 % of 1,024, 4 % of 2,000; under top-p 0.99 0.7, 3, 12 and 46 % (the
+// border lies among places of small weight); of 64 places without filters 0.1 %, at T 0.1 26 % (the second draw does).
 // What that buys: an f64 exponential alone is 26 instructions a place, and sums in f32 take their lane permutations along.
 template <int PLACES> __device__ __host__ constexpr float margin_of() { return PLACES <= 1024 ? 1.0f / 262144.0f : 1.0f / 131072.0f; }
 
@@ -474,9 +477,9 @@ __device__ __forceinline__ bool quick_draws(const SampleRows& a, const RowSettin
 }
 
 // A group of G lanes per row, the row in registers: read once, 8 bytes a draw written.  Bound by the issue of vector
-// instructions, not by memory: 100,000 x 64 under top-k 32, top-p 0.9 and min-p (sorted whole: 300 of 878 instructions a wave)
-// 22.7 us, of which 18 are issue; 27 MB would be copied in 6.  Without filters 8.8 us.  152,896 x 256 under top-p 0.9 63 us,
-// 59 of them issue of 952 instructions a wave (157 MB: 35).  One row 4.7 us: a chain of lane exchanges.
+// instructions, not by memory: 100,000 x 64 under top-k 32, top-p 0.9 and min-p (sorted whole: 300 of 877 instructions a wave)
+// 22.9 us, of which 18 are issue; 27 MB would be copied in 6.  Without filters, all places valid, 9.7 us.  152,896 x 256 under
+// top-p 0.9 64 us, 60 of them issue of 983 instructions a wave (157 MB: 35).  One row 4.4 us: a chain of lane exchanges.
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void k_sample(const T* __restrict__ x, SampleRows a) {
     __shared__ __attribute__((aligned(16))) float lds[E > 4 ? 256 / G : 1][E > 4 ? G * E : 1];
@@ -969,7 +972,7 @@ __device__ __forceinline__ void list_with_ties(const Span<T>& row, const Parts<T
 //   then the sum of what stays in each part of the row, and for each draw a look through the one part that holds it.
 // Rows are as many as a batch has requests, so most CUs idle; what a row costs is its CU's time: 48 x 50,001 bf16 under top-k
 // 50 and top-p 15 us (two reads of 100 KB, two lists sorted), top-k 500 27 us; under top-p alone 45 us, two f64
-// exponentials a place, and 69 us for 512 rows of 32,001 (two a CU); 150 rows of 131,072 under a top-k
+// exponentials a place, and 70 us for 512 rows of 32,001 (two a CU); 150 rows of 131,072 under a top-k
 // beyond LIST_K 700 us (general_draws).
 constexpr int BINS = 4096;
 constexpr float OCTAVES = 37.0f;          // a weight under 2^-37 is 0
@@ -1196,7 +1199,7 @@ __global__ __launch_bounds__(WIDE_T) void k_sample_wide(const T* __restrict__ x,
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int b = bin_of(v[j]);
-                // (without branches: as a chain of || this compiler left the assignment of 0 out)
+                // (selections, no branches; a chain of || gives the same picks)
                 const bool stays = (b < border_bin) | ((b == border_bin) & (with_place(key_of(v[j]), at + j) >= edge));
                 const double w = weight(v[j]);
                 bool taken = j >= here;

@@ -64,7 +64,9 @@ __global__ __launch_bounds__(256) void k_class_scores(Windows w, int lpr_bits, c
 // Rows in the order of their kinds are dealt to blocks in runs of RUN; a run may hold rows of several kinds.  A block adds
 // the gradients of one kind's rows into private columns acc[class][thread] in LDS - a thread's own additions, in order, no
 // atomics - sums the columns in a fixed order in f64 when the kind ends, and writes the sum as partial number (block +
-// kind): no two (block, kind) pairs that occur share it.
+// kind): no two (block, kind) pairs that occur share it.  A column is f32: a thread adds some 16 values of a run for rows
+// to 512 places and width / 32 for wider ones (4,096 at 131,072; with more than 128 classes, on fewer threads, as many times more),
+// each addition off by half a step at most; 256 columns of 128 classes in f64 would not fit LDS.
 // A run holds about 4096 places: enough that the columns' sums at its end weigh little, few enough that there are several
 // blocks for every CU.  100,000 x 64, 9 kinds of 9 classes: 51 MB in 22 us (2.3 TB/s); 26,279 x 512, 99 kinds: 108 MB in 34 us
 // (3.2 TB/s): the dependent trip from candidate to class, and a read-add-write of LDS a place.

@@ -799,7 +799,9 @@ class Trainer:
     def distill_loss(self, templates: List[Data], zs: List[torch.Tensor]) -> torch.Tensor:
         """Adds the gradient of ``distill_weight`` times the distillation loss of the teacher's top candidate logits - the
         mean over the slots that need a fan-in, over the graphs - to the generator's parameters and returns the loss (a
-        device scalar, no host read).  Graphs of one node count go through together."""
+        device scalar, no host read).  Graphs of one node count go through together.  A teacher with another window has
+        candidates that are none of the student's, and the other way round: its listed logits inside the student's window are
+        normalised over themselves then, and what is not listed is left out of the loss."""
         a, by_size = self.args, OrderedDict()
         for t, z in zip(templates, zs):
             by_size.setdefault(int(t.x.size(0)), []).append((t, z))
@@ -1404,7 +1406,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--teacher-ckpt", type=str, default=None,
                    help="generator state dict (.pt) of a teacher: the generator learns its candidate logits by distillation (without "
                         "one it never moves: the adversarial loss gives it no gradient)")
-    p.add_argument("--teacher-candidate-k", type=int, default=None, help="the teacher's window (default: --candidate-k)")
+    p.add_argument("--teacher-candidate-k", type=int, default=None, help="the teacher's window (default: --candidate-k).  With another one the loss compares the "
+                        "teacher's listed logits that lie in both windows, normalised over themselves; only with the same window does "
+                        "it hold the rest of the teacher's probability as well")
     p.add_argument("--distill-top", type=int, default=16, help="largest logits a slot that are taken of the teacher (1 to 256)")
     p.add_argument("--distill-temperature", type=float, default=2.0)
     p.add_argument("--distill-weight", type=float, default=1.0)

@@ -749,7 +749,8 @@ int aig_sum_rows(int64_t rows, const float* v, float factor, float* out, void* w
 /* Candidate logits by class (nodes with equal feature rows score alike, see aig_gen_wire_set.cls) as a lookup that can be
  * differentiated:  out[r*width + i] = table[row_kind[r]*classes + cls[cand[r*width + i]]]  for i < counts[r], -inf past it
  * and for a candidate, class or kind outside its range;  d_table[k][c] = sum of grad over the rows of kind k and their
- * places of class c, in f64 per block and in a fixed order (no atomics).
+ * places of class c, in a fixed order (no atomics): a thread's values of a run of rows in f32, everything behind
+ * that in f64.
  *   by_kind [rows]: the rows in the order of their kinds; kind_start [kinds+1]: where each kind begins in it (both for the
  *   gradient only) */
 typedef struct aig_score_windows {
