@@ -112,6 +112,17 @@ class _Enqueued:
         elif stream.cuda_stream != self.stream:
             stream.wait_event(self.event)
 
+    def __reduce__(self):          # (a template that is copied or pickled takes its plan along: when the work is done)
+        if self.event is not None:
+            self.event.synchronize()
+        return _finished, ()
+
+
+def _finished() -> "_Enqueued":
+    made = object.__new__(_Enqueued)
+    made.event, made.stream = None, 0
+    return made
+
 
 CLASS_LIMIT = 1024      # distinct feature rows up to which a template is scored per class (pair tables of C x C entries)
 SELECT_FORMS_SCORES_MAX_K = 127     # windows up to which aig_gen_wire_batch takes logits = NULL with scores by class

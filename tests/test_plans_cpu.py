@@ -1,4 +1,7 @@
 """Which plan a template gets (what a plan holds is made on the GPU; here it is a stand-in that remembers its features)."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -71,3 +74,26 @@ def test_clones_do_not_displace_each_others_plans(made):
     for _ in range(3):
         assert [plan_of(G, t) for t in (tpl, other) for G in (wide, narrow)] == kept
     assert len(made) == count == 4
+
+
+def test_a_plan_with_windows_can_be_copied_and_pickled():
+    """What was enqueued is waited for; the copy has nothing to wait for."""
+    class Event:
+        waited = 0
+
+        def synchronize(self):
+            Event.waited += 1
+
+        def __reduce__(self):
+            raise TypeError("an event is not copied")
+    plan = gen.GeneratorPlan()
+    made = object.__new__(gen._Enqueued)
+    made.event, made.stream = Event(), 7
+    plan.windows, plan.K = (torch.zeros(3), torch.ones(3), made), 8
+    tpl = Data(x=torch.rand(4, 2))
+    tpl.__dict__["_gen_plan"] = plan
+    for other in (copy.deepcopy(tpl), pickle.loads(pickle.dumps(tpl)), copy.copy(tpl)):
+        kept = other.__dict__["_gen_plan"].windows[2]
+        kept.wait(torch.device("cpu")) if kept is not made else None
+        assert torch.equal(other.__dict__["_gen_plan"].windows[1], torch.ones(3))
+    assert Event.waited == 2 and made.event is not None

@@ -1,4 +1,6 @@
 """Rows of logits: calls that their operators once answered wrongly, against definitions in 64 bits."""
+import copy
+
 import pytest
 import torch
 
@@ -260,3 +262,10 @@ def test_probabilities_of_many_entries_of_one_place_add_up(width):
     s = torch.zeros(4)
     check_distill(x, v, i, s, 1.0)
     check_distill(x, v, i, None, 1.0)
+
+
+def test_a_template_with_windows_can_be_copied():
+    G, tpl, z = generator(24), template(60, seed=1), torch.randn(1, 128, generator=rng(2)).to(DEV)
+    want = G.candidate_logits([tpl], z).detach()
+    other = copy.deepcopy(tpl)
+    assert torch.equal(G.candidate_logits([other], z).detach(), want)
