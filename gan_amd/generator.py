@@ -137,6 +137,15 @@ def _plan_key(x: torch.Tensor, nd: Optional[torch.Tensor], K: int):
             None if nd is None else (nd.data_ptr(), nd._version, nd.dtype))
 
 
+def _made_of(plan: Optional[GeneratorPlan], key) -> bool:
+    """Is it the plan of the tensors that ``key`` names?  (The tensors that a plan keeps have the addresses of its key, unless
+    it is a copy, which keeps copies: their addresses are looked at as well.)"""
+    if plan is None or plan.key != key:
+        return False
+    x, nd = plan.sources
+    return x.data_ptr() == key[1] and (nd is None or nd.data_ptr() == key[4][0])
+
+
 class AIGGenerator(nn.Module):
     def __init__(self, node_in_dim: int = 2, hidden_dim: int = 128, z_dim: int = 128, candidate_k: int = 512,
                  device: torch.device = torch.device("cpu"), score_dtype: str = "fp32"):
@@ -212,12 +221,12 @@ class AIGGenerator(nn.Module):
         sources = template.x, getattr(template, "node_depth", None)
         key = _plan_key(*sources, int(self.candidate_k))
         plan = template.__dict__.get("_gen_plan")
-        if plan is None or plan.key != key:
+        if not _made_of(plan, key):
             # (a template that two generators with windows of their own take turns on - a teacher and its student - keeps
             #  a plan for each width; a dict that a clone of the template shares is left as it is)
             others = template.__dict__.get("_gen_plans", {})
             plan = others.get(key[0])
-            if plan is None or plan.key != key:
+            if not _made_of(plan, key):
                 plan = GeneratorPlan.build(x, nd, int(self.candidate_k))
                 # (the plan keeps the tensors that its key names: no other tensor has their addresses while it lives)
                 plan.key, plan.sources = key, sources

@@ -97,3 +97,16 @@ def test_a_plan_with_windows_can_be_copied_and_pickled():
         kept.wait(torch.device("cpu")) if kept is not made else None
         assert torch.equal(other.__dict__["_gen_plan"].windows[1], torch.ones(3))
     assert Event.waited == 2 and made.event is not None
+
+
+def test_a_copy_of_a_template_and_features_at_the_originals_address(made):
+    """A copied plan names the original's features, which its copy does not keep alive."""
+    G = gen.AIGGenerator(candidate_k=8)
+    for _ in range(20):
+        tpl = Data(x=torch.rand(5000, 2))
+        plan_of(G, tpl)
+        other = copy.deepcopy(tpl)
+        made.clear()                           # (nothing else holds the original and its plan)
+        del tpl
+        other.x = torch.rand(5000, 2)          # (often the address that has just become free)
+        plan_of(G, other)
