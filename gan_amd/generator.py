@@ -20,6 +20,7 @@ or a copy, so ``loss_G.backward()`` never reaches these parameters (train.py:297
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 C_ = C      # (inside the methods that count classes, C is a number)
 from typing import Optional
@@ -34,6 +35,14 @@ from .data import Data
 PI, PO, AND = 0, 1, 2
 
 
+@contextlib.contextmanager
+def _kept():
+    """What is made here is kept and may be trained on later, whatever mode its first caller is in (tensors that are made in
+    inference mode cannot be)."""
+    with torch.inference_mode(False), torch.no_grad():
+        yield
+
+
 class GeneratorPlan:
     """Order, candidate windows and edge offsets of one template for one candidate_k."""
 
@@ -41,6 +50,7 @@ class GeneratorPlan:
                  "windows", "sources")
 
     @staticmethod
+    @_kept()
     def build(x: torch.Tensor, node_depth: Optional[torch.Tensor], K: int) -> "GeneratorPlan":
         lib = _abi.lib()
         dev = x.device
@@ -266,15 +276,16 @@ class AIGGenerator(nn.Module):
         if not 0 < C <= self.TRAIN_CLASS_LIMIT:
             raise ValueError(f"candidate logits can be differentiated for templates of 1 to {self.TRAIN_CLASS_LIMIT} distinct "
                              f"feature rows, got {C}")
-        cls, order = st["cls"].reshape(B, n), st["order"].reshape(B, n).long()
-        graph = torch.arange(B, device=cls.device, dtype=torch.int32)[:, None]
-        kind = (cls.gather(1, order) + graph * C).reshape(-1)
-        # (one template: its plan's own)
-        cand = st["cand"][:n] if B == 1 else (st["cand"].reshape(B, n, -1) + (graph * n)[:, :, None]).reshape(B * n, -1)
-        counts = st["cnt"].reshape(-1)
-        needs = (st["want"].reshape(-1) > 0) & (counts > 0)
-        windows = L.ScoreWindows.of(cand.contiguous(), counts, cls.reshape(-1), kind.contiguous(), B * C)
-        weight = needs.float() / needs.sum().clamp(min=1)
+        with _kept():
+            cls, order = st["cls"].reshape(B, n), st["order"].reshape(B, n).long()
+            graph = torch.arange(B, device=cls.device, dtype=torch.int32)[:, None]
+            kind = (cls.gather(1, order) + graph * C).reshape(-1)
+            # (one template: its plan's own)
+            cand = st["cand"][:n] if B == 1 else (st["cand"].reshape(B, n, -1) + (graph * n)[:, :, None]).reshape(B * n, -1)
+            counts = st["cnt"].reshape(-1)
+            needs = (st["want"].reshape(-1) > 0) & (counts > 0)
+            windows = L.ScoreWindows.of(cand.contiguous(), counts, cls.reshape(-1), kind.contiguous(), B * C)
+            weight = needs.float() / needs.sum().clamp(min=1)
         kept = windows, weight, _Enqueued(cls.device)
         if alone is None:
             st["windows"] = kept
@@ -372,15 +383,16 @@ class AIGGenerator(nn.Module):
             st["nd"] = nds[0] if nds[0] is not None and nds[0].numel() == n else None
             st["C"], st["cls"], st["x_cls"] = plans[0].C, plans[0].cls, plans[0].x_cls
             return st
-        st = {"plans": plans, "n": n, "E": [p.E for p in plans], "x": torch.cat(xs).contiguous()}
-        # classes: every template's class rows padded to the largest class count (the padding repeats row 0)
-        C = max(p.C for p in plans)
-        st["C"] = C
-        st["cls"] = torch.stack([p.cls for p in plans]).contiguous()
-        st["x_cls"] = torch.cat([torch.cat([p.x_cls, p.x_cls[:1].expand(C - p.C, 2)]) for p in plans]).contiguous()
-        for name in ("order", "rank", "want", "cnt", "fb", "eoff", "cand"):
-            st[name] = torch.stack([getattr(p, name) for p in plans]).contiguous()
-        st["nd"] = torch.cat(nds).contiguous() if all(v is not None and v.numel() == n for v in nds) else None
+        with _kept():
+            st = {"plans": plans, "n": n, "E": [p.E for p in plans], "x": torch.cat(xs).contiguous()}
+            # classes: every template's class rows padded to the largest class count (the padding repeats row 0)
+            C = max(p.C for p in plans)
+            st["C"] = C
+            st["cls"] = torch.stack([p.cls for p in plans]).contiguous()
+            st["x_cls"] = torch.cat([torch.cat([p.x_cls, p.x_cls[:1].expand(C - p.C, 2)]) for p in plans]).contiguous()
+            for name in ("order", "rank", "want", "cnt", "fb", "eoff", "cand"):
+                st[name] = torch.stack([getattr(p, name) for p in plans]).contiguous()
+            st["nd"] = torch.cat(nds).contiguous() if all(v is not None and v.numel() == n for v in nds) else None
         if len(cache) >= 4:
             cache.pop(next(iter(cache)))
         cache[key] = st

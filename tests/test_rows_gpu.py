@@ -269,3 +269,19 @@ def test_a_template_with_windows_can_be_copied():
     want = G.candidate_logits([tpl], z).detach()
     other = copy.deepcopy(tpl)
     assert torch.equal(G.candidate_logits([other], z).detach(), want)
+
+
+@pytest.mark.parametrize("count", [1, 2])
+def test_templates_that_were_sampled_in_inference_mode_can_be_trained_on(count):
+    tpls, z = [template(50, seed=1 + i) for i in range(count)], torch.randn(count, 128, generator=rng(3)).to(DEV)
+    grads = []
+    for first in (True, False):
+        G = generator(16)
+        here = tpls if first else [t.clone() for t in tpls]
+        if first:
+            with torch.inference_mode():
+                G(here[0], z[0]), G.forward_set(here, z), G.candidate_logits(here, z)
+        G.candidate_logits(here, z).nan_to_num(neginf=0.0).square().sum().backward()
+        grads.append([p.grad for p in G.parameters()])
+    assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(*grads))
+    assert any(g is not None and g.any() for g in grads[0])
