@@ -279,6 +279,22 @@ def _check_backward(what: str) -> None:
         raise RuntimeError(f"{what} can be differentiated once: call backward without create_graph")
 
 
+def _save(ctx, tensors) -> None:
+    """Operands for the backward pass.  (Torch refuses to save what was made in inference mode, as a teacher's rows may well
+    be: that is kept beside.)"""
+    ctx.beside = None
+    for v in tensors:
+        if v is not None and v.is_inference():
+            ctx.beside = [v if v is not None and v.is_inference() else None for v in tensors]
+            tensors = [v if b is None else None for v, b in zip(tensors, ctx.beside)]
+            break
+    ctx.save_for_backward(*tensors)
+
+
+def _saved(ctx):
+    return ctx.saved_tensors if ctx.beside is None else [v if b is None else b for v, b in zip(ctx.saved_tensors, ctx.beside)]
+
+
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, arg, held, reduce):
@@ -287,14 +303,14 @@ class _DistillLoss(torch.autograd.Function):
             ctx.stats = torch.empty((arg.rows, 8), dtype=torch.float32, device=logits.device)
             arg.stats = ctx.stats.data_ptr()
         _distill(logits.device, arg, loss, None)
-        ctx.save_for_backward(logits, *held)
+        _save(ctx, (logits, *held))
         ctx.arg, ctx.stride, ctx.dtype = arg, logits.stride(), logits.dtype
         return _sum_rows(loss) if reduce else loss
 
     @staticmethod
     def backward(ctx, g):
         _check_backward("distill_loss")
-        logits, *held = ctx.saved_tensors
+        logits, *held = _saved(ctx)
         a = _abi.Distill.from_buffer_copy(ctx.arg)
         if logits.data_ptr() != a.logits or logits.stride() != ctx.stride or logits.dtype is not ctx.dtype:
             # (a hook's copy has strides of its own)
@@ -367,7 +383,7 @@ class _ClassScores(torch.autograd.Function):
     def forward(ctx, table, windows, a):
         out = torch.empty((a.rows, a.width), dtype=torch.float32, device=table.device)
         _call("aig_class_scores", table.device, C.byref(a), table.data_ptr(), out.data_ptr(), meta=(a.rows, a.width))
-        ctx.save_for_backward(*windows)
+        _save(ctx, windows)
         ctx.arg = a
         return out
 
@@ -375,7 +391,7 @@ class _ClassScores(torch.autograd.Function):
     def backward(ctx, g):
         _check_backward("class_scores")
         a = _abi.ScoreWindowsArg.from_buffer_copy(ctx.arg)
-        held = _handed_back(a, ScoreWindows._fields, ctx.saved_tensors, g.device)
+        held = _handed_back(a, ScoreWindows._fields, _saved(ctx), g.device)
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
         return _table_grad(g, a), None, None

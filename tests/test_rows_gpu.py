@@ -285,3 +285,25 @@ def test_templates_that_were_sampled_in_inference_mode_can_be_trained_on(count):
         grads.append([p.grad for p in G.parameters()])
     assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(*grads))
     assert any(g is not None and g.any() for g in grads[0])
+
+
+@pytest.mark.parametrize("width", [40, 5000])
+def test_a_teacher_that_was_asked_in_inference_mode(width):
+    x = make_logits(30, width, F32, seed=1).to(DEV).requires_grad_(True)
+    cand, counts, cls, kind = (v.to(DEV) for v in make_windows(30, width, 100, 5, 9, seed=2))
+    table = torch.randn(5, 9, generator=rng(4)).to(DEV).requires_grad_(True)
+
+    def asked():
+        teacher = make_logits(30, width, F32, seed=2).to(DEV)
+        c, weight = counts.clone(), torch.rand(30, generator=rng(3)).to(DEV)
+        return L.top_rows(teacher, 8, counts=c, temperature=2.0), c, weight, L.ScoreWindows.of(cand, c, cls, kind, 5)
+
+    grads = []
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            top, c, weight, windows = asked()
+        L.distill_loss(x, top, counts=c, weight=weight, temperature=2.0).backward()
+        L.distill_loss(L.class_scores(table, windows), top, counts=c, temperature=2.0).backward()
+        grads.append((x.grad, table.grad))
+        x.grad = table.grad = None
+    assert all(torch.equal(a, b) and a.any() for a, b in zip(*grads))
