@@ -104,23 +104,33 @@ class _Enqueued:
 
     __slots__ = ("event", "stream")
 
-    def __init__(self, device: torch.device):
+    def __init__(self, device: torch.device, tensors):
         stream = torch.cuda.current_stream(device)
         self.event, self.stream = torch.cuda.Event(), stream.cuda_stream
         self.event.record(stream)
+        self.used_on(stream, tensors)
 
-    def wait(self, device: torch.device) -> None:
-        if self.event is None:
+    @staticmethod
+    def used_on(stream, tensors) -> None:          # (a template may be let go while this stream still reads them)
+        for v in tensors:
+            if v is not None:
+                v.record_stream(stream)
+
+    def wait(self, device: torch.device, tensors) -> None:
+        """In front of a use of ``tensors`` on the current stream."""
+        stream, recorded = torch.cuda.current_stream(device), torch.cuda.is_current_stream_capturing()
+        if self.event is not None and not recorded and self.event.query():
+            self.event = None
+        if stream.cuda_stream == self.stream:
             return
-        stream = torch.cuda.current_stream(device)
-        if torch.cuda.is_current_stream_capturing():
-            if stream.cuda_stream != self.stream:
+        if recorded:
+            if self.event is not None:
                 raise _abi.AigAbiError("candidate windows that were just made on another stream cannot be waited for in a recording: "
                                        "call score_windows once more, when they are finished, in front of it")
-        elif self.event.query():
-            self.event = None
-        elif stream.cuda_stream != self.stream:
+            return
+        if self.event is not None:
             stream.wait_event(self.event)
+        self.used_on(stream, tensors)
 
     def __reduce__(self):          # (a template that is copied or pickled takes its plan along: when the work is done)
         if self.event is not None:
@@ -130,7 +140,7 @@ class _Enqueued:
 
 def _finished() -> "_Enqueued":
     made = object.__new__(_Enqueued)
-    made.event, made.stream = None, 0
+    made.event, made.stream = None, None
     return made
 
 
@@ -268,7 +278,7 @@ class AIGGenerator(nn.Module):
         kept = st.get("windows") if alone is None else alone.windows
         if kept is not None:
             windows, weight, made = kept
-            made.wait(windows.cand.device)
+            made.wait(windows.cand.device, (*windows, weight, st["x_cls"]))
             return windows, weight, st
         if torch.cuda.is_current_stream_capturing():
             raise _abi.AigAbiError("candidate windows are kept, so they are made in front of a recording: call score_windows there once")
@@ -286,7 +296,7 @@ class AIGGenerator(nn.Module):
             needs = (st["want"].reshape(-1) > 0) & (counts > 0)
             windows = L.ScoreWindows.of(cand.contiguous(), counts, cls.reshape(-1), kind.contiguous(), B * C)
             weight = needs.float() / needs.sum().clamp(min=1)
-        kept = windows, weight, _Enqueued(cls.device)
+        kept = windows, weight, _Enqueued(cls.device, (*windows, st["x_cls"]))
         if alone is None:
             st["windows"] = kept
         else:

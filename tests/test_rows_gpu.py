@@ -307,3 +307,26 @@ def test_a_teacher_that_was_asked_in_inference_mode(width):
         grads.append((x.grad, table.grad))
         x.grad = table.grad = None
     assert all(torch.equal(a, b) and a.any() for a, b in zip(*grads))
+
+
+def test_windows_that_are_let_go_while_another_stream_reads_them():
+    """Their memory is not given to others before that stream is through."""
+    G, z = generator(24), torch.randn(2, 128, generator=rng(4)).to(DEV)
+    tpls = [template(3000, seed=90 + i) for i in range(2)]
+    want = generator(24).candidate_logits([t.clone() for t in tpls], z).detach()
+    windows, weight, _ = G.score_windows(tpls)
+    sizes = {v.data_ptr(): v.numel() for v in (*windows, weight)}
+    busy = torch.zeros(1 << 28, device=DEV)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other), torch.no_grad():
+        for _ in range(60):                         # (some 30 ms)
+            busy.add_(1.0)
+        got = G.candidate_logits(tpls, z)
+    del windows, weight, tpls
+    G.__dict__["_plan_stacks"].clear()
+    mine = [torch.full((n,), -1, dtype=torch.int32, device=DEV) for n in sizes.values() for _ in range(3)]
+    assert not other.query()
+    assert not {v.data_ptr() for v in mine} & set(sizes)
+    other.synchronize()
+    assert torch.equal(got, want)
