@@ -80,9 +80,6 @@ def _start_dp_teacher():
     global DP_TEACHER
     tmp = tempfile.mkdtemp(prefix="aig_dpt_")
     out_path, log_path = os.path.join(tmp, "dp.json"), os.path.join(tmp, "dp.log")
-    keep = os.path.join(ROOT, "gpurun_out")
-    if os.path.isdir(keep) and os.access(keep, os.W_OK):
-        log_path = os.path.join(keep, "dp_teacher.log")
     with socket.socket() as sock:
         sock.bind(("127.0.0.1", 0))
         port = sock.getsockname()[1]
